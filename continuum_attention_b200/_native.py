@@ -17,6 +17,7 @@ CA_DTYPE_F32, CA_DTYPE_BF16, CA_DTYPE_F16 = 0, 1, 2
 CA_IMPL_AUTO, CA_IMPL_SIMT, CA_IMPL_TCGEN05 = 0, 1, 2
 CA_LAYOUT_BHTD, CA_LAYOUT_BTHD = 0, 1
 CA_BWD_DETERMINISTIC = 1
+CA_ROTARY_INTERLEAVED, CA_ROTARY_HALF = 0, 1
 STATUS_NAMES = {0: "CA_OK", 1: "CA_ERR_INVALID_ARGUMENT", 2: "CA_ERR_UNSUPPORTED", 3: "CA_ERR_CUDA",
                 4: "CA_ERR_WORKSPACE", 5: "CA_ERR_DEVICE_TIMEOUT"}
 
@@ -49,6 +50,13 @@ SIGNATURES = {
     "ca_add_rmsnorm_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _i64, _i64, _vp]),
     "ca_gelu_tanh_forward": (_int, [_vp, _vp, _i64, _int, _vp]),
     "ca_gelu_tanh_backward": (_int, [_vp, _vp, _vp, _i64, _int, _vp]),
+    "ca_rotary_qkv_forward": (_int, [_vp, _i64, _vp, _vp, _i64, _vp, _vp, _vp] + [_i64] * 7 + [_int, _int, _vp]),
+    "ca_rotary_qkv_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _vp] + [_i64] * 7 + [_int, _int, _vp]),
+    "ca_rotary_append": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]
+                         + [_i64] * 10 + [_int, _int, _vp]),
+    "ca_paged_workspace_size": (_sz, [_i64] * 5 + [_int]),
+    "ca_paged_forward": (_int, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _sz]
+                         + [_i64] * 9 + [_int, _vp]),
 }
 
 _lock = threading.Lock()

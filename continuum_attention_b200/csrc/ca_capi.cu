@@ -434,6 +434,185 @@ int ca_gelu_tanh_backward(const void* x, const void* dy, void* dx, int64_t n, in
   return ok();
 }
 
+// what the rotary entry points share; 32-bit indexing: tokens, heads, table rows
+static int check_rotary(const char* fn, int64_t tokens, int64_t H, int64_t G, int64_t D, int64_t R, int64_t rows,
+                        int64_t qkv_stride, int layout, int dtype) {
+  if (tokens < 0 || H < 0 || G < 0 || D < 0)
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: negative shape (tokens %lld, heads %lld, kv_heads %lld, D %lld)", fn,
+                (long long)tokens, (long long)H, (long long)G, (long long)D);
+  if (dtype < CA_DTYPE_F32 || dtype > CA_DTYPE_F16)
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: unknown dtype code %d", fn, dtype);
+  if (layout != CA_ROTARY_INTERLEAVED && layout != CA_ROTARY_HALF)
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: unknown rotary layout code %d", fn, layout);
+  if (D % 8 != 0 || D > 256)
+    return fail(CA_ERR_UNSUPPORTED, "%s: head dim D=%lld must be a multiple of 8 and <= 256", fn, (long long)D);
+  if (R < 2 || R > D || R % 2 != 0)
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: rotary_dim=%lld must be even, from 2 to D=%lld", fn, (long long)R,
+                (long long)D);
+  if (rows < 1 || rows > 0x7fffffffLL)
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: a table of %lld rows", fn, (long long)rows);
+  if (H > (1LL << 20) || G > (1LL << 20)) return fail(CA_ERR_UNSUPPORTED, "%s: more than 2^20 heads", fn);
+  if (tokens > 0x7fffffffLL) return fail(CA_ERR_UNSUPPORTED, "%s: %lld tokens exceed 2^31-1", fn, (long long)tokens);
+  const int64_t esz = dtype == CA_DTYPE_F32 ? 4 : 2;
+  if (qkv_stride < (H + 2 * G) * D || qkv_stride * esz % 16)
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: qkv row stride %lld must hold (heads + 2 kv_heads) D values and be a "
+                "multiple of 16 bytes", fn, (long long)qkv_stride);
+  return CA_OK;
+}
+
+static int rotary_qkv(const char* fn, const void* qkv, int64_t qkv_stride, const float* cos_sin,
+                      const int32_t* positions, int64_t position_stride, const void* q, const void* k, const void* v,
+                      int64_t B, int64_t T, int64_t H, int64_t G, int64_t D, int64_t R, int64_t rows, int layout,
+                      int dtype, void* stream, bool back) {
+  g_last_launches = 0;
+  if (B < 0 || T < 0) return fail(CA_ERR_INVALID_ARGUMENT, "%s: negative shape", fn);
+  if (T > 0x7fffffffLL || (T > 0 && B > 0x7fffffffLL / T))
+    return fail(CA_ERR_UNSUPPORTED, "%s: B*T=%lld*%lld tokens exceed 2^31-1", fn, (long long)B, (long long)T);
+  int st = check_rotary(fn, B * T, H, G, D, R, rows, qkv_stride, layout, dtype);
+  if (st != CA_OK) return st;
+  if (!positions && T > rows)
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: T=%lld positions, a table of %lld rows", fn, (long long)T,
+                (long long)rows);
+  if (B * T == 0 || H + G == 0) return ok();
+  if (!qkv || !cos_sin || (H && !q) || (G && (!k || !v))) return fail(CA_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
+  if (!all_aligned16({qkv, cos_sin, q, k, v}))
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: buffers must be 16-byte aligned", fn);
+  ca::rotary::QkvArgs a{(void*)qkv, qkv_stride, cos_sin, positions, position_stride, (void*)q, (void*)k, (void*)v,
+                        (int)B, (int)T, (int)H, (int)G, (int)D, (int)R, (int)rows, layout, (cudaStream_t)stream};
+  cudaError_t e = ca::rotary::qkv(a, dtype, back);
+  if (e != cudaSuccess) return cuda_fail(e, fn);
+  g_last_launches = 1;
+  return ok();
+}
+
+int ca_rotary_qkv_forward(const void* qkv, int64_t qkv_stride, const float* cos_sin, const int32_t* positions,
+                          int64_t position_stride, void* q, void* k, void* v, int64_t B, int64_t T, int64_t heads,
+                          int64_t kv_heads, int64_t D, int64_t rotary_dim, int64_t table_rows, int layout,
+                          int dtype, void* stream) {
+  return rotary_qkv("ca_rotary_qkv_forward", qkv, qkv_stride, cos_sin, positions, position_stride, q, k, v, B, T,
+                    heads, kv_heads, D, rotary_dim, table_rows, layout, dtype, stream, false);
+}
+
+int ca_rotary_qkv_backward(const void* dq, const void* dk, const void* dv, const float* cos_sin,
+                           const int32_t* positions, int64_t position_stride, void* dqkv, int64_t B, int64_t T,
+                           int64_t heads, int64_t kv_heads, int64_t D, int64_t rotary_dim, int64_t table_rows,
+                           int layout, int dtype, void* stream) {
+  return rotary_qkv("ca_rotary_qkv_backward", dqkv, (heads + 2 * kv_heads) * D, cos_sin, positions, position_stride,
+                    dq, dk, dv, B, T, heads, kv_heads, D, rotary_dim, table_rows, layout, dtype, stream, true);
+}
+
+// what the entry points on a paged cache share: its shape, strides and the packed rows
+static int check_cache(const char* fn, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+                       int64_t page_table_stride, int64_t rows, int64_t seqs, int64_t num_pages, int64_t page_size,
+                       int64_t pages_per_seq, int dtype) {
+  if (rows < 0 || seqs < 0 || num_pages < 0 || pages_per_seq < 0)
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: negative shape (rows %lld, seqs %lld, pages %lld, pages_per_seq %lld)",
+                fn, (long long)rows, (long long)seqs, (long long)num_pages, (long long)pages_per_seq);
+  if (page_size < 1) return fail(CA_ERR_INVALID_ARGUMENT, "%s: page_size must be >= 1", fn);
+  if (rows > 0x7fffffffLL || seqs >= 0x7fffffffLL || num_pages > 0x7fffffffLL)
+    return fail(CA_ERR_UNSUPPORTED, "%s: rows, sequences and pages are limited to 2^31-1", fn);
+  if (pages_per_seq > 0 && page_size > 0x7fffffffLL / pages_per_seq)
+    return fail(CA_ERR_UNSUPPORTED, "%s: pages_per_seq * page_size = %lld * %lld keys exceed 2^31-1", fn,
+                (long long)pages_per_seq, (long long)page_size);
+  if (page_table_stride < 0 || (seqs > 1 && page_table_stride < pages_per_seq))
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: page table rows of %lld entries are %lld apart", fn,
+                (long long)pages_per_seq, (long long)page_table_stride);
+  const int64_t esz = dtype == CA_DTYPE_F32 ? 4 : 2;
+  if (page_stride < 0 || head_stride < 0 || slot_stride < 0 || page_stride * esz % 16 || head_stride * esz % 16 ||
+      slot_stride * esz % 16)
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: cache strides must be multiples of 16 bytes", fn);
+  return CA_OK;
+}
+
+int ca_rotary_append(const void* qkv, int64_t qkv_stride, const float* cos_sin, void* q, void* k_cache,
+                     void* v_cache, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+                     const int32_t* page_table, int64_t page_table_stride, const int32_t* kv_lens,
+                     const int32_t* q_starts, int64_t num_rows, int64_t num_seqs, int64_t heads, int64_t kv_heads,
+                     int64_t D, int64_t rotary_dim, int64_t table_rows, int64_t num_pages, int64_t page_size,
+                     int64_t pages_per_seq, int layout, int dtype, void* stream) {
+  const char* fn = "ca_rotary_append";
+  g_last_launches = 0;
+  int st = check_rotary(fn, num_rows, heads, kv_heads, D, rotary_dim, table_rows, qkv_stride, layout, dtype);
+  if (st != CA_OK) return st;
+  st = check_cache(fn, page_stride, head_stride, slot_stride, page_table_stride, num_rows, num_seqs, num_pages,
+                   page_size, pages_per_seq, dtype);
+  if (st != CA_OK) return st;
+  if (num_rows == 0 || num_seqs == 0 || heads + kv_heads == 0) return ok();
+  if (!qkv || !cos_sin || !kv_lens || !q_starts || (heads && !q) || (num_pages && kv_heads && (!k_cache || !v_cache)) ||
+      (pages_per_seq && !page_table))
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
+  if (!all_aligned16({qkv, cos_sin, q, k_cache, v_cache}))
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: buffers must be 16-byte aligned", fn);
+  ca::rotary::AppendArgs a{qkv, qkv_stride, cos_sin, q, k_cache, v_cache, page_stride, head_stride, slot_stride,
+                           page_table, page_table_stride, kv_lens, q_starts, (int)num_rows, (int)num_seqs, (int)heads,
+                           (int)kv_heads, (int)D, (int)rotary_dim, (int)table_rows, layout, (int)num_pages,
+                           (int)page_size, (int)pages_per_seq, (cudaStream_t)stream};
+  cudaError_t e = ca::rotary::append(a, dtype);
+  if (e != cudaSuccess) return cuda_fail(e, fn);
+  g_last_launches = 1;
+  return ok();
+}
+
+size_t ca_paged_workspace_size(int64_t num_seqs, int64_t max_q_len, int64_t heads, int64_t kv_heads, int64_t D,
+                               int dtype) {
+  if (num_seqs <= 0 || max_q_len <= 0 || heads <= 0 || kv_heads <= 0 || D <= 0) return 0;
+  return align_up(ca::paged::workspace_bytes(num_seqs, max_q_len, heads, kv_heads, D, dtype));
+}
+
+int ca_paged_forward(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
+                     const void* v_cache, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+                     const int32_t* page_table, int64_t page_table_stride, const int32_t* kv_lens,
+                     const int32_t* q_starts, const float* log_gain, void* o, void* workspace,
+                     size_t workspace_bytes, int64_t num_rows, int64_t num_seqs, int64_t max_q_len, int64_t heads,
+                     int64_t kv_heads, int64_t D, int64_t num_pages, int64_t page_size, int64_t pages_per_seq,
+                     int dtype, void* stream) {
+  const char* fn = "ca_paged_forward";
+  g_last_launches = 0;
+  if (dtype < CA_DTYPE_F32 || dtype > CA_DTYPE_F16)
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: unknown dtype code %d", fn, dtype);
+  int st = check_cache(fn, page_stride, head_stride, slot_stride, page_table_stride, num_rows, num_seqs, num_pages,
+                       page_size, pages_per_seq, dtype);
+  if (st != CA_OK) return st;
+  if (heads < 0 || kv_heads < 0 || max_q_len < 0)
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: negative shape (heads %lld, kv_heads %lld, max_q_len %lld)", fn,
+                (long long)heads, (long long)kv_heads, (long long)max_q_len);
+  if (D < 8 || D % 8 != 0 || D > 128)
+    return fail(CA_ERR_UNSUPPORTED, "%s: head dim D=%lld must be a multiple of 8 and <= 128", fn, (long long)D);
+  if (num_rows == 0 || num_seqs == 0 || heads == 0) return ok();
+  if (kv_heads == 0 || heads % kv_heads != 0)
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: heads=%lld is not a multiple of kv_heads=%lld", fn, (long long)heads,
+                (long long)kv_heads);
+  if (max_q_len < 1) return fail(CA_ERR_INVALID_ARGUMENT, "%s: max_q_len must be >= 1", fn);
+  if (max_q_len > num_rows) max_q_len = num_rows;   // no sequence has more rows than there are
+  if (num_seqs > ca::paged::kMaxSeqs)
+    return fail(CA_ERR_UNSUPPORTED, "%s: %lld sequences in one call, at most %d are covered", fn, (long long)num_seqs,
+                ca::paged::kMaxSeqs);
+  if (heads > (1LL << 20) || max_q_len > 0x7fffffffLL / heads)
+    return fail(CA_ERR_UNSUPPORTED, "%s: max_q_len * heads = %lld * %lld exceeds 2^31-1", fn, (long long)max_q_len,
+                (long long)heads);
+  const int64_t esz = dtype == CA_DTYPE_F32 ? 4 : 2;
+  if (q_token_stride < 0 || q_head_stride < 0 || q_token_stride * esz % 16 || q_head_stride * esz % 16)
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: q strides must be multiples of 16 bytes", fn);
+  if (!q || !kv_lens || !q_starts || !log_gain || !o || (num_pages && (!k_cache || !v_cache)) ||
+      (pages_per_seq && !page_table))
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: null pointer", fn);
+  if (!all_aligned16({q, k_cache, v_cache, o}))
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: buffers must be 16-byte aligned", fn);
+  const size_t need = ca_paged_workspace_size(num_seqs, max_q_len, heads, kv_heads, D, dtype);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(CA_ERR_WORKSPACE, "%s: workspace of %zu bytes < required %zu", fn, workspace_bytes, need);
+  if (need && ((uintptr_t)workspace) % kAlign != 0)
+    return fail(CA_ERR_INVALID_ARGUMENT, "%s: workspace must be %zu-byte aligned", fn, kAlign);
+  ca::paged::Args a{q, q_token_stride, q_head_stride, k_cache, v_cache, page_stride, head_stride, slot_stride,
+                    page_table, page_table_stride, kv_lens, q_starts, log_gain, o, (int)num_rows, (int)num_seqs,
+                    (int)max_q_len, (int)heads, (int)kv_heads, (int)D, (int)num_pages, (int)page_size,
+                    (int)pages_per_seq, (float)(1.0 / std::sqrt((double)D)), (cudaStream_t)stream};
+  cudaError_t e = ca::paged::forward(a, dtype, workspace);
+  if (e != cudaSuccess) return cuda_fail(e, fn);
+  g_last_launches = ca::paged::launches(a, dtype);
+  return ok();
+}
+
 int ca_device_status(int reset) {
   int value = 0;
   cudaError_t e = ca::read_device_status(&value, reset != 0);

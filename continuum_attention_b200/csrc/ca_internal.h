@@ -150,6 +150,70 @@ cudaError_t forward(const void* x, void* y, size_t n, int dtype, cudaStream_t s)
 cudaError_t backward(const void* x, const void* dy, void* dx, size_t n, int dtype, cudaStream_t s);
 }  // namespace gelu
 
+namespace rotary {
+// Pairs of the first R of D head values turned by cos_sin [table_rows][R/2][2]; half: pair p is
+// (p, p + R/2), else (2p, 2p + 1).  All buffers 16-byte aligned, strides in elements.
+struct QkvArgs {
+  void* qkv;               // [B*T] rows of (H + 2G) D, qkv_stride apart
+  long long qkv_stride;
+  const float* cos_sin;
+  const int* positions;    // null: 0 .. T-1; else [T] (pos_stride 0) or [B][T]
+  long long pos_stride;
+  void* q;                 // [B][H][T][D]
+  void* k;                 // [B][G][T][D]
+  void* v;
+  int B, T, H, G, D, R, table_rows, half;
+  cudaStream_t stream;
+};
+struct AppendArgs {
+  const void* qkv;         // [tokens] rows of (H + 2G) D, qkv_stride apart
+  long long qkv_stride;
+  const float* cos_sin;
+  void* q;                 // [tokens][H][D]
+  void* k_cache;           // page, key head and slot strides in elements
+  void* v_cache;
+  long long page_stride, head_stride, slot_stride;
+  const int* page_table;
+  long long page_table_stride;
+  const int* kv_lens;
+  const int* q_starts;
+  int tokens, seqs, H, G, D, R, table_rows, half;
+  int num_pages, page_size, pages_per_seq;
+  cudaStream_t stream;
+};
+cudaError_t qkv(const QkvArgs& a, int dtype, bool back);
+cudaError_t append(const AppendArgs& a, int dtype);
+// the word that records positions, lengths or pages out of range (0: none so far)
+cudaError_t read_status(int* out, bool reset);
+}  // namespace rotary
+
+namespace paged {
+// Continuum Attention of packed new tokens over a paged cache (ca_paged.cu)
+struct Args {
+  const void* q;           // [rows][H][D], token and head strides in elements
+  long long q_token_stride, q_head_stride;
+  const void* k_cache;     // page, key head and slot strides in elements
+  const void* v_cache;
+  long long page_stride, head_stride, slot_stride;
+  const int* page_table;
+  long long page_table_stride;
+  const int* kv_lens;
+  const int* q_starts;
+  const float* log_gain;
+  void* o;                 // [rows][H][D]
+  int rows, seqs, max_q_len, H, G, D;
+  int num_pages, page_size, pages_per_seq;
+  float inv_sqrt_d;
+  cudaStream_t stream;
+};
+constexpr int kMaxSeqs = 4096;   // sequences in one call
+size_t workspace_bytes(long long seqs, long long max_q_len, long long H, long long G, long long D, int dtype);
+cudaError_t forward(const Args& a, int dtype, void* workspace);
+int launches(const Args& a, int dtype);
+cudaError_t read_status(int* out, bool reset);
+}  // namespace paged
+
+// the first word that is set: a wait that gave up, or a page, position or length out of range
 cudaError_t read_device_status(int* out, bool reset);
 
 }  // namespace ca

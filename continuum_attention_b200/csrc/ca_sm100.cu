@@ -2054,9 +2054,18 @@ cudaError_t read_device_status(int* out, bool reset) {
   cudaError_t e = cudaDeviceSynchronize();
   if (e != cudaSuccess) return e;
   e = cudaMemcpyFromSymbol(out, sm100::g_device_status, sizeof(int));
-  if (e != cudaSuccess || !reset) return e;
-  const int zero = 0;
-  return cudaMemcpyToSymbol(sm100::g_device_status, &zero, sizeof(int));
+  if (e != cudaSuccess) return e;
+  int more[2] = {0, 0};
+  e = rotary::read_status(&more[0], reset);
+  if (e != cudaSuccess) return e;
+  e = paged::read_status(&more[1], reset);
+  if (e != cudaSuccess) return e;
+  if (reset) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(sm100::g_device_status, &zero, sizeof(int));
+  }
+  if (*out == 0) *out = more[0] ? more[0] : more[1];
+  return e;
 }
 
 }  // namespace ca

@@ -256,15 +256,99 @@ int ca_add_rmsnorm_backward(const float* x_new, const float* w, const void* dy, 
 int ca_gelu_tanh_forward(const void* x, void* y, int64_t n, int dtype, void* stream);
 int ca_gelu_tanh_backward(const void* x, const void* dy, void* dx, int64_t n, int dtype, void* stream);
 
+/*
+ * Rotary positions in general form (no reference counterpart beyond
+ * ca_rope_qkv_*, which is the interleaved full-head case).  The first
+ * rotary_dim values of each query and key head are turned pairwise by
+ * (c, s) = cos_sin[t][p], float32 [table_rows][rotary_dim/2][2]:
+ *   (x, y) -> (x c - y s, y c + x s)
+ * with (x, y) = (h_{2p}, h_{2p+1}) for CA_ROTARY_INTERLEAVED and
+ * (h_p, h_{p + rotary_dim/2}) for CA_ROTARY_HALF; the other values and the
+ * value heads pass through.  The table carries any stretching of the context.
+ *   qkv        [B*T] rows of (heads + 2 kv_heads) * D values: the query heads, then
+ *              the key heads, then the value heads; rows qkv_stride elements apart
+ *   positions  int32 [T] (position_stride 0) or [B] rows position_stride apart;
+ *              NULL for 0 .. T-1
+ *   q, k, v    [B][heads][T][D], [B][kv_heads][T][D] twice
+ * D a multiple of 8, at most 256; rotary_dim even, 2 .. D; every buffer 16-byte
+ * aligned and row strides a multiple of 16 bytes.  fp32 arithmetic, one rounding per
+ * output.  A position outside the table makes the token's turned values NaN and is
+ * recorded in ca_device_status().  One launch, no allocation.
+ */
+enum ca_rotary_layout { CA_ROTARY_INTERLEAVED = 0, CA_ROTARY_HALF = 1 };
+int ca_rotary_qkv_forward(const void* qkv, int64_t qkv_stride, const float* cos_sin, const int32_t* positions,
+                          int64_t position_stride, void* q, void* k, void* v, int64_t B, int64_t T, int64_t heads,
+                          int64_t kv_heads, int64_t D, int64_t rotary_dim, int64_t table_rows, int layout,
+                          int dtype, void* stream);
+
+/* Gradient of ca_rotary_qkv_forward: dq, dk, dv -> dqkv (rows (heads + 2 kv_heads) * D
+ * apart) with the transposed turn. */
+int ca_rotary_qkv_backward(const void* dq, const void* dk, const void* dv, const float* cos_sin,
+                           const int32_t* positions, int64_t position_stride, void* dqkv, int64_t B, int64_t T,
+                           int64_t heads, int64_t kv_heads, int64_t D, int64_t rotary_dim, int64_t table_rows,
+                           int layout, int dtype, void* stream);
+
+/*
+ * The paged cache.  Keys and values of key head g, slot r of page p start at element
+ * p * page_stride + g * head_stride + r * slot_stride of k_cache / v_cache (strides
+ * multiples of 16 bytes, the D values contiguous).  Sequence s holds kv_lens[s] keys;
+ * key j is in slot j % page_size of page page_table[s * page_table_stride + j / page_size].
+ * New tokens are packed: rows q_starts[s] .. q_starts[s+1] - 1 belong to sequence s
+ * (q_starts has num_seqs + 1 entries), and kv_lens counts them: row n sits at position
+ * kv_lens[s] - (q_starts[s+1] - n).  Rows behind q_starts[num_seqs] are left as they
+ * were.  kv_lens, q_starts and page_table are int32 on the device; entries of the page
+ * table that no key needs are never used.  A page outside 0 .. num_pages-1, a length
+ * beyond pages_per_seq * page_size, or rows outside the buffers are recorded in
+ * ca_device_status() as CA_ERR_INVALID_ARGUMENT; nothing is read or written there.
+ *
+ * ca_rotary_append: turns the new tokens' queries and keys at their positions (as
+ * ca_rotary_qkv_forward), writes q [num_rows][heads][D] and writes keys and values into
+ * the cache.  A row at a negative position (more rows than keys) writes no key and a q
+ * of zeros; a row whose position or page is out of range writes no key and a q of NaN.
+ * No two rows may share a slot.  One launch, no allocation.
+ */
+int ca_rotary_append(const void* qkv, int64_t qkv_stride, const float* cos_sin, void* q, void* k_cache,
+                     void* v_cache, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+                     const int32_t* page_table, int64_t page_table_stride, const int32_t* kv_lens,
+                     const int32_t* q_starts, int64_t num_rows, int64_t num_seqs, int64_t heads, int64_t kv_heads,
+                     int64_t D, int64_t rotary_dim, int64_t table_rows, int64_t num_pages, int64_t page_size,
+                     int64_t pages_per_seq, int layout, int dtype, void* stream);
+
+/*
+ * Continuum Attention of new tokens over the paged cache, for serving (no gradient): row n
+ * of query head h attends to the keys at positions 0 .. its own of key head
+ * h / (heads / kv_heads), with the scores, trajectories and caps of ca_forward.  A row at a
+ * negative position gives zeros.  q rows are q_token_stride and heads q_head_stride elements
+ * apart; o is [num_rows][heads][D].  The rows of a sequence whose length is out of range, and
+ * those that see a page out of range, come out NaN (see above).  max_q_len is the number of new
+ * tokens of the longest sequence, by which the kernel is chosen; a wrong one costs time only.
+ * heads a multiple of kv_heads; D a multiple of 8, at most 128; every buffer and stride a
+ * multiple of 16 bytes (o and q included).  workspace holds
+ * ca_paged_workspace_size() bytes (256-byte aligned; its contents are ignored, and it
+ * belongs to this call until the call's GPU work has finished).
+ */
+size_t ca_paged_workspace_size(int64_t num_seqs, int64_t max_q_len, int64_t heads, int64_t kv_heads, int64_t D,
+                               int dtype);
+int ca_paged_forward(const void* q, int64_t q_token_stride, int64_t q_head_stride, const void* k_cache,
+                     const void* v_cache, int64_t page_stride, int64_t head_stride, int64_t slot_stride,
+                     const int32_t* page_table, int64_t page_table_stride, const int32_t* kv_lens,
+                     const int32_t* q_starts, const float* log_gain, void* o, void* workspace,
+                     size_t workspace_bytes, int64_t num_rows, int64_t num_seqs, int64_t max_q_len, int64_t heads,
+                     int64_t kv_heads, int64_t D, int64_t num_pages, int64_t page_size, int64_t pages_per_seq,
+                     int dtype, void* stream);
+
 /* Number of kernels the last successful ca_forward / ca_backward /
- * ca_rope_qkv_* / ca_rmsnorm_* / ca_add_rmsnorm_* / ca_gelu_tanh_* call on this
+ * ca_rope_qkv_* / ca_rmsnorm_* / ca_add_rmsnorm_* / ca_gelu_tanh_* / ca_rotary_* /
+ * ca_paged_forward call on this
  * thread enqueued (memsets excluded).  Diagnostic for launch accounting. */
 int ca_last_launch_count(void);
 
 /*
  * Device status word of the calling thread's current device: 0 if every
- * bounded device-side wait since the last reset completed, else a CA_ERR_*
- * code recorded by a kernel that gave up waiting.  Synchronises the device.
+ * bounded device-side wait since the last reset completed and every length, page
+ * and position read on the device was in range, else a CA_ERR_* code recorded by
+ * a kernel that gave up waiting (CA_ERR_DEVICE_TIMEOUT) or met one that was not
+ * (CA_ERR_INVALID_ARGUMENT).  Synchronises the device.
  * reset != 0 clears the word after reading it.
  */
 int ca_device_status(int reset);
