@@ -206,7 +206,7 @@ struct Args {
   float inv_sqrt_d;
   cudaStream_t stream;
 };
-constexpr int kMaxSeqs = 4096;   // sequences in one call
+constexpr int kMaxSeqs = 2048;   // sequences in one call
 size_t workspace_bytes(long long seqs, long long max_q_len, long long H, long long G, long long D, int dtype);
 cudaError_t forward(const Args& a, int dtype, void* workspace);
 int launches(const Args& a, int dtype);

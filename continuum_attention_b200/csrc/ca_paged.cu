@@ -5,12 +5,10 @@
 
 #include "ca_common.cuh"
 #include "ca_internal.h"
+#include "ca_paged.cuh"
 
 namespace ca {
 namespace paged {
-
-__device__ int g_status = 0;
-__device__ __forceinline__ void record_invalid() { atomicCAS(&g_status, 0, 1); }
 
 constexpr int kWarps = 8;
 
@@ -91,8 +89,11 @@ __global__ void simple_kernel(Args a) {
   for (int t = (int)(w / a.H); t < n; t += a.max_q_len) simple_row<T>(a, s, t, (int)(w % a.H));
 }
 
-size_t workspace_bytes(long long, long long, long long, long long, long long, int) { return 0; }
-int launches(const Args&, int) { return 1; }
+size_t workspace_bytes(long long seqs, long long max_q_len, long long H, long long G, long long D, int dtype) {
+  (void)seqs;
+  return dtype == 0 ? 0 : mma_workspace_bytes(max_q_len, H, G, D);
+}
+int launches(const Args& a, int dtype) { return dtype == 0 ? 1 : mma_launches(a); }
 
 template <typename T>
 static cudaError_t forward_t(const Args& a) {
@@ -101,17 +102,17 @@ static cudaError_t forward_t(const Args& a) {
                     dim3(kWarps * 32), 0, a.stream, a);
 }
 
-cudaError_t forward(const Args& a, int dtype, void*) {
-  switch (dtype) {
-    case 0: return forward_t<float>(a);
-    case 1: return forward_t<__nv_bfloat16>(a);
-    default: return forward_t<__half>(a);
-  }
+cudaError_t forward(const Args& a, int dtype, void* workspace) {
+  return dtype == 0 ? forward_t<float>(a) : mma_forward(a, dtype, workspace);
 }
 
 cudaError_t read_status(int* out, bool reset) {
-  cudaError_t e = cudaMemcpyFromSymbol(out, g_status, sizeof(int));
-  if (e != cudaSuccess || !reset || *out == 0) return e;
+  int own = 0;
+  cudaError_t e = mma_read_status(out, reset);
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&own, g_status, sizeof(int));
+  if (e != cudaSuccess) return e;
+  if (*out == 0) *out = own;
+  if (!reset || own == 0) return e;
   const int zero = 0;
   return cudaMemcpyToSymbol(g_status, &zero, sizeof(int));
 }

@@ -1,0 +1,219 @@
+// ca_paged.cuh -- how the kernels over a paged cache divide their work: units (row tile,
+// key head, sequence), their tiles of keys, and equal ranges of all tiles for the workers.
+#pragma once
+
+#include <algorithm>
+
+#include "ca_common.cuh"
+#include "ca_internal.h"
+
+namespace ca {
+namespace paged {
+
+// set to CA_ERR_INVALID_ARGUMENT by a length, row range or page that is out of range (one word per
+// source file that includes this; ca_paged.cu reads them all)
+static __device__ int g_status = 0;
+__device__ __forceinline__ void record_invalid() { atomicCAS(&g_status, 0, 1); }
+
+constexpr int kChunkBlocksPerSM = 3;
+
+struct Plan {
+  int group;              // query heads per key head
+  int page_shift;         // log2(page_size), or -1
+  int page_size;
+  int capacity;           // keys that a page-table row covers
+  int row_lo, row_hi;     // rows (tokens * group) of the sequences that this launch takes
+  unsigned min_tiles;     // of a worker's range
+
+  __device__ __forceinline__ int page_of(int key) const { return page_shift >= 0 ? key >> page_shift : key / page_size; }
+  __device__ __forceinline__ unsigned tiles_per_worker(unsigned total, int workers) const {
+    return max((total + workers - 1) / (unsigned)workers, min_tiles);
+  }
+};
+
+inline Plan make_plan(const Args& a) {
+  Plan p;
+  p.group = a.H / a.G;
+  p.page_size = a.page_size;
+  p.page_shift = -1;
+  for (int s = 0; s < 31; ++s)
+    if (a.page_size == 1 << s) p.page_shift = s;
+  p.capacity = a.pages_per_seq * a.page_size;
+  p.row_lo = 0;
+  p.row_hi = 0x7fffffff;
+  p.min_tiles = 1;
+  return p;
+}
+
+// bf16 and f16 (ca_paged_mma.cu)
+size_t mma_workspace_bytes(long long max_q_len, long long H, long long G, long long D);
+int mma_launches(const Args& a);
+cudaError_t mma_forward(const Args& a, int dtype, void* workspace);
+cudaError_t mma_read_status(int* out, bool reset);
+
+// a worker whose unit goes on behind its range: what merge_kernel joins
+struct Meta {
+  int pieces, slot, start, rows, h, rt;
+};
+
+// Prefix sums of the sequences' tiles in shared memory (all threads of the block take part in the
+// constructor), and cursors into the stream of tiles: sequence, key head, row tile, key tile.
+template <int BR, int TK>
+struct Schedule {
+  const Args& a;
+  const Plan& plan;
+  unsigned* prefix;    // [seqs + 1]
+  unsigned total;
+
+  struct Cursor {
+    int s, h, rt, kt, nt;
+    int start, n, len, bad;
+    int tiles_rt;      // row tiles
+  };
+
+  // tiles of a unit whose last row stands at position i
+  static __device__ __forceinline__ int tiles_to(int i) { return i < 0 ? 1 : i / TK + 1; }
+
+  __device__ __forceinline__ int unit_tiles(int rt, int rows, int lead) const {
+    return tiles_to(lead + (min(rows, (rt + 1) * BR) - 1) / plan.group);
+  }
+
+  // n = 0 for a sequence that this launch does not take
+  __device__ __forceinline__ void load(int s, int& start, int& n, int& len, int& bad) const {
+    start = a.q_starts[s];
+    const int end = a.q_starts[s + 1];
+    len = a.kv_lens[s];
+    n = 0;
+    bad = 0;
+    if (start < 0 || end > a.rows || start > end) {
+      record_invalid();
+      return;
+    }
+    const int rows = (end - start) * plan.group;
+    if (rows < plan.row_lo || rows > plan.row_hi) return;
+    n = end - start;
+    if (n > 0 && (len < 0 || len > plan.capacity)) {
+      record_invalid();
+      bad = 1;
+      len = 0;
+    }
+  }
+
+  __device__ Schedule(const Args& a_, const Plan& plan_, unsigned* prefix_) : a(a_), plan(plan_), prefix(prefix_) {
+    const int lane = threadIdx.x & 31;
+    // whole warps walk the sequences, so that several row tiles are summed by all lanes
+    for (int s0 = (threadIdx.x >> 5) * 32; s0 < a.seqs; s0 += blockDim.x) {
+      const int s = s0 + lane;
+      int start = 0, n = 0, len = 0, bad = 0;
+      if (s < a.seqs) load(s, start, n, len, bad);
+      const int rows = n * plan.group;
+      const int nrt = (rows + BR - 1) / BR;
+      unsigned long long tiles = nrt == 1 ? unit_tiles(0, rows, len - n) : 0;
+      unsigned many = __ballot_sync(0xffffffffu, nrt > 1);
+      while (many) {
+        const int b = __ffs(many) - 1;
+        many &= many - 1;
+        const int rows_b = __shfl_sync(0xffffffffu, rows, b), lead_b = __shfl_sync(0xffffffffu, len - n, b);
+        const int nrt_b = __shfl_sync(0xffffffffu, nrt, b);
+        unsigned long long sum = 0;
+        for (int rt = lane; rt < nrt_b; rt += 32) sum += unit_tiles(rt, rows_b, lead_b);
+#pragma unroll
+        for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        if (lane == b) tiles = sum;
+      }
+      tiles *= (unsigned)a.G;
+      if (s < a.seqs) prefix[s + 1] = (unsigned)min(tiles, 0x7fffffffull);
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      unsigned long long carry = 0;
+      for (int s0 = 0; s0 < a.seqs; s0 += 32) {
+        const int s = s0 + lane;
+        unsigned long long v = s < a.seqs ? prefix[s + 1] : 0;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const unsigned long long u = __shfl_up_sync(0xffffffffu, v, off);
+          if (lane >= off) v += u;
+        }
+        v += carry;
+        if (s < a.seqs) prefix[s + 1] = (unsigned)min(v, 0x7fffffffull);
+        carry = __shfl_sync(0xffffffffu, v, 31);
+      }
+      if (lane == 0) {
+        prefix[0] = 0;
+        if (carry >= 0x7fffffffull) {    // more tiles than the stream's index holds: no answer at all
+          record_invalid();
+          prefix[a.seqs] = 0;
+        }
+      }
+    }
+    __syncthreads();
+    total = prefix[a.seqs];
+  }
+
+  __device__ __forceinline__ void enter(Cursor& c) const {   // a new sequence
+    load(c.s, c.start, c.n, c.len, c.bad);
+    c.tiles_rt = (c.n * plan.group + BR - 1) / BR;
+  }
+
+  // whole warps call this
+  __device__ Cursor locate(unsigned x) const {
+    Cursor c;
+    int lo = 0, hi = a.seqs;               // the sequence with prefix[s] <= x < prefix[s + 1]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid] <= x) lo = mid;
+      else hi = mid;
+    }
+    c.s = lo;
+    enter(c);
+    const unsigned per_head = (prefix[lo + 1] - prefix[lo]) / (unsigned)a.G;
+    unsigned y = x - prefix[lo];
+    c.h = (int)(y / per_head);
+    y -= (unsigned)c.h * per_head;
+    c.rt = 0;
+    const int rows = c.n * plan.group, lead = c.len - c.n;
+    if (c.tiles_rt > 1) {
+      const int lane = threadIdx.x & 31;
+      for (int r0 = 0; r0 < c.tiles_rt; r0 += 32) {
+        const int rt = r0 + lane;
+        const unsigned own = rt < c.tiles_rt ? (unsigned)unit_tiles(rt, rows, lead) : 0;
+        unsigned v = own;
+#pragma unroll
+        for (int off = 1; off < 32; off <<= 1) {
+          const unsigned u = __shfl_up_sync(0xffffffffu, v, off);
+          if (lane >= off) v += u;
+        }
+        const unsigned in = __ballot_sync(0xffffffffu, v > y);
+        if (in) {
+          const int b = __ffs(in) - 1;
+          c.rt = r0 + b;
+          y -= __shfl_sync(0xffffffffu, v - own, b);
+          break;
+        }
+        y -= __shfl_sync(0xffffffffu, v, 31);
+      }
+    }
+    c.kt = (int)y;
+    c.nt = unit_tiles(c.rt, rows, lead);
+    return c;
+  }
+
+  __device__ __forceinline__ void advance(Cursor& c) const {
+    if (++c.kt < c.nt) return;
+    c.kt = 0;
+    if (++c.rt == c.tiles_rt) {
+      c.rt = 0;
+      if (++c.h == a.G) {
+        c.h = 0;
+        do ++c.s;
+        while (prefix[c.s + 1] == prefix[c.s]);
+        enter(c);
+      }
+    }
+    c.nt = unit_tiles(c.rt, c.n * plan.group, c.len - c.n);
+  }
+};
+
+}  // namespace paged
+}  // namespace ca

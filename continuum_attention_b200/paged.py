@@ -113,7 +113,8 @@ def continuum_attention_paged(q, k_cache, v_cache, page_table, kv_lens, q_starts
     lib = _native.lib()
     code = _DTYPE_CODE[q.dtype]
     max_q_len = min(int(max_q_len), N)
-    nbytes = int(lib.ca_paged_workspace_size(S, max_q_len, H, G, D, code))
+    with torch.cuda.device(q.device):
+        nbytes = int(lib.ca_paged_workspace_size(S, max_q_len, H, G, D, code))
     if workspace is None:
         workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
     elif workspace.device != q.device or workspace.numel() * workspace.element_size() < nbytes \
