@@ -15,8 +15,6 @@ namespace paged {
 static __device__ int g_status = 0;
 __device__ __forceinline__ void record_invalid() { atomicCAS(&g_status, 0, 1); }
 
-constexpr int kChunkBlocksPerSM = 3;
-
 struct Plan {
   int group;              // query heads per key head
   int page_shift;         // log2(page_size), or -1
@@ -24,6 +22,7 @@ struct Plan {
   int capacity;           // keys that a page-table row covers
   int row_lo, row_hi;     // rows (tokens * group) of the sequences that this launch takes
   unsigned min_tiles;     // of a worker's range
+  int unit_rows;          // rows that one copy brings
 
   __device__ __forceinline__ int page_of(int key) const { return page_shift >= 0 ? key >> page_shift : key / page_size; }
   __device__ __forceinline__ unsigned tiles_per_worker(unsigned total, int workers) const {
@@ -42,6 +41,7 @@ inline Plan make_plan(const Args& a) {
   p.row_lo = 0;
   p.row_hi = 0x7fffffff;
   p.min_tiles = 1;
+  p.unit_rows = 1;
   return p;
 }
 

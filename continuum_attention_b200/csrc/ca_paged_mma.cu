@@ -14,22 +14,27 @@
 // four warps with 16 rows each that share the ring.
 //
 // Cutting keys.  Segments, not keys, are divided: the segment from key j-1 to key j belongs
-// to the tile of j.  A tile with keys a .. a+TK-1 therefore weighs keys a-1 .. a+TK-2, V is
-// staged one row early, and only the mass that ends at key a+TK-1 is carried on.  The first
-// tile of a piece also stages K row a-1 (its score starts the first segment), the last one
-// V row a+TK-1 (for the carried mass, and the row's own cap).
+// to the tile of j.  A tile of keys a .. a+TK-1 therefore weighs keys a-1 .. a+TK-2, and only
+// the mass that ends at key a+TK-1 is carried on.  The first tile of a piece brings K and V
+// row a-1 along (the score that the first segment starts from, the row it weighs); later
+// tiles keep the V row of the tile before.
 //
 // Registers.  The products run on mma.sync m16n8k16 with scores in registers: the bound of
-// this operator is the scalar work per score (one exp2, one reciprocal, about 17 other
-// instructions), not the tensor pipe, and register scores spare the trip through tensor
+// this operator is the scalar work per score (one exp2, one reciprocal, about 13 packed or
+// single instructions), not the tensor pipe, and register scores spare the trip through tensor
 // memory.  B fragments may come from any rows, so keys are dealt to lanes in runs: column
-// 2c + e of score tile j is key (TK/4) c + j + (TK/8) e.  A lane's pair (j, j + TK/8) then
-// has the pair (j-1, j-1 + TK/8) as its left neighbours, every step of the moments is one
+// 2c + e of score tile j is key (TK/4) c + j + NJ e, NJ = TK/8.  A lane's pair (j, j + NJ)
+// then has the pair (j-1, j-1 + NJ) as its left neighbours, every step of the moments is one
 // packed f32x2 instruction for two keys, and neighbours in other lanes are needed once per
 // run.  The weights leave as A fragments with the same dealing of V rows.  Each weight is
 // split into two 16-bit parts (hi + lo, 16 bits or more): one rounding to bf16 would put
 // 1.1e-3 of the output's size on every row.  With 8 rows or fewer hi and lo are the two
 // halves of one fragment and cost one product.
+//
+// Shared memory.  The eight rows of a fragment lie NJ rows apart, so every NJ rows are
+// followed by 16 bytes: the eight land in different banks without any address arithmetic, and
+// each NJ rows (512 or 1024 bytes) are one bulk copy where the page holds them in one run,
+// else one copy per row.
 #include <algorithm>
 
 #include "ca_common.cuh"
@@ -42,15 +47,52 @@ namespace {
 
 constexpr float kRescaleNats = 8.f;   // the reference maximum moves when it grows by more
 
-__device__ uint4 g_nan16 = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};   // NaN in bf16, f16 and f32
-
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool fill) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(fill ? 0 : 16));
+
+__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
-__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;"); }
-template <int N>
-__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+               "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
+// Whole warp; gives up after two seconds (the barrier of copies that never land): records the timeout and
+// raises the group's flag, which ends the others' waits too.
+__device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+  unsigned long long t0, t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  bool ok = false;
+  while (!ok) {
+    ok = bar_try(bar, parity);
+    if (*gave_up) break;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    if (!ok && t - t0 > 2000000000ull) {
+      atomicCAS(&g_status, 0, 5);
+      *gave_up = 1;
+      break;
+    }
+  }
+  return ok;
+}
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+  bool ok = bar_try(bar, parity);
+  if (!ok) ok = bar_wait_slow(bar, parity, gave_up);
+  return __all_sync(0xffffffffu, ok);
+}
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+// orders this thread's shared-memory writes before later bulk copies into the same place
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -116,21 +158,22 @@ __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Weights of one lane's run of one row.  raw[j] = unscaled scores of keys (kc + j, kc + NJ + j), sL the
-// scaled score of key kc - 1, m2 the reference maximum in log2 units.  On return W[j] weighs keys
-// (kc - 1 + j, kc + NJ - 1 + j), but for the mass that ends at key kc - 1, which the lane to the
-// left adds to W[0].x; last is the mass that ends at the run's last key.
-// kEdge: keys beyond position i are masked by selects (their exponentials may overflow), segment
-// k counts for 1 <= k <= i, keys 0 and i have half caps; key i's belongs to this piece when i >= lowest
-// (the piece before it has weighed its own last key to the end).
-template <bool kEdge, int NJ>
-__device__ __forceinline__ void weigh(const float2 (&raw)[NJ], float scale, float m2, int kc, int i, int lowest,
-                                      float sL, float2 (&W)[NJ], float& last, float2& z2) {
-  const float2 l2e = splat2(kLog2e), nm2 = splat2(-m2), sc = splat2(scale);
-  float2 sv[NJ], ev[NJ], M1[NJ];
+// A score that no exponential feels: what masked keys and the key before key 0 get.  Their segments'
+// moments vanish without a select: the closed form divides by 1e30, and between two of them both
+// exponentials are 0.  (Finite, since infinities would meet as NaN.)
+constexpr float kMasked = -1e30f;
+
+// Weights of one lane's run of one row.  sv[j] = scaled scores of keys (kc + j, kc + NJ + j), sL that of key
+// kc - 1, m2 the reference maximum in log2 units.  On return W[j] weighs keys (kc - 1 + j, kc + NJ - 1 + j),
+// but for the mass that ends at key kc - 1, which the lane to the left adds to W[0].x; last is the mass
+// that ends at the run's last key.
+template <int NJ>
+__device__ __forceinline__ void weigh(const float2 (&sv)[NJ], float m2, float sL, float2 (&W)[NJ], float& last,
+                                      float2& z2) {
+  const float2 l2e = splat2(kLog2e), nm2 = splat2(-m2);
+  float2 ev[NJ], M1[NJ];
 #pragma unroll
   for (int j = 0; j < NJ; ++j) {
-    sv[j] = mul2(raw[j], sc);
     const float2 arg = fma2(sv[j], l2e, nm2);
     ev[j] = make_float2(ex2_approx(arg.x), ex2_approx(arg.y));
   }
@@ -143,27 +186,14 @@ __device__ __forceinline__ void weigh(const float2 (&raw)[NJ], float scale, floa
     const float2 rn = make_float2(rcp_approx(nd.x), rcp_approx(nd.y));         // -1/d
     float2 ps = fma2(splat2(-1.f / 30.f), nd, splat2(1.f / 8.f));              // J1's series in -nd
     ps = fma2(ps, nd, splat2(-1.f / 3.f));
-    ps = mul2(fma2(ps, nd, splat2(1.f / 2.f)), eL);
+    ps = fma2(ps, nd, splat2(1.f / 2.f));
     const float2 m0c = mul2(sub2(eL, ev[j]), rn);
     const float2 m1c = mul2(sub2(m0c, ev[j]), rn);
-    float2 m1 = make_float2(fabsf(nd.x) < kSeriesMaxFwd ? ps.x : m1c.x, fabsf(nd.y) < kSeriesMaxFwd ? ps.y : m1c.y);
-    float2 m0 = fma2(nd, m1, ev[j]);
-    if (kEdge) {
-      const int kx = kc + j, ky = kc + NJ + j;
-      const bool okx = kx >= 1 && kx <= i, oky = ky <= i;
-      m0 = make_float2(okx ? m0.x : 0.f, oky ? m0.y : 0.f);
-      m1 = make_float2(okx ? m1.x : 0.f, oky ? m1.y : 0.f);
-    }
-    M1[j] = m1;
-    W[j] = sub2(m0, m1);
+    M1[j] = make_float2(sel_series(m1c.x, nd.x, eL.x, ps.x, kSeriesMaxFwd),
+                        sel_series(m1c.y, nd.y, eL.y, ps.y, kSeriesMaxFwd));
+    const float2 m0 = fma2(nd, M1[j], ev[j]);
+    W[j] = sub2(m0, M1[j]);
     z2 = add2(z2, m0);
-    if (kEdge) {
-      const int kx = kc + j - 1, ky = kc + NJ + j - 1;   // the keys these weights belong to
-      const float nx = (kx == 0 && i >= 0 ? 0.5f : 0.f) + (kx == i && i >= lowest ? 0.5f : 0.f);
-      const float2 cap = make_float2(nx > 0.f ? nx * eL.x : 0.f, ky == i ? 0.5f * eL.y : 0.f);
-      W[j] = add2(W[j], cap);
-      z2 = add2(z2, cap);
-    }
   }
 #pragma unroll
   for (int j = NJ - 1; j >= 1; --j) W[j] = add2(W[j], M1[j - 1]);
@@ -171,27 +201,62 @@ __device__ __forceinline__ void weigh(const float2 (&raw)[NJ], float scale, floa
   last = M1[NJ - 1].y;
 }
 
+// The half caps of keys 0 and i, where this run weighs them (keys kc - 1 .. kc + 2 NJ - 2).  Key i's belongs
+// to this piece when i >= lowest: the piece before it has weighed its own last key to the end.
+template <int NJ>
+__device__ __forceinline__ void add_caps(const float2 (&sv)[NJ], float m2, float sL, int kc, int i, int lowest,
+                                         float2 (&W)[NJ], float2& z2) {
+  if (kc == 0 && i >= 0) {
+    const float cap = 0.5f * ex2_approx(fmaf(sv[0].x, kLog2e, -m2));
+    W[1].x += cap;
+    z2.x += cap;
+  }
+  const int t = i - kc + 1;     // key i's place
+  if (t < 0 || t >= 2 * NJ || i < lowest) return;
+  float si = sL;
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    if (t == j + 1) si = sv[j].x;
+    if (t == j + NJ + 1) si = sv[j].y;
+  }
+  const float cap = 0.5f * ex2_approx(fmaf(si, kLog2e, -m2));
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    W[j].x += t == j ? cap : 0.f;
+    W[j].y += t == j + NJ ? cap : 0.f;
+  }
+  z2.x += cap;
+}
+
 // ------------------------------------------------------------------ the kernel
 
-// RPW rows per warp (8 or 16), RW warps that share a ring (1 or 4), GROUPS rings per block,
-// NST stages of TK keys of DP (padded) values
-template <typename T, int DP_, int RPW_, int RW_, int GROUPS_, int NST_>
+// RPW rows per warp (8 or 16), RW warps that share a ring (1 or 4), GROUPS rings per block, NST stages of
+// TK keys of DP (padded) values, AHEAD of which are filled before they are needed; BPS blocks per SM
+template <int DP_, int TK_, int RPW_, int RW_, int GROUPS_, int NST_, int BPS_>
 struct Config {
-  static constexpr int DP = DP_, TK = DP_ == 64 ? 64 : 32, RPW = RPW_, RW = RW_, GROUPS = GROUPS_, NST = NST_;
+  static constexpr int DP = DP_, TK = TK_, RPW = RPW_, RW = RW_, GROUPS = GROUPS_, NST = NST_, BPS = BPS_;
+  // one warp refills the stage it has just left; several are given a tile's time to leave theirs
+  static constexpr int AHEAD = RW == 1 ? NST - 1 : NST - 2;
   static constexpr int NT = RW * 32;                    // threads of a group
   static constexpr int BR = RPW * RW;                   // rows of a unit
   static constexpr int NJ = TK / 8;                     // score tiles of 8 keys; half a lane's run
   static constexpr int CH = DP / 8;                     // 16-byte chunks of a row
   static constexpr int ROWB = DP * 2;
+  static constexpr int PITCH = NJ * ROWB + 16;          // of NJ rows
+  static constexpr int KV_BYTES = 8 * PITCH;
   static constexpr bool kStageQ = RW == 1 && RPW == 8 && DP == 64;   // as far as shared memory goes
-  static constexpr int KV_BYTES = (TK + 1) * ROWB;      // row TK: the halo
-  static constexpr int Q_BYTES = kStageQ ? RPW * ROWB : 0;
-  static constexpr int STAGE = 2 * KV_BYTES + Q_BYTES;
-  static constexpr int RING = NST + 1;                  // descriptors and row offsets live one tile longer
-  static constexpr int OFFS = TK + 1;
-  static constexpr int GROUP_BYTES = NST * STAGE + RING * (OFFS * 8 + 40);
-  static constexpr int GROUP_STRIDE = (GROUP_BYTES + 255) / 256 * 256;
+  static constexpr int HALO = 2 * KV_BYTES;             // K row, then V row before the tile
+  static constexpr int Q_AT = HALO + 2 * ROWB;
+  static constexpr int STAGE = Q_AT + (kStageQ ? RPW * ROWB : 0);
+  static constexpr int RING = NST + 1;                  // descriptors live one tile longer
+  // behind the stages: each warp's V row of the tile before (in the banks that the fragments leave free),
+  // descriptors, barriers, the flag of a wait that gave up
+  static constexpr int WARP_HALO = ROWB + 128;
+  static constexpr int DESC_AT = NST * STAGE + RW * WARP_HALO;
+  static constexpr int BAR_AT = DESC_AT + RING * 48;
+  static constexpr int GROUP_STRIDE = (BAR_AT + 2 * NST * 8 + 16 + 127) / 128 * 128;
   static constexpr int SMEM = GROUPS * GROUP_STRIDE;    // and the prefix sums behind it
+  static_assert(KV_BYTES % 128 == 0 && STAGE % 128 == 0 && DESC_AT % 16 == 0, "");
 };
 
 struct Desc {   // one tile of the stream
@@ -199,19 +264,15 @@ struct Desc {   // one tile of the stream
   int first, last;    // of the piece
   int start, n, len;  // the sequence
   int h, rt;          // key head, row tile
-  int bad;            // the sequence's length is out of range
+  int bad;            // the sequence's length or one of the tile's pages is out of range
+  int fill[2];
 };
-static_assert(sizeof(Desc) == 40, "");
-
-template <int RW>
-__device__ __forceinline__ void group_sync() {
-  if constexpr (RW == 1) __syncwarp();
-  else __syncthreads();
-}
+static_assert(sizeof(Desc) == 48, "");
 
 template <typename T, typename C>
-__global__ void __launch_bounds__(C::NT* C::GROUPS, C::RW == 1 ? 1 : 3)
-    mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Plan plan, float* __restrict__ part_o, float2* __restrict__ part_mz, Meta* __restrict__ meta) {
+__global__ void __launch_bounds__(C::NT* C::GROUPS, C::BPS)
+    mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Plan plan, float* __restrict__ part_o,
+               float2* __restrict__ part_mz, Meta* __restrict__ meta) {
   extern __shared__ __align__(1024) uint8_t smem[];
   pdl_wait();
   pdl_launch_dependents();
@@ -219,52 +280,57 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::RW == 1 ? 1 : 3)
   constexpr int NKK = DP / 16;                 // k-steps of Q K^T
   constexpr int NN = DP / 8;                   // column tiles of the output
   const int lane = threadIdx.x & 31, c4 = lane & 3, r8 = lane >> 2;
-  const int group = threadIdx.x / C::NT, gt = threadIdx.x % C::NT, warp = gt >> 5;
+  const int group = threadIdx.x / C::NT, warp = (threadIdx.x % C::NT) >> 5;
   unsigned* prefix = reinterpret_cast<unsigned*>(smem + C::SMEM);
+  uint8_t* gsm = smem + (size_t)group * C::GROUP_STRIDE;
+  const uint32_t g0 = smem_addr(gsm);
+  Desc* descs = reinterpret_cast<Desc*>(gsm + C::DESC_AT);
+  const uint32_t full = g0 + C::BAR_AT, empty = full + 8 * NST;
+  volatile int* gave_up = reinterpret_cast<volatile int*>(gsm + C::BAR_AT + 16 * NST);
 
-  Schedule<C::BR, TK> sched(a, plan, prefix);
+  if (warp == 0 && lane == 0) {
+    for (int i = 0; i < NST; ++i) {
+      bar_init(full + 8 * i, 1);
+      bar_init(empty + 8 * i, C::RW);
+    }
+    *gave_up = 0;
+  }
+  // values behind D stay 0 (copies write D values a row)
+  if (a.D < DP) {
+    for (int x = (int)(threadIdx.x % C::NT); x < NST * C::STAGE / 16; x += C::NT)
+      *reinterpret_cast<uint4*>(gsm + 16 * x) = make_uint4(0u, 0u, 0u, 0u);
+  }
+  fence_async();
+  Schedule<C::BR, TK> sched(a, plan, prefix);   // a barrier of the block among other things
   const unsigned total = sched.total;
   const int worker = blockIdx.x * C::GROUPS + group, workers = gridDim.x * C::GROUPS;
   const unsigned per = plan.tiles_per_worker(total, workers);
   const unsigned long long x0l = (unsigned long long)worker * per;
   if (x0l >= total) {
-    if (gt == 0) meta[worker].pieces = 0;
+    if (warp == 0 && lane == 0) meta[worker].pieces = 0;
     return;
   }
   const unsigned x0 = (unsigned)x0l, x1 = min(total, x0 + per);
 
-  uint8_t* gsm = smem + (size_t)group * C::GROUP_STRIDE;
-  long long* offs_ring = reinterpret_cast<long long*>(gsm + NST * C::STAGE);
-  Desc* desc_ring = reinterpret_cast<Desc*>(offs_ring + C::RING * C::OFFS);
+  // ---- the loader, the group's first warp: `cur` stands at tile xa, the next to be described, whose pages
+  // are fetched a tile before its copies are issued
+  typename Schedule<C::BR, TK>::Cursor cur;
+  unsigned xa = x0, xb = x0;      // next to be described; next to be copied
+  int slot_a = 0, slot_b = 0, stage_b = 0;
+  uint32_t empty_parity = 1;      // of the stages' previous use: the first one needs no wait
+  constexpr int NP = TK / 32;
+  int pg[NP];
 
-  // ---- the loader's side: where the stream's next tile lies
-  typename Schedule<C::BR, TK>::Cursor cur = sched.locate(x0);
-  unsigned xa = x0;          // the tile `cur` stands at: the next to be described
-  int slot_a = 0;            // xa % RING
-  unsigned xb = x0;          // the next tile to be copied
-  int slot_b = 0, stage_b = 0;
-
-  // describe tile xa: its rows' offsets in the cache (keys a-1 .. a+TK-1; -1: none, -2: bad page)
   auto describe = [&]() {
     if (xa < x1) {
-      const int base = cur.kt * TK;
-      for (int r = gt; r < C::OFFS; r += C::NT) {
-        const int key = base - 1 + r;
-        long long off = -1;
-        if (key >= 0 && key < cur.len) {
-          const int col = plan.page_of(key);
-          const int page = a.page_table[(size_t)cur.s * a.page_table_stride + col];
-          if (page < 0 || page >= a.num_pages) {
-            off = -2;
-            record_invalid();
-          } else {
-            off = (long long)page * a.page_stride + (long long)cur.h * a.head_stride +
-                  (long long)(key - col * a.page_size) * a.slot_stride;
-          }
-        }
-        offs_ring[slot_a * C::OFFS + r] = off;
+#pragma unroll
+      for (int k = 0; k < NP; ++k) {
+        const int row = plan.unit_rows == 1 ? lane + 32 * k : (k == 0 && lane < 8 ? lane * NJ : TK);
+        const int key = cur.kt * TK + row;
+        pg[k] = -1;
+        if (row < TK && key < cur.len) pg[k] = a.page_table[(size_t)cur.s * a.page_table_stride + plan.page_of(key)];
       }
-      if (gt == 0) {
+      if (lane == 0) {
         Desc d;
         d.kt = cur.kt;
         d.nt = cur.nt;
@@ -276,100 +342,147 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::RW == 1 ? 1 : 3)
         d.h = cur.h;
         d.rt = cur.rt;
         d.bad = cur.bad;
-        desc_ring[slot_a] = d;
+        // the page of the key before the piece
+        d.fill[0] = d.first && cur.kt > 0
+                        ? a.page_table[(size_t)cur.s * a.page_table_stride + plan.page_of(cur.kt * TK - 1)] : -1;
+        descs[slot_a] = d;
       }
       if (xa + 1 < x1) sched.advance(cur);
     }
     ++xa;
     if (++slot_a == C::RING) slot_a = 0;
+    __syncwarp();
   };
 
-  // copy tile xb into its stage
-  auto copy = [&]() {
+  auto cache_at = [&](int page, int h, int key) {
+    return (size_t)page * a.page_stride + (size_t)h * a.head_stride +
+           (size_t)(key - plan.page_of(key) * a.page_size) * a.slot_stride;
+  };
+
+  auto issue = [&]() {
     if (xb < x1) {
-      const long long* offs = offs_ring + slot_b * C::OFFS;
-      const Desc& d = desc_ring[slot_b];
-      const uint32_t ks = smem_addr(gsm + stage_b * C::STAGE), vs = ks + C::KV_BYTES;
-      const T* kc = (const T*)a.k_cache + (gt % CH) * 8;
-      const T* vc = (const T*)a.v_cache + (gt % CH) * 8;
-      const bool pad = (gt % CH) * 8 >= a.D;
-      const int ch = gt % CH;
-#pragma unroll 8
-      for (int r = gt / CH; r < TK; r += C::NT / CH) {
-        const long long ov = offs[r], ok = offs[r + 1];
-        const uint32_t dst = (uint32_t)r * ROWB + (uint32_t)((ch ^ (r / NJ)) << 4);
-        cp_async16(ks + dst, ok < -1 ? (const void*)&g_nan16 : (const void*)(kc + (ok < 0 ? 0 : ok)), ok == -1 || pad);
-        cp_async16(vs + dst, ov < -1 ? (const void*)&g_nan16 : (const void*)(vc + (ov < 0 ? 0 : ov)), ov == -1 || pad);
+      Desc& d = descs[slot_b];
+      const uint32_t st = g0 + stage_b * C::STAGE, bar = full + 8 * stage_b;
+      const int base = d.kt * TK, len = d.len, h = d.h, first = d.first;
+      const uint32_t row_bytes = (uint32_t)a.D * 2;
+      const uint32_t unit_bytes = plan.unit_rows * row_bytes;
+      bool go[NP], bad = false;
+      uint32_t bytes = 0;
+#pragma unroll
+      for (int k = 0; k < NP; ++k) {
+        const int row = plan.unit_rows == 1 ? lane + 32 * k : (k == 0 && lane < 8 ? lane * NJ : TK);
+        go[k] = row < TK && base + row < len;
+        const bool in = pg[k] >= 0 && pg[k] < a.num_pages;
+        bad |= go[k] && !in;
+        go[k] = go[k] && in;
+        bytes += __popc(__ballot_sync(0xffffffffu, go[k])) * 2 * unit_bytes;
       }
-      if (gt < CH) {
-        if (d.first) {
-          const long long ok = offs[0];
-          cp_async16(ks + TK * ROWB + (ch << 4), ok < -1 ? (const void*)&g_nan16 : (const void*)(kc + (ok < 0 ? 0 : ok)),
-                     ok == -1 || pad);
-        }
-        if (d.last) {
-          const long long ov = offs[TK];
-          cp_async16(vs + TK * ROWB + (ch << 4), ov < -1 ? (const void*)&g_nan16 : (const void*)(vc + (ov < 0 ? 0 : ov)),
-                     ov == -1 || pad);
-        }
-      }
+      const int halo_page = d.fill[0];
+      const bool halo = first && base > 0 && base - 1 < len;
+      const bool halo_go = halo && halo_page >= 0 && halo_page < a.num_pages;
+      bad |= halo && !halo_go;
+      if (halo_go) bytes += 2 * row_bytes;
+      int q_row = -1;
       if constexpr (C::kStageQ) {
-        if (d.first) {
-          for (int x = gt; x < C::RPW * CH; x += C::NT) {
-            const int r = x / CH, q = x % CH;
-            const int row = d.rt * C::BR + r;
-            const bool none = row >= d.n * plan.group || q * 8 >= a.D;
-            const int t = none ? 0 : row / plan.group, hh = none ? 0 : row - t * plan.group;
-            const T* src = (const T*)a.q + (none ? 0 : (size_t)(d.start + t) * a.q_token_stride +
-                                                          (size_t)(d.h * plan.group + hh) * a.q_head_stride + q * 8);
-            cp_async16(vs + C::KV_BYTES + r * ROWB + (q << 4), src, none);
-          }
+        if (first && lane < C::RPW && d.rt * C::BR + lane < d.n * plan.group) q_row = d.rt * C::BR + lane;
+        bytes += __popc(__ballot_sync(0xffffffffu, q_row >= 0)) * row_bytes;
+      }
+      bad = __any_sync(0xffffffffu, bad);
+      if (lane == 0) {
+        if (bad) {
+          d.bad = 1;
+          record_invalid();
         }
+        bar_expect(bar, bytes);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int k = 0; k < NP; ++k) {
+        if (go[k]) {
+          const int row = plan.unit_rows == 1 ? lane + 32 * k : lane * NJ;
+          const size_t at = cache_at(pg[k], h, base + row);
+          const uint32_t dst = st + (row / NJ) * C::PITCH + (row % NJ) * ROWB;
+          bulk_load(dst, (const T*)a.k_cache + at, unit_bytes, bar);
+          bulk_load(dst + C::KV_BYTES, (const T*)a.v_cache + at, unit_bytes, bar);
+        }
+      }
+      if (halo_go && lane == 31) {
+        const size_t at = cache_at(halo_page, h, base - 1);
+        bulk_load(st + C::HALO, (const T*)a.k_cache + at, row_bytes, bar);
+        bulk_load(st + C::HALO + ROWB, (const T*)a.v_cache + at, row_bytes, bar);
+      }
+      if (q_row >= 0) {
+        const int t = q_row / plan.group;
+        bulk_load(st + C::Q_AT + lane * ROWB,
+                  (const T*)a.q + (size_t)(d.start + t) * a.q_token_stride +
+                      (size_t)(h * plan.group + q_row - t * plan.group) * a.q_head_stride,
+                  row_bytes, bar);
       }
     }
-    cp_commit();
     ++xb;
     if (++slot_b == C::RING) slot_b = 0;
-    if (++stage_b == NST) stage_b = 0;
+    if (++stage_b == NST) {
+      stage_b = 0;
+      empty_parity ^= 1;
+    }
   };
 
-  // ---- the consumer's state
+  if (warp == 0) {
+    cur = sched.locate(x0);
+    describe();
+    for (int i = 0; i < C::AHEAD; ++i) {
+      issue();
+      describe();
+    }
+  }
+
+  // ---- the consumers' state
   constexpr int RS = C::RPW == 8 ? 1 : 2;      // row sets per lane: rows r8 (and r8 + 8)
   uint32_t qf[NKK][4];
   float o[NN][4];
   float m[RS], carry_s[RS], carry_b[RS], scale[RS];
   float2 z2[RS];
   int pos[RS];
-  int i_min = 0, i_max = -1, kt0 = 0;
+  int i_min = 0, i_max = -1, kt0 = 0, piece_bad = 0;
   bool in_first = true;                         // the piece starts the worker's range
 
-  // lanes' addresses within a stage: B fragments of K (score tile j: + j rows) and of V
+  // lanes' addresses within a stage: B fragments of K (score tile j: + j rows) and of V (k-step kk: + 2 kk
+  // rows, one row early; place 0 of a run is the row before it)
   const int mi = lane >> 3, rr = lane & 7;
-  const uint32_t k_lane = (uint32_t)((2 * NJ * (rr >> 1) + NJ * (rr & 1)) * ROWB + ((mi ^ rr) << 4));
-  const uint32_t v_lane = (uint32_t)((2 * NJ * (rr >> 1) + NJ * (rr & 1) + (mi & 1)) * ROWB + (((mi >> 1) ^ rr) << 4));
-
-  describe();
-  group_sync<C::RW>();
-#pragma unroll
-  for (int i = 0; i < NST - 1; ++i) {
-    copy();
-    describe();
-    group_sync<C::RW>();
-  }
+  const uint32_t k_lane = (uint32_t)(rr * C::PITCH + mi * 16);
+  const uint32_t v_lane = (uint32_t)(C::KV_BYTES + rr * C::PITCH + ((mi & 1) - 1) * ROWB + (mi >> 1) * 16);
+  const uint32_t my_halo = g0 + NST * C::STAGE + warp * C::WARP_HALO + 112;
+  uint8_t* my_halo_p = gsm + NST * C::STAGE + warp * C::WARP_HALO + 112;
 
   int slot = 0, stage = 0;
-  for (unsigned x = x0; x < x1; ++x) {
-    cp_wait<NST - 2>();
-    group_sync<C::RW>();     // this tile has arrived, and every warp has left the stage filled next
-    copy();
-    describe();
+  uint32_t parity = 0;
+  bool alive = true;
+  unsigned x = x0;
+  for (; x < x1; ++x) {
+    if constexpr (C::RW > 1) {
+      if (warp == 0) {
+        // tile x + AHEAD goes where tile x - 2 was; every warp has to have left it
+        if (xb < x1 && xb >= x0 + NST) alive = bar_wait(empty + 8 * stage_b, empty_parity, gave_up);
+        if (!alive) break;
+        issue();
+        describe();
+      }
+    }
+    alive = bar_wait(full + 8 * stage, parity, gave_up);
+    if (!alive) break;
+    if constexpr (C::RW == 1) {
+      issue();             // into the stage that this warp has just left
+      describe();
+    }
 
-    const Desc& d = desc_ring[slot];
-    const uint32_t ks = smem_addr(gsm + stage * C::STAGE), vs = ks + C::KV_BYTES;
+    const Desc& d = descs[slot];
+    uint8_t* sm = gsm + stage * C::STAGE;
+    const uint32_t st = g0 + stage * C::STAGE;
     const int base = d.kt * TK;
     const int rows = d.n * plan.group;
     if (d.first) {
       kt0 = d.kt;
+      piece_bad = 0;
       in_first = x == x0;
       const int row0 = d.rt * C::BR + warp * C::RPW;
       const int row_last = min(rows, row0 + C::RPW) - 1;    // < row0: the warp has no row
@@ -387,7 +500,8 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::RW == 1 ? 1 : 3)
         scale[u] = expf(a.log_gain[head]) * a.inv_sqrt_d;
         m[u] = -INFINITY;
         z2[u] = splat2(0.f);
-        carry_s[u] = carry_b[u] = 0.f;
+        carry_s[u] = kMasked;
+        carry_b[u] = 0.f;
         qrow[u] = none ? nullptr : (const T*)a.q + (size_t)(d.start + t) * a.q_token_stride +
                                        (size_t)head * a.q_head_stride;
       }
@@ -396,7 +510,7 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::RW == 1 ? 1 : 3)
 #pragma unroll
       for (int k = 0; k < NKK; ++k) {
         if constexpr (C::kStageQ) {
-          const uint8_t* qs = gsm + stage * C::STAGE + 2 * C::KV_BYTES + r8 * ROWB + (16 * k + 2 * c4) * 2;
+          const uint8_t* qs = sm + C::Q_AT + r8 * ROWB + (16 * k + 2 * c4) * 2;
           qf[k][0] = *reinterpret_cast<const uint32_t*>(qs);
           qf[k][2] = *reinterpret_cast<const uint32_t*>(qs + 16);
           qf[k][1] = qf[k][3] = 0u;
@@ -415,58 +529,75 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::RW == 1 ? 1 : 3)
       if (d.kt > 0 && base - 1 <= i_max) {
         // the score of key base - 1, in every column of one score tile
         float s[4] = {0.f, 0.f, 0.f, 0.f};
-        const uint32_t addr = ks + TK * ROWB + (mi << 4);
 #pragma unroll
         for (int kp = 0; kp < NKK / 2; ++kp) {
           uint32_t b[4];
-          ldsm4(b, addr + (kp << 6));
+          ldsm4(b, st + C::HALO + mi * 16 + kp * 64);
           mma<T>(s, qf[2 * kp][0], qf[2 * kp][1], qf[2 * kp][2], qf[2 * kp][3], b[0], b[1]);
           mma<T>(s, qf[2 * kp + 1][0], qf[2 * kp + 1][1], qf[2 * kp + 1][2], qf[2 * kp + 1][3], b[2], b[3]);
         }
 #pragma unroll
         for (int u = 0; u < RS; ++u) {
-          carry_s[u] = s[2 * u] * scale[u];
-          if (base - 1 <= pos[u]) m[u] = carry_s[u];
+          if (base - 1 <= pos[u]) m[u] = carry_s[u] = s[2 * u] * scale[u];
         }
       }
+      if (lane < CH)
+        *reinterpret_cast<uint4*>(my_halo_p + 16 * lane) =
+            d.kt > 0 ? *reinterpret_cast<const uint4*>(sm + C::HALO + ROWB + 16 * lane) : make_uint4(0u, 0u, 0u, 0u);
     }
+    piece_bad |= d.bad;
+    if (base + TK > d.len) {
+      // V behind the sequence's end may hold anything, and 0 times it has to be 0.  The warps of a group
+      // write the same zeros.
+      for (int r = max(d.len - base, 0) * CH + lane; r < TK * CH; r += 32) {
+        const int row = r / CH;
+        *reinterpret_cast<uint4*>(sm + C::KV_BYTES + (row / NJ) * C::PITCH + (row % NJ) * ROWB + (r % CH) * 16) =
+            make_uint4(0u, 0u, 0u, 0u);
+      }
+      fence_async();
+    }
+    __syncwarp();
 
     // a warp none of whose rows sees a segment of this tile, or its first weight, has nothing to do
     if (base - 1 <= i_max && i_max >= 0) {
       float2 s[RS][NJ];
+      const uint32_t ka = st + k_lane;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int kp = 0; kp < NKK / 2; ++kp) {
           uint32_t b[4];
-          ldsm4(b, (ks + k_lane + j * ROWB) ^ (kp << 6));
+          ldsm4(b, ka + j * ROWB + kp * 64);
           mma<T>(acc, qf[2 * kp][0], qf[2 * kp][1], qf[2 * kp][2], qf[2 * kp][3], b[0], b[1]);
           mma<T>(acc, qf[2 * kp + 1][0], qf[2 * kp + 1][1], qf[2 * kp + 1][2], qf[2 * kp + 1][3], b[2], b[3]);
         }
 #pragma unroll
-        for (int u = 0; u < RS; ++u) s[u][j] = make_float2(acc[2 * u], acc[2 * u + 1]);
+        for (int u = 0; u < RS; ++u) s[u][j] = mul2(make_float2(acc[2 * u], acc[2 * u + 1]), splat2(scale[u]));
       }
+      // keys beyond a row's own, or caps among the weights
       const bool edge = base == 0 || base + TK - 1 > i_min;
       const int kc = base + 2 * NJ * c4;        // first key of the lane's run
-      const int lowest = d.first ? base : base - 1;
+      if (edge) {
+#pragma unroll
+        for (int u = 0; u < RS; ++u) {
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) {
+            if (kc + j > pos[u]) s[u][j].x = kMasked;
+            if (kc + NJ + j > pos[u]) s[u][j].y = kMasked;
+          }
+        }
+      }
       uint32_t hi[RS][NJ], lo[RS][NJ];
 #pragma unroll
       for (int u = 0; u < RS; ++u) {
-        float top = -INFINITY;
-        if (edge) {
+        float top = max3f(s[u][0].x, s[u][0].y, s[u][1].x);
+        top = fmaxf(top, s[u][1].y);
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            if (kc + j <= pos[u]) top = fmaxf(top, s[u][j].x);
-            if (kc + NJ + j <= pos[u]) top = fmaxf(top, s[u][j].y);
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) top = max3f(top, s[u][j].x, s[u][j].y);
-        }
+        for (int j = 2; j < NJ; ++j) top = max3f(top, s[u][j].x, s[u][j].y);
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * scale[u];
-        const bool move = top > m[u] + kRescaleNats || (m[u] == -INFINITY && top > -INFINITY);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const bool move = top > kMasked && top > m[u] + kRescaleNats;
         if (__any_sync(0xffffffffu, move)) {
           const float to = move ? top : m[u];
           const float f = move ? exp_rel(m[u] - to) : 1.f;
@@ -485,25 +616,28 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::RW == 1 ? 1 : 3)
         }
         const float m2 = m[u] == -INFINITY ? 0.f : m[u] * kLog2e;
         const int left = (lane & ~3) | ((lane + 3) & 3);
-        float got = __shfl_sync(0xffffffffu, s[u][NJ - 1].y * scale[u], left);
+        float got = __shfl_sync(0xffffffffu, s[u][NJ - 1].y, left);
         const float sL = c4 == 0 ? carry_s[u] : got;
-        if (c4 == 0) carry_s[u] = got;
+        carry_s[u] = got;                       // of use to the quad's first lane only
         float2 W[NJ];
         float last;
-        if (edge) weigh<true, NJ>(s[u], scale[u], m2, kc, pos[u], lowest, sL, W, last, z2[u]);
-        else weigh<false, NJ>(s[u], scale[u], m2, kc, pos[u], lowest, sL, W, last, z2[u]);
+        weigh<NJ>(s[u], m2, sL, W, last, z2[u]);
+        if (edge) add_caps<NJ>(s[u], m2, sL, kc, pos[u], d.first ? base : base - 1, W, z2[u]);
         got = __shfl_sync(0xffffffffu, last, left);
         W[0].x += c4 == 0 ? carry_b[u] : got;
-        if (c4 == 0) carry_b[u] = got;
+        carry_b[u] = got;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) split2<T>(W[j], hi[u][j], lo[u][j]);
       }
+      const uint32_t va = st + v_lane;
+      const uint32_t va0 = lane == 0 || lane == 16 ? my_halo + (mi >> 1) * 16
+                           : (mi & 1) || rr == 0 ? va : va - C::PITCH + NJ * ROWB;
 #pragma unroll
       for (int kk = 0; kk < TK / 16; ++kk) {
 #pragma unroll
         for (int np = 0; np < NN / 2; ++np) {
           uint32_t b[4];
-          ldsm4_t(b, (vs + v_lane + 2 * kk * ROWB) ^ (np << 5));
+          ldsm4_t(b, (kk == 0 ? va0 : va + 2 * kk * ROWB) + np * 32);
           if constexpr (RS == 1) {
             mma<T>(o[2 * np], hi[0][2 * kk], lo[0][2 * kk], hi[0][2 * kk + 1], lo[0][2 * kk + 1], b[0], b[1]);
             mma<T>(o[2 * np + 1], hi[0][2 * kk], lo[0][2 * kk], hi[0][2 * kk + 1], lo[0][2 * kk + 1], b[2], b[3]);
@@ -519,6 +653,7 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::RW == 1 ? 1 : 3)
       }
     }
 
+    const uint8_t* vlast = sm + C::KV_BYTES + 7 * C::PITCH + (NJ - 1) * ROWB;   // V of the tile's last key
     if (d.last) {
       const bool whole = kt0 == 0 && d.kt + 1 == d.nt;
       const int row0 = d.rt * C::BR + warp * C::RPW;
@@ -535,15 +670,13 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::RW == 1 ? 1 : 3)
         float z = z2[u].x + z2[u].y + (c4 == 0 ? cap : 0.f);
         z += __shfl_xor_sync(0xffffffffu, z, 1);
         z += __shfl_xor_sync(0xffffffffu, z, 2);
-        if (d.bad) z = __int_as_float(0x7fffffff);
+        if (piece_bad) z = __int_as_float(0x7fffffff);
         if (row >= rows) continue;
         const bool seen = key <= pos[u];         // else the weight is 0, and V may hold anything
         const int t = row / plan.group;
         T* dst = (T*)a.o + ((size_t)(d.start + t) * a.H + (size_t)d.h * plan.group + (row - t * plan.group)) * a.D;
         float* po = part_o + (slot_row + r8 + 8 * u) * DP;
-        // z = 0: the row sees no key
         const float inv = 1.f / z;
-        const uint8_t* vrow = gsm + stage * C::STAGE + C::KV_BYTES + TK * ROWB + 4 * c4;
 #pragma unroll
         for (int n = 0; n < NN; ++n) {
           const int col = 8 * n + 2 * c4;
@@ -553,11 +686,12 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::RW == 1 ? 1 : 3)
             y.y += o[n][3];
           }
           if (seen) {
-            const float2 v = unpack2<T>(*reinterpret_cast<const uint32_t*>(vrow + 16 * n));
+            const float2 v = unpack2<T>(*reinterpret_cast<const uint32_t*>(vlast + 4 * c4 + 16 * n));
             y.x = fmaf(w, v.x, y.x);
             y.y = fmaf(w, v.y, y.y);
           }
           if (whole) {
+            // z = 0: the row sees no key
             if (col < a.D) *reinterpret_cast<uint32_t*>(dst + col) = z == 0.f ? 0u : pack2<T>(y.x * inv, y.y * inv);
           } else {
             *reinterpret_cast<float2*>(po + col) = y;
@@ -565,8 +699,11 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::RW == 1 ? 1 : 3)
         }
         if (!whole && c4 == 0) part_mz[slot_row + r8 + 8 * u] = make_float2(m[u], z);
       }
+    } else {
+      __syncwarp();
+      if (lane < CH) *reinterpret_cast<uint4*>(my_halo_p + 16 * lane) = *reinterpret_cast<const uint4*>(vlast + 16 * lane);
     }
-    if (x + 1 == x1 && gt == 0) {
+    if (x + 1 == x1 && warp == 0 && lane == 0) {
       // this worker joins the unit that starts in its range and goes on behind it
       Meta mt;
       mt.pieces = kt0 == 0 && d.kt + 1 < d.nt ? 1 + (d.nt - d.kt - 2 + (int)per) / (int)per : 0;
@@ -577,10 +714,34 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::RW == 1 ? 1 : 3)
       mt.rt = d.rt;
       meta[worker] = mt;
     }
+    __syncwarp();
+    if constexpr (C::RW > 1) {
+      if (lane == 0) bar_arrive(empty + 8 * stage);
+    }
     if (++slot == C::RING) slot = 0;
-    if (++stage == NST) stage = 0;
+    if (++stage == NST) {
+      stage = 0;
+      parity ^= 1;
+    }
   }
-  cp_wait<0>();
+  if (!alive) {
+    // copies of tiles x .. xb - 1 may still be on their way: leave no sooner than they land, or a second
+    // limit runs out
+    if (warp == 0) {
+      if (lane == 0) {
+        meta[worker].pieces = 0;
+        *gave_up = 0;
+      }
+      __syncwarp();
+      for (; x < x1 && x < xb; ++x) {
+        bar_wait(full + 8 * stage, parity, gave_up);
+        if (++stage == NST) {
+          stage = 0;
+          parity ^= 1;
+        }
+      }
+    }
+  }
 }
 
 // Joins the pieces of a cut unit in the order of their keys: piece 0 is in this worker's slot, the others
@@ -631,9 +792,9 @@ __global__ void __launch_bounds__(128) merge_kernel(Args a, int group, const flo
 namespace {
 
 // The forms: decoding with 8 or 16 rows a warp, and chunks
-template <typename T, int DP> using Decode8 = Config<T, DP, 8, 1, 4, 3>;
-template <typename T, int DP> using Decode16 = Config<T, DP, 16, 1, 4, 3>;
-template <typename T, int DP> using Chunk = Config<T, DP, 16, 4, 1, 3>;
+template <int DP> using Decode8 = Config<DP, DP == 64 ? 64 : 32, 8, 1, 4, 3, 1>;
+template <int DP> using Decode16 = Config<DP, DP == 64 ? 64 : 32, 16, 1, 4, 3, 1>;
+template <int DP> using Chunk = Config<DP, DP == 64 ? 64 : 32, 16, 4, 1, 4, 3>;
 
 size_t part_bytes(long long workers, int br, int dp) {
   return (size_t)workers * 2 * br * (dp * sizeof(float) + sizeof(float2)) + (size_t)workers * sizeof(Meta) + 768;
@@ -653,7 +814,8 @@ cudaError_t launch(const Args& a, Plan plan, void* workspace) {
     if (e != cudaSuccess) return e;
     set_dev = dev;
   }
-  const int blocks = num_sms_cached() * (C::RW == 1 ? 1 : kChunkBlocksPerSM);
+  const int blocks = num_sms_cached() * C::BPS;
+  plan.unit_rows = a.D == C::DP && a.slot_stride == C::DP && a.page_size % C::NJ == 0 ? C::NJ : 1;
   const long long workers = (long long)blocks * C::GROUPS;
   char* ws = (char*)workspace;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
@@ -672,27 +834,33 @@ cudaError_t forward_dp(const Args& a, void* workspace) {
   const long long rows = (long long)a.max_q_len * plan.group;
   if (rows <= 16) {
     // every sequence, whatever its rows: max_q_len may be wrong
-    return rows <= 8 ? launch<T, Decode8<T, DP>>(a, plan, workspace) : launch<T, Decode16<T, DP>>(a, plan, workspace);
+    return rows <= 8 ? launch<T, Decode8<DP>>(a, plan, workspace) : launch<T, Decode16<DP>>(a, plan, workspace);
   }
   // sequences of up to 16 rows in the decoding form, the others as chunks; both use the workspace, one
   // after the other
   plan.min_tiles = 4;
   plan.row_lo = 17;
-  cudaError_t e = launch<T, Chunk<T, DP>>(a, plan, workspace);
+  cudaError_t e = launch<T, Chunk<DP>>(a, plan, workspace);
   if (e != cudaSuccess || a.seqs == 1) return e;
   plan.min_tiles = 1;
   plan.row_lo = 0;
   plan.row_hi = 16;
-  return launch<T, Decode16<T, DP>>(a, plan, workspace);
+  return launch<T, Decode16<DP>>(a, plan, workspace);
 }
 
 }  // namespace
 
 size_t mma_workspace_bytes(long long max_q_len, long long H, long long G, long long D) {
-  const int dp = D <= 64 ? 64 : 128;
-  const long long sms = num_sms_cached(), rows = max_q_len * (H / G);
-  const size_t decode = part_bytes(sms * 4, 16, dp);
-  return rows <= 16 ? decode : std::max(decode, part_bytes(sms * kChunkBlocksPerSM, 64, dp));
+  const long long rows = max_q_len * (H / G);
+  auto bytes = [&](auto d8, auto d16, auto chunk) {
+    auto part = [](auto c) {
+      using C = decltype(c);
+      return part_bytes((long long)num_sms_cached() * C::BPS * C::GROUPS, C::BR, C::DP);
+    };
+    const size_t decode = std::max(part(d8), part(d16));
+    return rows <= 16 ? decode : std::max(decode, part(chunk));
+  };
+  return D <= 64 ? bytes(Decode8<64>{}, Decode16<64>{}, Chunk<64>{}) : bytes(Decode8<128>{}, Decode16<128>{}, Chunk<128>{});
 }
 
 cudaError_t mma_read_status(int* out, bool reset) {
