@@ -9,9 +9,11 @@
 // directly; the pieces of a cut one (row maximum, mass, accumulator, all fp32) go to the
 // workspace and merge_kernel joins them in order, so results do not depend on timing.
 //
-// A worker of the decoding form is one warp with up to 16 rows: four run on an SM, each
-// with a ring of its own, and no barrier couples them.  The form for chunks is a block of
-// four warps with 16 rows each that share the ring.
+// A worker is RW consumer warps with 16 (or 8) rows each that share a ring of key tiles, and
+// one producer warp that walks the stream ahead of them: it looks pages up, issues the copies
+// and describes each tile.  With the copies in the consumers' own hands their warp 0 did a
+// third more work than the others, who waited for it at every tile.  In the decoding form
+// a worker has one consumer and 8 or 16 rows, for chunks four and 64 rows.
 //
 // Cutting keys.  Segments, not keys, are divided: the segment from key j-1 to key j belongs
 // to the tile of j.  A tile of keys a .. a+TK-1 therefore weighs keys a-1 .. a+TK-2, and only
@@ -36,6 +38,7 @@
 // each NJ rows (512 or 1024 bytes) are one bulk copy where the page holds them in one run,
 // else one copy per row.
 #include <algorithm>
+#include <type_traits>
 
 #include "ca_common.cuh"
 #include "ca_paged.cuh"
@@ -66,27 +69,25 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
 }
 // Whole warp; gives up after two seconds (the barrier of copies that never land): records the timeout and
 // raises the group's flag, which ends the others' waits too.
-__device__ __noinline__ bool bar_wait_slow(uint32_t bar, uint32_t parity, volatile int* gave_up) {
-  unsigned long long t0, t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
-  bool ok = false;
-  while (!ok) {
-    ok = bar_try(bar, parity);
-    if (*gave_up) break;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    if (!ok && t - t0 > 2000000000ull) {
-      atomicCAS(&g_status, 0, 5);
-      *gave_up = 1;
-      break;
-    }
-  }
-  return ok;
-}
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
   bool ok = bar_try(bar, parity);
-  if (!ok) ok = bar_wait_slow(bar, parity, gave_up);
+  if (!ok) {
+    unsigned long long t0, t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+    while (!(ok = bar_try(bar, parity)) && !*gave_up) {
+      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+      if (t - t0 > 2000000000ull) {
+        atomicCAS(&g_status, 0, 5);
+        *gave_up = 1;
+      }
+    }
+  }
   return __all_sync(0xffffffffu, ok);
 }
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
                "l"(src), "r"(bytes), "r"(bar) : "memory");
@@ -96,11 +97,11 @@ __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 __device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
 }
 template <typename T>
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -108,13 +109,13 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
 template <>
 __device__ __forceinline__ void mma<__nv_bfloat16>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                    uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 template <>
 __device__ __forceinline__ void mma<__half>(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                             uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
@@ -230,21 +231,22 @@ __device__ __forceinline__ void add_caps(const float2 (&sv)[NJ], float m2, float
 
 // ------------------------------------------------------------------ the kernel
 
-// RPW rows per warp (8 or 16), RW warps that share a ring (1 or 4), GROUPS rings per block, NST stages of
-// TK keys of DP (padded) values, AHEAD of which are filled before they are needed; BPS blocks per SM
-template <int DP_, int TK_, int RPW_, int RW_, int GROUPS_, int NST_, int BPS_>
+// Tiles of TK keys of DP (padded) values; RPW rows per warp (8 or 16); RW consumer warps that share a
+// ring of NST stages (1 or 4); GROUPS rings per block.  One block per SM.  REGS_C and REGS_P: registers of a
+// consumer and a producer thread, 0 where the launch's even share suffices.
+template <int DP_, int TK_, int RPW_, int RW_, int GROUPS_, int NST_, int REGS_C_, int REGS_P_>
 struct Config {
-  static constexpr int DP = DP_, TK = TK_, RPW = RPW_, RW = RW_, GROUPS = GROUPS_, NST = NST_, BPS = BPS_;
-  // one warp refills the stage it has just left; several are given a tile's time to leave theirs
-  static constexpr int AHEAD = RW == 1 ? NST - 1 : NST - 2;
-  static constexpr int NT = RW * 32;                    // threads of a group
+  static constexpr int DP = DP_, TK = TK_, RPW = RPW_, RW = RW_, GROUPS = GROUPS_, NST = NST_;
+  static constexpr int REGS_C = REGS_C_, REGS_P = REGS_P_;
+  static constexpr int CONSUMERS = GROUPS * RW;                          // warps
+  static constexpr int THREADS = (CONSUMERS + (GROUPS + 3) / 4 * 4) * 32;   // producers in whole warpgroups
   static constexpr int BR = RPW * RW;                   // rows of a unit
   static constexpr int NJ = TK / 8;                     // score tiles of 8 keys; half a lane's run
   static constexpr int CH = DP / 8;                     // 16-byte chunks of a row
   static constexpr int ROWB = DP * 2;
   static constexpr int PITCH = NJ * ROWB + 16;          // of NJ rows
   static constexpr int KV_BYTES = 8 * PITCH;
-  static constexpr bool kStageQ = RW == 1 && RPW == 8 && DP == 64;   // as far as shared memory goes
+  static constexpr bool kStageQ = RW == 1;
   static constexpr int HALO = 2 * KV_BYTES;             // K row, then V row before the tile
   static constexpr int Q_AT = HALO + 2 * ROWB;
   static constexpr int STAGE = Q_AT + (kStageQ ? RPW * ROWB : 0);
@@ -257,6 +259,10 @@ struct Config {
   static constexpr int GROUP_STRIDE = (BAR_AT + 2 * NST * 8 + 16 + 127) / 128 * 128;
   static constexpr int SMEM = GROUPS * GROUP_STRIDE;    // and the prefix sums behind it
   static_assert(KV_BYTES % 128 == 0 && STAGE % 128 == 0 && DESC_AT % 16 == 0, "");
+  // setmaxnreg draws on what the block was launched with
+  static constexpr int REGS_LAUNCH = 65536 / THREADS / 8 * 8;
+  static_assert(REGS_C == 0 || (CONSUMERS % 4 == 0 && CONSUMERS * REGS_C + (THREADS / 32 - CONSUMERS) * REGS_P <=
+                                                          THREADS / 32 * REGS_LAUNCH), "");
 };
 
 struct Desc {   // one tile of the stream
@@ -270,7 +276,7 @@ struct Desc {   // one tile of the stream
 static_assert(sizeof(Desc) == 48, "");
 
 template <typename T, typename C>
-__global__ void __launch_bounds__(C::NT* C::GROUPS, C::BPS)
+__global__ void __launch_bounds__(C::THREADS, 1)
     mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Plan plan, float* __restrict__ part_o,
                float2* __restrict__ part_mz, Meta* __restrict__ meta) {
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -280,7 +286,9 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::BPS)
   constexpr int NKK = DP / 16;                 // k-steps of Q K^T
   constexpr int NN = DP / 8;                   // column tiles of the output
   const int lane = threadIdx.x & 31, c4 = lane & 3, r8 = lane >> 2;
-  const int group = threadIdx.x / C::NT, warp = (threadIdx.x % C::NT) >> 5;
+  const int wid = threadIdx.x >> 5;
+  const bool producer = wid >= C::CONSUMERS;
+  const int group = producer ? wid - C::CONSUMERS : wid / C::RW, warp = wid % C::RW;
   unsigned* prefix = reinterpret_cast<unsigned*>(smem + C::SMEM);
   uint8_t* gsm = smem + (size_t)group * C::GROUP_STRIDE;
   const uint32_t g0 = smem_addr(gsm);
@@ -288,36 +296,39 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::BPS)
   const uint32_t full = g0 + C::BAR_AT, empty = full + 8 * NST;
   volatile int* gave_up = reinterpret_cast<volatile int*>(gsm + C::BAR_AT + 16 * NST);
 
-  if (warp == 0 && lane == 0) {
-    for (int i = 0; i < NST; ++i) {
-      bar_init(full + 8 * i, 1);
-      bar_init(empty + 8 * i, C::RW);
+  if (producer && group < C::GROUPS) {
+    if (lane == 0) {
+      for (int i = 0; i < NST; ++i) {
+        bar_init(full + 8 * i, 1);
+        bar_init(empty + 8 * i, C::RW);
+      }
+      *gave_up = 0;
     }
-    *gave_up = 0;
+    // values behind D stay 0 (copies write D values a row)
+    if (a.D < DP) {
+      for (int x = lane; x < NST * C::STAGE / 16; x += 32)
+        *reinterpret_cast<uint4*>(gsm + 16 * x) = make_uint4(0u, 0u, 0u, 0u);
+    }
+    fence_async();
   }
-  // values behind D stay 0 (copies write D values a row)
-  if (a.D < DP) {
-    for (int x = (int)(threadIdx.x % C::NT); x < NST * C::STAGE / 16; x += C::NT)
-      *reinterpret_cast<uint4*>(gsm + 16 * x) = make_uint4(0u, 0u, 0u, 0u);
-  }
-  fence_async();
   Schedule<C::BR, TK> sched(a, plan, prefix);   // a barrier of the block among other things
   const unsigned total = sched.total;
   const int worker = blockIdx.x * C::GROUPS + group, workers = gridDim.x * C::GROUPS;
   const unsigned per = plan.tiles_per_worker(total, workers);
   const unsigned long long x0l = (unsigned long long)worker * per;
-  if (x0l >= total) {
-    if (warp == 0 && lane == 0) meta[worker].pieces = 0;
-    return;
-  }
-  const unsigned x0 = (unsigned)x0l, x1 = min(total, x0 + per);
+  const unsigned x0 = (unsigned)min(x0l, (unsigned long long)total), x1 = min(total, x0 + per);
 
-  // ---- the loader, the group's first warp: `cur` stands at tile xa, the next to be described, whose pages
-  // are fetched a tile before its copies are issued
-  typename Schedule<C::BR, TK>::Cursor cur;
-  unsigned xa = x0, xb = x0;      // next to be described; next to be copied
-  int slot_a = 0, slot_b = 0, stage_b = 0;
-  uint32_t empty_parity = 1;      // of the stages' previous use: the first one needs no wait
+  if (producer) {
+    if constexpr (C::REGS_C > 0) regs_down<C::REGS_P>();
+    if (group >= C::GROUPS || x0 >= x1) {
+      if (group < C::GROUPS && lane == 0) meta[worker].pieces = 0;
+      return;
+    }
+    // `cur` stands at tile xa, the next to be described; a tile's pages are fetched when it is described, one
+    // tile before its copies are issued
+  typename Schedule<C::BR, TK>::Cursor cur = sched.locate(x0);
+  unsigned xa = x0;
+  int slot_a = 0;
   constexpr int NP = TK / 32;
   int pg[NP];
 
@@ -359,8 +370,24 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::BPS)
            (size_t)(key - plan.page_of(key) * a.page_size) * a.slot_stride;
   };
 
-  auto issue = [&]() {
-    if (xb < x1) {
+  int slot_b = 0, stage_b = 0;
+  uint32_t empty_parity = 1;      // of the stage's previous use
+  describe();
+  for (unsigned xb = x0; xb < x1; ++xb) {
+    if (xb >= x0 + NST && !bar_wait(empty + 8 * stage_b, empty_parity, gave_up)) {
+      // copies may still be on their way: leave no sooner than they land, or another limit runs out
+      *gave_up = 0;
+      __syncwarp();
+      for (int i = 0; i < NST; ++i) {
+        bar_wait(full + 8 * stage_b, empty_parity, gave_up);
+        if (++stage_b == NST) {
+          stage_b = 0;
+          empty_parity ^= 1;
+        }
+      }
+      return;
+    }
+    {
       Desc& d = descs[slot_b];
       const uint32_t st = g0 + stage_b * C::STAGE, bar = full + 8 * stage_b;
       const int base = d.kt * TK, len = d.len, h = d.h, first = d.first;
@@ -419,23 +446,17 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::BPS)
                   row_bytes, bar);
       }
     }
-    ++xb;
     if (++slot_b == C::RING) slot_b = 0;
     if (++stage_b == NST) {
       stage_b = 0;
       empty_parity ^= 1;
     }
-  };
-
-  if (warp == 0) {
-    cur = sched.locate(x0);
     describe();
-    for (int i = 0; i < C::AHEAD; ++i) {
-      issue();
-      describe();
-    }
+  }
+  return;
   }
 
+  if constexpr (C::REGS_C > 0) regs_up<C::REGS_C>();
   // ---- the consumers' state
   constexpr int RS = C::RPW == 8 ? 1 : 2;      // row sets per lane: rows r8 (and r8 + 8)
   uint32_t qf[NKK][4];
@@ -456,25 +477,11 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::BPS)
 
   int slot = 0, stage = 0;
   uint32_t parity = 0;
-  bool alive = true;
-  unsigned x = x0;
-  for (; x < x1; ++x) {
-    if constexpr (C::RW > 1) {
-      if (warp == 0) {
-        // tile x + AHEAD goes where tile x - 2 was; every warp has to have left it
-        if (xb < x1 && xb >= x0 + NST) alive = bar_wait(empty + 8 * stage_b, empty_parity, gave_up);
-        if (!alive) break;
-        issue();
-        describe();
-      }
+  for (unsigned x = x0; x < x1; ++x) {
+    if (!bar_wait(full + 8 * stage, parity, gave_up)) {
+      if (warp == 0 && lane == 0) meta[worker].pieces = 0;
+      return;
     }
-    alive = bar_wait(full + 8 * stage, parity, gave_up);
-    if (!alive) break;
-    if constexpr (C::RW == 1) {
-      issue();             // into the stage that this warp has just left
-      describe();
-    }
-
     const Desc& d = descs[slot];
     uint8_t* sm = gsm + stage * C::STAGE;
     const uint32_t st = g0 + stage * C::STAGE;
@@ -513,7 +520,8 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::BPS)
           const uint8_t* qs = sm + C::Q_AT + r8 * ROWB + (16 * k + 2 * c4) * 2;
           qf[k][0] = *reinterpret_cast<const uint32_t*>(qs);
           qf[k][2] = *reinterpret_cast<const uint32_t*>(qs + 16);
-          qf[k][1] = qf[k][3] = 0u;
+          qf[k][1] = RS == 2 ? *reinterpret_cast<const uint32_t*>(qs + 8 * ROWB) : 0u;
+          qf[k][3] = RS == 2 ? *reinterpret_cast<const uint32_t*>(qs + 8 * ROWB + 16) : 0u;
         } else {
 #pragma unroll
           for (int u = 0; u < RS; ++u) {
@@ -562,19 +570,30 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::BPS)
     if (base - 1 <= i_max && i_max >= 0) {
       float2 s[RS][NJ];
       const uint32_t ka = st + k_lane;
+      // score tiles side by side, so that no product waits for the one before it
+      float acc[NJ][4];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < NJ; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
 #pragma unroll
-        for (int kp = 0; kp < NKK / 2; ++kp) {
-          uint32_t b[4];
-          ldsm4(b, ka + j * ROWB + kp * 64);
-          mma<T>(acc, qf[2 * kp][0], qf[2 * kp][1], qf[2 * kp][2], qf[2 * kp][3], b[0], b[1]);
-          mma<T>(acc, qf[2 * kp + 1][0], qf[2 * kp + 1][1], qf[2 * kp + 1][2], qf[2 * kp + 1][3], b[2], b[3]);
+      for (int kp = 0; kp < NKK / 2; ++kp) {
+#pragma unroll
+        for (int j = 0; j < NJ; j += 2) {
+          uint32_t b[2][4];
+          ldsm4(b[0], ka + j * ROWB + kp * 64);
+          ldsm4(b[1], ka + (j + 1) * ROWB + kp * 64);
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            mma<T>(acc[j], qf[2 * kp + e][0], qf[2 * kp + e][1], qf[2 * kp + e][2], qf[2 * kp + e][3], b[0][2 * e],
+                   b[0][2 * e + 1]);
+            mma<T>(acc[j + 1], qf[2 * kp + e][0], qf[2 * kp + e][1], qf[2 * kp + e][2], qf[2 * kp + e][3], b[1][2 * e],
+                   b[1][2 * e + 1]);
+          }
         }
-#pragma unroll
-        for (int u = 0; u < RS; ++u) s[u][j] = mul2(make_float2(acc[2 * u], acc[2 * u + 1]), splat2(scale[u]));
       }
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+#pragma unroll
+        for (int u = 0; u < RS; ++u) s[u][j] = mul2(make_float2(acc[j][2 * u], acc[j][2 * u + 1]), splat2(scale[u]));
       // keys beyond a row's own, or caps among the weights
       const bool edge = base == 0 || base + TK - 1 > i_min;
       const int kc = base + 2 * NJ * c4;        // first key of the lane's run
@@ -635,19 +654,23 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::BPS)
 #pragma unroll
       for (int kk = 0; kk < TK / 16; ++kk) {
 #pragma unroll
-        for (int np = 0; np < NN / 2; ++np) {
-          uint32_t b[4];
-          ldsm4_t(b, (kk == 0 ? va0 : va + 2 * kk * ROWB) + np * 32);
-          if constexpr (RS == 1) {
-            mma<T>(o[2 * np], hi[0][2 * kk], lo[0][2 * kk], hi[0][2 * kk + 1], lo[0][2 * kk + 1], b[0], b[1]);
-            mma<T>(o[2 * np + 1], hi[0][2 * kk], lo[0][2 * kk], hi[0][2 * kk + 1], lo[0][2 * kk + 1], b[2], b[3]);
-          } else {
-            mma<T>(o[2 * np], hi[0][2 * kk], hi[RS - 1][2 * kk], hi[0][2 * kk + 1], hi[RS - 1][2 * kk + 1], b[0], b[1]);
-            mma<T>(o[2 * np + 1], hi[0][2 * kk], hi[RS - 1][2 * kk], hi[0][2 * kk + 1], hi[RS - 1][2 * kk + 1], b[2],
-                   b[3]);
-            mma<T>(o[2 * np], lo[0][2 * kk], lo[RS - 1][2 * kk], lo[0][2 * kk + 1], lo[RS - 1][2 * kk + 1], b[0], b[1]);
-            mma<T>(o[2 * np + 1], lo[0][2 * kk], lo[RS - 1][2 * kk], lo[0][2 * kk + 1], lo[RS - 1][2 * kk + 1], b[2],
-                   b[3]);
+        for (int np = 0; np < NN / 2; np += 2) {
+          uint32_t b[2][4];
+          ldsm4_t(b[0], (kk == 0 ? va0 : va + 2 * kk * ROWB) + np * 32);
+          ldsm4_t(b[1], (kk == 0 ? va0 : va + 2 * kk * ROWB) + np * 32 + 32);
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            const uint32_t b0 = b[t >> 1][2 * (t & 1)], b1 = b[t >> 1][2 * (t & 1) + 1];
+            if constexpr (RS == 1)
+              mma<T>(o[2 * np + t], hi[0][2 * kk], lo[0][2 * kk], hi[0][2 * kk + 1], lo[0][2 * kk + 1], b0, b1);
+            else
+              mma<T>(o[2 * np + t], hi[0][2 * kk], hi[RS - 1][2 * kk], hi[0][2 * kk + 1], hi[RS - 1][2 * kk + 1], b0, b1);
+          }
+          if constexpr (RS == 2) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+              mma<T>(o[2 * np + t], lo[0][2 * kk], lo[RS - 1][2 * kk], lo[0][2 * kk + 1], lo[RS - 1][2 * kk + 1],
+                     b[t >> 1][2 * (t & 1)], b[t >> 1][2 * (t & 1) + 1]);
           }
         }
       }
@@ -715,73 +738,82 @@ __global__ void __launch_bounds__(C::NT* C::GROUPS, C::BPS)
       meta[worker] = mt;
     }
     __syncwarp();
-    if constexpr (C::RW > 1) {
-      if (lane == 0) bar_arrive(empty + 8 * stage);
-    }
+    if (lane == 0) bar_arrive(empty + 8 * stage);
     if (++slot == C::RING) slot = 0;
     if (++stage == NST) {
       stage = 0;
       parity ^= 1;
     }
   }
-  if (!alive) {
-    // copies of tiles x .. xb - 1 may still be on their way: leave no sooner than they land, or a second
-    // limit runs out
-    if (warp == 0) {
-      if (lane == 0) {
-        meta[worker].pieces = 0;
-        *gave_up = 0;
-      }
-      __syncwarp();
-      for (; x < x1 && x < xb; ++x) {
-        bar_wait(full + 8 * stage, parity, gave_up);
-        if (++stage == NST) {
-          stage = 0;
-          parity ^= 1;
-        }
-      }
-    }
-  }
 }
 
-// Joins the pieces of a cut unit in the order of their keys: piece 0 is in this worker's slot, the others
-// are the first pieces of the workers that follow.
+// Joins the pieces of a cut unit: piece 0 is in this worker's slot, the others are the first pieces of the
+// workers that follow.  A row's pieces are dealt to up to SLICES teams of DP/4 lanes (as many rows at once
+// as that leaves), each sums its own in order and then the teams' sums are added in order.  One thread per
+// output summing all pieces took 38 us for the 32 pieces of a 2048-key row.
+constexpr int kMergeThreads = 256;
+
 template <typename T, int DP, int BR>
-__global__ void __launch_bounds__(128) merge_kernel(Args a, int group, const float* __restrict__ part_o,
-                                                    const float2* __restrict__ part_mz,
-                                                    const Meta* __restrict__ meta) {
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(Args a, int group, const float* __restrict__ part_o,
+                                                              const float2* __restrict__ part_mz,
+                                                              const Meta* __restrict__ meta) {
   pdl_wait();
   pdl_launch_dependents();
+  constexpr int V = DP / 4, SLICES = kMergeThreads / V;
+  __shared__ float4 sum_y[kMergeThreads];
+  __shared__ float2 sum_mz[SLICES];
   const int w = blockIdx.x;
   const Meta mt = meta[w];
   if (mt.pieces == 0) return;
   const int nrows = min(BR, mt.rows - mt.rt * BR);
-  constexpr int V = DP / 4;
-  for (int x = threadIdx.x; x < nrows * V; x += blockDim.x) {
-    const int r = x / V, d0 = (x - r * V) * 4;
+  int per_row = 2;                                   // teams per row
+  while (per_row < SLICES && per_row < mt.pieces) per_row *= 2;
+  const int team = threadIdx.x / V, v = threadIdx.x % V, d0 = 4 * v;
+  const int share = team % per_row;
+  for (int r0 = 0; r0 < nrows; r0 += SLICES / per_row) {
+    const int r = r0 + team / per_row;
     float m = -INFINITY, z = 0.f;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (r < nrows) {
 #pragma unroll 4
-    for (int p = 0; p < mt.pieces; ++p) {
-      const long long row = ((long long)(w + p) * 2 + (p == 0 ? mt.slot : 0)) * BR + r;
-      const float2 mz = part_mz[row];
-      const float4 v = *reinterpret_cast<const float4*>(part_o + row * DP + d0);
-      if (mz.x == -INFINITY) {   // no key seen: no mass, or the NaN of a bad page or length
-        z += mz.y;
-        continue;
+      for (int p = share; p < mt.pieces; p += per_row) {
+        const long long row = ((long long)(w + p) * 2 + (p == 0 ? mt.slot : 0)) * BR + r;
+        const float2 mz = part_mz[row];
+        const float4 x = *reinterpret_cast<const float4*>(part_o + row * DP + d0);
+        // a piece without a key the row sees has m = -inf and no mass, or the NaN of a bad page or length
+        const bool none = mz.x == -INFINITY;
+        const float top = fmaxf(m, mz.x);
+        const float fa = none ? 1.f : exp_rel(m - top), fb = none ? 0.f : exp_rel(mz.x - top);
+        z = none ? z + mz.y : fmaf(z, fa, mz.y * fb);
+        y.x = fmaf(y.x, fa, none ? 0.f : x.x * fb);
+        y.y = fmaf(y.y, fa, none ? 0.f : x.y * fb);
+        y.z = fmaf(y.z, fa, none ? 0.f : x.z * fb);
+        y.w = fmaf(y.w, fa, none ? 0.f : x.w * fb);
+        m = top;
       }
-      const float top = fmaxf(m, mz.x);
-      const float fa = exp_rel(m - top), fb = exp_rel(mz.x - top);
-      z = fmaf(z, fa, mz.y * fb);
-      y = make_float4(fmaf(y.x, fa, v.x * fb), fmaf(y.y, fa, v.y * fb), fmaf(y.z, fa, v.z * fb), fmaf(y.w, fa, v.w * fb));
-      m = top;
     }
-    const float inv = z == 0.f ? 0.f : 1.f / z;   // y is 0 then
-    const int row = mt.rt * BR + r, t = row / group;
-    T* dst = (T*)a.o + ((size_t)(mt.start + t) * a.H + (size_t)mt.h * group + (row - t * group)) * a.D + d0;
-    if (d0 < a.D) {
-      *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(y.x * inv, y.y * inv), pack2<T>(y.z * inv, y.w * inv));
+    sum_y[threadIdx.x] = y;
+    if (v == 0) sum_mz[team] = make_float2(m, z);
+    __syncthreads();
+    if (share == 0 && r < nrows) {
+      for (int q = 1; q < per_row; ++q) {
+        const float2 mz = sum_mz[team + q];
+        const float4 x = sum_y[threadIdx.x + q * V];
+        const bool none = mz.x == -INFINITY;
+        const float top = fmaxf(m, mz.x);
+        const float fa = none ? 1.f : exp_rel(m - top), fb = none ? 0.f : exp_rel(mz.x - top);
+        z = none ? z + mz.y : fmaf(z, fa, mz.y * fb);
+        y = make_float4(fmaf(y.x, fa, x.x * fb), fmaf(y.y, fa, x.y * fb), fmaf(y.z, fa, x.z * fb),
+                        fmaf(y.w, fa, x.w * fb));
+        m = top;
+      }
+      const float inv = z == 0.f ? 0.f : 1.f / z;   // y is 0 then
+      const int row = mt.rt * BR + r, t = row / group;
+      T* dst = (T*)a.o + ((size_t)(mt.start + t) * a.H + (size_t)mt.h * group + (row - t * group)) * a.D + d0;
+      if (d0 < a.D)
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(y.x * inv, y.y * inv), pack2<T>(y.z * inv, y.w * inv));
     }
+    __syncthreads();
   }
 }
 
@@ -792,9 +824,9 @@ __global__ void __launch_bounds__(128) merge_kernel(Args a, int group, const flo
 namespace {
 
 // The forms: decoding with 8 or 16 rows a warp, and chunks
-template <int DP> using Decode8 = Config<DP, DP == 64 ? 64 : 32, 8, 1, 4, 3, 1>;
-template <int DP> using Decode16 = Config<DP, DP == 64 ? 64 : 32, 16, 1, 4, 3, 1>;
-template <int DP> using Chunk = Config<DP, DP == 64 ? 64 : 32, 16, 4, 1, 4, 3>;
+template <int DP> using Decode8 = std::conditional_t<DP == 64, Config<64, 32, 8, 1, 8, 2, 200, 56>, Config<128, 32, 8, 1, 4, 2, 0, 0>>;
+template <int DP> using Decode16 = std::conditional_t<DP == 64, Config<64, 32, 16, 1, 8, 2, 200, 56>, Config<128, 32, 16, 1, 4, 2, 0, 0>>;
+template <int DP> using Chunk = Config<DP, DP == 64 ? 64 : 32, 16, 4, 3, 4, 152, 56>;
 
 size_t part_bytes(long long workers, int br, int dp) {
   return (size_t)workers * 2 * br * (dp * sizeof(float) + sizeof(float2)) + (size_t)workers * sizeof(Meta) + 768;
@@ -814,7 +846,7 @@ cudaError_t launch(const Args& a, Plan plan, void* workspace) {
     if (e != cudaSuccess) return e;
     set_dev = dev;
   }
-  const int blocks = num_sms_cached() * C::BPS;
+  const int blocks = num_sms_cached();
   plan.unit_rows = a.D == C::DP && a.slot_stride == C::DP && a.page_size % C::NJ == 0 ? C::NJ : 1;
   const long long workers = (long long)blocks * C::GROUPS;
   char* ws = (char*)workspace;
@@ -822,9 +854,9 @@ cudaError_t launch(const Args& a, Plan plan, void* workspace) {
   float* po = (float*)ws;
   float2* mz = (float2*)(ws + up((size_t)workers * 2 * C::BR * C::DP * sizeof(float)));
   Meta* meta = (Meta*)((char*)mz + up((size_t)workers * 2 * C::BR * sizeof(float2)));
-  e = launch_pdl(mma_kernel<T, C>, dim3(blocks), dim3(C::NT * C::GROUPS), smem, a.stream, a, plan, po, mz, meta);
+  e = launch_pdl(mma_kernel<T, C>, dim3(blocks), dim3(C::THREADS), smem, a.stream, a, plan, po, mz, meta);
   if (e != cudaSuccess) return e;
-  return launch_pdl(merge_kernel<T, C::DP, C::BR>, dim3((unsigned)workers), dim3(128), 0, a.stream, a, plan.group,
+  return launch_pdl(merge_kernel<T, C::DP, C::BR>, dim3((unsigned)workers), dim3(kMergeThreads), 0, a.stream, a, plan.group,
                     (const float*)po, (const float2*)mz, (const Meta*)meta);
 }
 
@@ -855,7 +887,7 @@ size_t mma_workspace_bytes(long long max_q_len, long long H, long long G, long l
   auto bytes = [&](auto d8, auto d16, auto chunk) {
     auto part = [](auto c) {
       using C = decltype(c);
-      return part_bytes((long long)num_sms_cached() * C::BPS * C::GROUPS, C::BR, C::DP);
+      return part_bytes((long long)num_sms_cached() * C::GROUPS, C::BR, C::DP);
     };
     const size_t decode = std::max(part(d8), part(d16));
     return rows <= 16 ? decode : std::max(decode, part(chunk));
