@@ -132,10 +132,14 @@ __device__ __forceinline__ void split2<__nv_bfloat16>(float2 w, uint32_t& hi, ui
 }
 template <>
 __device__ __forceinline__ void split2<__half>(float2 w, uint32_t& hi, uint32_t& lo) {
-  const __half2 h = __floats2half2_rn(w.x, w.y);
+  // 10 bits of mantissa by truncation, exact in f16 above its subnormals (2^-14 of the largest weight, where
+  // hi rounds by 2^-25 at most); the remainder is exact
+  const float2 t = make_float2(__uint_as_float(__float_as_uint(w.x) & 0xffffe000u),
+                               __uint_as_float(__float_as_uint(w.y) & 0xffffe000u));
+  const __half2 h = __floats2half2_rn(t.x, t.y);
   hi = *reinterpret_cast<const uint32_t*>(&h);
-  const float2 f = __half22float2(h);
-  const __half2 l = __floats2half2_rn(w.x - f.x, w.y - f.y);
+  const float2 r = sub2(w, t);
+  const __half2 l = __floats2half2_rn(r.x, r.y);
   lo = *reinterpret_cast<const uint32_t*>(&l);
 }
 template <typename T>
@@ -164,69 +168,81 @@ __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
 // exponentials are 0.  (Finite, since infinities would meet as NaN.)
 constexpr float kMasked = -1e30f;
 
-// Weights of one lane's run of one row.  sv[j] = scaled scores of keys (kc + j, kc + NJ + j), sL that of key
-// kc - 1, m2 the reference maximum in log2 units.  On return W[j] weighs keys (kc - 1 + j, kc + NJ - 1 + j),
-// but for the mass that ends at key kc - 1, which the lane to the left adds to W[0].x; last is the mass
-// that ends at the run's last key.
-template <int NJ>
-__device__ __forceinline__ void weigh(const float2 (&sv)[NJ], float m2, float sL, float2 (&W)[NJ], float& last,
-                                      float2& z2) {
+// Weights of one lane's run of one row, as two 16-bit parts.  sv[j] = scaled scores of keys (kc + j, kc + NJ + j),
+// sL that of key kc - 1, m2 the reference maximum in log2 units.  Parts j weigh keys (kc - 1 + j, kc + NJ - 1 + j);
+// first is the pair of place 0, unsplit, but for the mass that ends at key kc - 1, which is the lane's to
+// the left; last is the mass that ends at the run's last key.  Pair by pair, each needing the one before:
+// a score's registers take its weight's parts.
+// kEdge adds the half caps of keys 0 and i where this run weighs them.  Key i's belongs to this piece when
+// i >= lowest: the piece before it has weighed its own last key to the end.
+template <typename T, bool kEdge, int NJ>
+__device__ __forceinline__ void weigh(const float2 (&sv)[NJ], float m2, float sL, int kc, int i, int lowest,
+                                      uint32_t (&hi)[NJ], uint32_t (&lo)[NJ], float2& first, float& last, float2& z2) {
   const float2 l2e = splat2(kLog2e), nm2 = splat2(-m2);
-  float2 ev[NJ], M1[NJ];
+  auto exps = [&](float2 v) {
+    const float2 arg = fma2(v, l2e, nm2);
+    return make_float2(ex2_approx(arg.x), ex2_approx(arg.y));
+  };
+  const float2 e_end = exps(sv[NJ - 1]);
+  float2 sl0 = make_float2(sL, sv[NJ - 1].x);
+  float2 el0 = make_float2(ex2_approx(fmaf(sL, kLog2e, -m2)), e_end.x);
+  float2 m1_before = splat2(0.f);
+  // four pairs side by side, step by step: their chains hide each other's latencies
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    const float2 arg = fma2(sv[j], l2e, nm2);
-    ev[j] = make_float2(ex2_approx(arg.x), ex2_approx(arg.y));
-  }
-  const float eL0 = ex2_approx(fmaf(sL, kLog2e, -m2));
+  for (int j0 = 0; j0 < NJ; j0 += 4) {
+    float2 e[4], nd[4], rn[4], ps[4], m1[4], w[4];
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    const float2 sl = j ? sv[j - 1] : make_float2(sL, sv[NJ - 1].x);
-    const float2 eL = j ? ev[j - 1] : make_float2(eL0, ev[NJ - 1].x);
-    const float2 nd = sub2(sl, sv[j]);                                          // -d
-    const float2 rn = make_float2(rcp_approx(nd.x), rcp_approx(nd.y));         // -1/d
-    float2 ps = fma2(splat2(-1.f / 30.f), nd, splat2(1.f / 8.f));              // J1's series in -nd
-    ps = fma2(ps, nd, splat2(-1.f / 3.f));
-    ps = fma2(ps, nd, splat2(1.f / 2.f));
-    const float2 m0c = mul2(sub2(eL, ev[j]), rn);
-    const float2 m1c = mul2(sub2(m0c, ev[j]), rn);
-    M1[j] = make_float2(sel_series(m1c.x, nd.x, eL.x, ps.x, kSeriesMaxFwd),
-                        sel_series(m1c.y, nd.y, eL.y, ps.y, kSeriesMaxFwd));
-    const float2 m0 = fma2(nd, M1[j], ev[j]);
-    W[j] = sub2(m0, M1[j]);
-    z2 = add2(z2, m0);
-  }
+    for (int t = 0; t < 4; ++t) e[t] = j0 + t == NJ - 1 ? e_end : exps(sv[j0 + t]);
 #pragma unroll
-  for (int j = NJ - 1; j >= 1; --j) W[j] = add2(W[j], M1[j - 1]);
-  W[0].y += M1[NJ - 1].x;
-  last = M1[NJ - 1].y;
-}
-
-// The half caps of keys 0 and i, where this run weighs them (keys kc - 1 .. kc + 2 NJ - 2).  Key i's belongs
-// to this piece when i >= lowest: the piece before it has weighed its own last key to the end.
-template <int NJ>
-__device__ __forceinline__ void add_caps(const float2 (&sv)[NJ], float m2, float sL, int kc, int i, int lowest,
-                                         float2 (&W)[NJ], float2& z2) {
-  if (kc == 0 && i >= 0) {
-    const float cap = 0.5f * ex2_approx(fmaf(sv[0].x, kLog2e, -m2));
-    W[1].x += cap;
-    z2.x += cap;
-  }
-  const int t = i - kc + 1;     // key i's place
-  if (t < 0 || t >= 2 * NJ || i < lowest) return;
-  float si = sL;
+    for (int t = 0; t < 4; ++t) nd[t] = sub2(t ? sv[j0 + t - 1] : sl0, sv[j0 + t]);                  // -d
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    if (t == j + 1) si = sv[j].x;
-    if (t == j + NJ + 1) si = sv[j].y;
-  }
-  const float cap = 0.5f * ex2_approx(fmaf(si, kLog2e, -m2));
+    for (int t = 0; t < 4; ++t) rn[t] = make_float2(rcp_approx(nd[t].x), rcp_approx(nd[t].y));     // -1/d
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    W[j].x += t == j ? cap : 0.f;
-    W[j].y += t == j + NJ ? cap : 0.f;
+    for (int t = 0; t < 4; ++t) ps[t] = fma2(splat2(-1.f / 30.f), nd[t], splat2(1.f / 8.f));      // J1's series in -nd
+#pragma unroll
+    for (int t = 0; t < 4; ++t) ps[t] = fma2(ps[t], nd[t], splat2(-1.f / 3.f));
+#pragma unroll
+    for (int t = 0; t < 4; ++t) ps[t] = fma2(ps[t], nd[t], splat2(1.f / 2.f));
+#pragma unroll
+    for (int t = 0; t < 4; ++t) w[t] = mul2(sub2(t ? e[t - 1] : el0, e[t]), rn[t]);                 // M0
+#pragma unroll
+    for (int t = 0; t < 4; ++t) w[t] = mul2(sub2(w[t], e[t]), rn[t]);                               // M1, closed
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const float2 el = t ? e[t - 1] : el0;
+      m1[t] = make_float2(sel_series(w[t].x, nd[t].x, el.x, ps[t].x, kSeriesMaxFwd),
+                          sel_series(w[t].y, nd[t].y, el.y, ps[t].y, kSeriesMaxFwd));
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) w[t] = fma2(nd[t], m1[t], e[t]);                                   // M0
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      z2 = add2(z2, w[t]);
+      w[t] = sub2(w[t], m1[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if (j0 + t > 0) w[t] = add2(w[t], t ? m1[t - 1] : m1_before);
+      if (kEdge) {
+        const float2 el = t ? e[t - 1] : el0;
+        const int kx = kc + j0 + t - 1, ky = kx + NJ;      // the keys these weights belong to
+        const float nx = (kx == 0 && i >= 0 ? 0.5f : 0.f) + (kx == i && i >= lowest ? 0.5f : 0.f);
+        const float2 cap = make_float2(nx > 0.f ? nx * el.x : 0.f, ky == i ? 0.5f * el.y : 0.f);
+        w[t] = add2(w[t], cap);
+        z2 = add2(z2, cap);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if (j0 + t > 0) split2<T>(w[t], hi[j0 + t], lo[j0 + t]);
+      else first = w[t];
+    }
+    m1_before = m1[3];
+    sl0 = sv[j0 + 3];
+    el0 = e[3];
   }
-  z2.x += cap;
+  first.y += m1_before.x;
+  last = m1_before.y;
 }
 
 // ------------------------------------------------------------------ the kernel
@@ -638,15 +654,17 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         float got = __shfl_sync(0xffffffffu, s[u][NJ - 1].y, left);
         const float sL = c4 == 0 ? carry_s[u] : got;
         carry_s[u] = got;                       // of use to the quad's first lane only
-        float2 W[NJ];
+        float2 first;
         float last;
-        weigh<NJ>(s[u], m2, sL, W, last, z2[u]);
-        if (edge) add_caps<NJ>(s[u], m2, sL, kc, pos[u], d.first ? base : base - 1, W, z2[u]);
+        if (edge) {
+          weigh<T, true, NJ>(s[u], m2, sL, kc, pos[u], d.first ? base : base - 1, hi[u], lo[u], first, last, z2[u]);
+        } else {
+          weigh<T, false, NJ>(s[u], m2, sL, kc, pos[u], base, hi[u], lo[u], first, last, z2[u]);
+        }
         got = __shfl_sync(0xffffffffu, last, left);
-        W[0].x += c4 == 0 ? carry_b[u] : got;
+        first.x += c4 == 0 ? carry_b[u] : got;
         carry_b[u] = got;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) split2<T>(W[j], hi[u][j], lo[u][j]);
+        split2<T>(first, hi[u][0], lo[u][0]);
       }
       const uint32_t va = st + v_lane;
       const uint32_t va0 = lane == 0 || lane == 16 ? my_halo + (mi >> 1) * 16
@@ -748,72 +766,74 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 }
 
 // Joins the pieces of a cut unit: piece 0 is in this worker's slot, the others are the first pieces of the
-// workers that follow.  A row's pieces are dealt to up to SLICES teams of DP/4 lanes (as many rows at once
-// as that leaves), each sums its own in order and then the teams' sums are added in order.  One thread per
-// output summing all pieces took 38 us for the 32 pieces of a 2048-key row.
-constexpr int kMergeThreads = 256;
+// workers that follow.  A warp takes a row; where rows are fewer than warps, several warps share a row's
+// pieces, each sums its own in order, and then the warps' sums are added in order.
+constexpr int kMergeWarps = 16;
+
+struct Sum {
+  float m = -INFINITY, z = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+  // adds a piece with maximum m2, mass z2 and row y2.  A piece without a key that the row sees has m = -inf
+  // and no mass, or the NaN of a bad page or length.
+  __device__ __forceinline__ void add(float m2, float z2, float4 y2) {
+    const bool none = m2 == -INFINITY;
+    const float top = fmaxf(m, m2);
+    const float fa = none ? 1.f : exp_rel(m - top), fb = none ? 0.f : exp_rel(m2 - top);
+    z = none ? z + z2 : fmaf(z, fa, z2 * fb);
+    y[0] = fmaf(y[0], fa, none ? 0.f : y2.x * fb);
+    y[1] = fmaf(y[1], fa, none ? 0.f : y2.y * fb);
+    y[2] = fmaf(y[2], fa, none ? 0.f : y2.z * fb);
+    y[3] = fmaf(y[3], fa, none ? 0.f : y2.w * fb);
+    m = top;
+  }
+};
 
 template <typename T, int DP, int BR>
-__global__ void __launch_bounds__(kMergeThreads) merge_kernel(Args a, int group, const float* __restrict__ part_o,
-                                                              const float2* __restrict__ part_mz,
-                                                              const Meta* __restrict__ meta) {
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(Args a, int group, const float* __restrict__ part_o,
+                                                                 const float2* __restrict__ part_mz,
+                                                                 const Meta* __restrict__ meta) {
   pdl_wait();
   pdl_launch_dependents();
-  constexpr int V = DP / 4, SLICES = kMergeThreads / V;
-  __shared__ float4 sum_y[kMergeThreads];
-  __shared__ float2 sum_mz[SLICES];
+  constexpr int VL = DP / 32;                        // values per lane: 2 or 4
+  __shared__ float4 sum_y[kMergeWarps][32];
+  __shared__ float2 sum_mz[kMergeWarps];
   const int w = blockIdx.x;
   const Meta mt = meta[w];
   if (mt.pieces == 0) return;
   const int nrows = min(BR, mt.rows - mt.rt * BR);
-  int per_row = 2;                                   // teams per row
-  while (per_row < SLICES && per_row < mt.pieces) per_row *= 2;
-  const int team = threadIdx.x / V, v = threadIdx.x % V, d0 = 4 * v;
-  const int share = team % per_row;
-  for (int r0 = 0; r0 < nrows; r0 += SLICES / per_row) {
-    const int r = r0 + team / per_row;
-    float m = -INFINITY, z = 0.f;
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r < nrows) {
+  int share = 1;                                     // warps per row
+  while (share * 2 * nrows <= kMergeWarps && share * 4 <= mt.pieces) share *= 2;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % share;
+  for (int r = warp / share; r < nrows; r += kMergeWarps / share) {
+    Sum acc;
 #pragma unroll 4
-      for (int p = share; p < mt.pieces; p += per_row) {
-        const long long row = ((long long)(w + p) * 2 + (p == 0 ? mt.slot : 0)) * BR + r;
-        const float2 mz = part_mz[row];
-        const float4 x = *reinterpret_cast<const float4*>(part_o + row * DP + d0);
-        // a piece without a key the row sees has m = -inf and no mass, or the NaN of a bad page or length
-        const bool none = mz.x == -INFINITY;
-        const float top = fmaxf(m, mz.x);
-        const float fa = none ? 1.f : exp_rel(m - top), fb = none ? 0.f : exp_rel(mz.x - top);
-        z = none ? z + mz.y : fmaf(z, fa, mz.y * fb);
-        y.x = fmaf(y.x, fa, none ? 0.f : x.x * fb);
-        y.y = fmaf(y.y, fa, none ? 0.f : x.y * fb);
-        y.z = fmaf(y.z, fa, none ? 0.f : x.z * fb);
-        y.w = fmaf(y.w, fa, none ? 0.f : x.w * fb);
-        m = top;
+    for (int p = part; p < mt.pieces; p += share) {
+      const long long row = ((long long)(w + p) * 2 + (p == 0 ? mt.slot : 0)) * BR + r;
+      const float2 mz = part_mz[row];
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+      if constexpr (VL == 4) {
+        y = *reinterpret_cast<const float4*>(part_o + row * DP + 4 * lane);
+      } else {
+        const float2 t = *reinterpret_cast<const float2*>(part_o + row * DP + 2 * lane);
+        y.x = t.x;
+        y.y = t.y;
       }
+      acc.add(mz.x, mz.y, y);
     }
-    sum_y[threadIdx.x] = y;
-    if (v == 0) sum_mz[team] = make_float2(m, z);
-    __syncthreads();
-    if (share == 0 && r < nrows) {
-      for (int q = 1; q < per_row; ++q) {
-        const float2 mz = sum_mz[team + q];
-        const float4 x = sum_y[threadIdx.x + q * V];
-        const bool none = mz.x == -INFINITY;
-        const float top = fmaxf(m, mz.x);
-        const float fa = none ? 1.f : exp_rel(m - top), fb = none ? 0.f : exp_rel(mz.x - top);
-        z = none ? z + mz.y : fmaf(z, fa, mz.y * fb);
-        y = make_float4(fmaf(y.x, fa, x.x * fb), fmaf(y.y, fa, x.y * fb), fmaf(y.z, fa, x.z * fb),
-                        fmaf(y.w, fa, x.w * fb));
-        m = top;
-      }
-      const float inv = z == 0.f ? 0.f : 1.f / z;   // y is 0 then
-      const int row = mt.rt * BR + r, t = row / group;
-      T* dst = (T*)a.o + ((size_t)(mt.start + t) * a.H + (size_t)mt.h * group + (row - t * group)) * a.D + d0;
-      if (d0 < a.D)
-        *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(y.x * inv, y.y * inv), pack2<T>(y.z * inv, y.w * inv));
+    if (share > 1) {                                 // then every warp takes this loop once, or not at all
+      sum_y[warp][lane] = make_float4(acc.y[0], acc.y[1], acc.y[2], acc.y[3]);
+      if (lane == 0) sum_mz[warp] = make_float2(acc.m, acc.z);
+      asm volatile("bar.sync 1, %0;" ::"r"(nrows * share * 32) : "memory");
+      if (part > 0) return;
+      for (int q = 1; q < share; ++q) acc.add(sum_mz[warp + q].x, sum_mz[warp + q].y, sum_y[warp + q][lane]);
     }
-    __syncthreads();
+    const float inv = acc.z == 0.f ? 0.f : 1.f / acc.z;   // y is 0 then
+    const int row = mt.rt * BR + r, t = row / group;
+    T* dst = (T*)a.o + ((size_t)(mt.start + t) * a.H + (size_t)mt.h * group + (row - t * group)) * a.D + VL * lane;
+    if (VL * lane < a.D) {
+      const uint32_t u = pack2<T>(acc.y[0] * inv, acc.y[1] * inv);
+      if constexpr (VL == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(u, pack2<T>(acc.y[2] * inv, acc.y[3] * inv));
+      else *reinterpret_cast<uint32_t*>(dst) = u;
+    }
   }
 }
 
@@ -856,7 +876,7 @@ cudaError_t launch(const Args& a, Plan plan, void* workspace) {
   Meta* meta = (Meta*)((char*)mz + up((size_t)workers * 2 * C::BR * sizeof(float2)));
   e = launch_pdl(mma_kernel<T, C>, dim3(blocks), dim3(C::THREADS), smem, a.stream, a, plan, po, mz, meta);
   if (e != cudaSuccess) return e;
-  return launch_pdl(merge_kernel<T, C::DP, C::BR>, dim3((unsigned)workers), dim3(kMergeThreads), 0, a.stream, a, plan.group,
+  return launch_pdl(merge_kernel<T, C::DP, C::BR>, dim3((unsigned)workers), dim3(kMergeWarps * 32), 0, a.stream, a, plan.group,
                     (const float*)po, (const float2*)mz, (const Meta*)meta);
 }
 
