@@ -39,6 +39,28 @@ def _stream(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def raw_stream(device: torch.device) -> int:
+    """The handle of the device's current stream, without the stream object around it (2 us a call less
+    than ``_stream``, which shows in calls that the GPU answers within 10 us)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+class _NoSwitch:
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_no_switch = _NoSwitch()
+
+
+def on_device(device: torch.device):
+    """``torch.cuda.device(device)``, free where that device is current already."""
+    return _no_switch if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
 def _validate(q, k, v, log_gain):
     if q.dtype != k.dtype or q.dtype != v.dtype:
         raise ValueError("CA Q,K,V must share dtype")

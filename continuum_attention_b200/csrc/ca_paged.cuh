@@ -1,5 +1,10 @@
 // ca_paged.cuh -- how the kernels over a paged cache divide their work: units (row tile,
 // key head, sequence), their tiles of keys, and equal ranges of all tiles for the workers.
+//
+// Entering and leaving a unit costs as much as some tiles (row set-up, query loads, the
+// output), so a unit takes `unit_cost` places in the stream before its first tile: a tile is
+// done by the worker in whose range its place lies.  Without them a batch with many short
+// sequences left 40% of the SMs' time unused behind the workers that had got those.
 #pragma once
 
 #include <algorithm>
@@ -21,12 +26,13 @@ struct Plan {
   int page_size;
   int capacity;           // keys that a page-table row covers
   int row_lo, row_hi;     // rows (tokens * group) of the sequences that this launch takes
-  unsigned min_tiles;     // of a worker's range
+  unsigned min_places;     // places of a worker's range, at least
+  int unit_cost;          // places that a unit takes before its first tile
   int unit_rows;          // rows that one copy brings
 
   __device__ __forceinline__ int page_of(int key) const { return page_shift >= 0 ? key >> page_shift : key / page_size; }
-  __device__ __forceinline__ unsigned tiles_per_worker(unsigned total, int workers) const {
-    return max((total + workers - 1) / (unsigned)workers, min_tiles);
+  __device__ __forceinline__ unsigned places_per_worker(unsigned total, int workers) const {
+    return max((total + workers - 1) / (unsigned)workers, min_places);
   }
 };
 
@@ -40,7 +46,8 @@ inline Plan make_plan(const Args& a) {
   p.capacity = a.pages_per_seq * a.page_size;
   p.row_lo = 0;
   p.row_hi = 0x7fffffff;
-  p.min_tiles = 1;
+  p.min_places = 1;
+  p.unit_cost = 0;
   p.unit_rows = 1;
   return p;
 }
@@ -56,7 +63,7 @@ struct Meta {
   int pieces, slot, start, rows, h, rt;
 };
 
-// Prefix sums of the sequences' tiles in shared memory (all threads of the block take part in the
+// Prefix sums of the sequences' places in shared memory (all threads of the block take part in the
 // constructor), and cursors into the stream of tiles: sequence, key head, row tile, key tile.
 template <int BR, int TK>
 struct Schedule {
@@ -67,6 +74,7 @@ struct Schedule {
 
   struct Cursor {
     int s, h, rt, kt, nt;
+    unsigned at;       // the tile's place in the stream
     int start, n, len, bad;
     int tiles_rt;      // row tiles
   };
@@ -108,7 +116,7 @@ struct Schedule {
       if (s < a.seqs) load(s, start, n, len, bad);
       const int rows = n * plan.group;
       const int nrt = (rows + BR - 1) / BR;
-      unsigned long long tiles = nrt == 1 ? unit_tiles(0, rows, len - n) : 0;
+      unsigned long long tiles = nrt == 1 ? unit_tiles(0, rows, len - n) + plan.unit_cost : 0;
       unsigned many = __ballot_sync(0xffffffffu, nrt > 1);
       while (many) {
         const int b = __ffs(many) - 1;
@@ -116,7 +124,7 @@ struct Schedule {
         const int rows_b = __shfl_sync(0xffffffffu, rows, b), lead_b = __shfl_sync(0xffffffffu, len - n, b);
         const int nrt_b = __shfl_sync(0xffffffffu, nrt, b);
         unsigned long long sum = 0;
-        for (int rt = lane; rt < nrt_b; rt += 32) sum += unit_tiles(rt, rows_b, lead_b);
+        for (int rt = lane; rt < nrt_b; rt += 32) sum += unit_tiles(rt, rows_b, lead_b) + plan.unit_cost;
 #pragma unroll
         for (int off = 16; off; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
         if (lane == b) tiles = sum;
@@ -156,7 +164,7 @@ struct Schedule {
     c.tiles_rt = (c.n * plan.group + BR - 1) / BR;
   }
 
-  // whole warps call this
+  // the first tile at place x or behind it, in the unit that has x; whole warps call this
   __device__ Cursor locate(unsigned x) const {
     Cursor c;
     int lo = 0, hi = a.seqs;               // the sequence with prefix[s] <= x < prefix[s + 1]
@@ -177,7 +185,7 @@ struct Schedule {
       const int lane = threadIdx.x & 31;
       for (int r0 = 0; r0 < c.tiles_rt; r0 += 32) {
         const int rt = r0 + lane;
-        const unsigned own = rt < c.tiles_rt ? (unsigned)unit_tiles(rt, rows, lead) : 0;
+        const unsigned own = rt < c.tiles_rt ? (unsigned)(unit_tiles(rt, rows, lead) + plan.unit_cost) : 0;
         unsigned v = own;
 #pragma unroll
         for (int off = 1; off < 32; off <<= 1) {
@@ -194,20 +202,24 @@ struct Schedule {
         y -= __shfl_sync(0xffffffffu, v, 31);
       }
     }
-    c.kt = (int)y;
+    c.kt = max((int)y - plan.unit_cost, 0);
+    c.at = x + max(plan.unit_cost - (int)y, 0);
     c.nt = unit_tiles(c.rt, rows, lead);
     return c;
   }
 
   __device__ __forceinline__ void advance(Cursor& c) const {
+    ++c.at;
     if (++c.kt < c.nt) return;
     c.kt = 0;
+    c.at += plan.unit_cost;
     if (++c.rt == c.tiles_rt) {
       c.rt = 0;
       if (++c.h == a.G) {
         c.h = 0;
         do ++c.s;
-        while (prefix[c.s + 1] == prefix[c.s]);
+        while (c.s < a.seqs && prefix[c.s + 1] == prefix[c.s]);
+        if (c.s == a.seqs) return;      // behind the last tile; `at` is behind every range
         enter(c);
       }
     }

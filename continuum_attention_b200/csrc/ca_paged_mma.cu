@@ -270,7 +270,10 @@ struct Config {
   // behind the stages: each warp's V row of the tile before (in the banks that the fragments leave free),
   // descriptors, barriers, the flag of a wait that gave up
   static constexpr int WARP_HALO = ROWB + 128;
-  static constexpr int DESC_AT = NST * STAGE + RW * WARP_HALO;
+  // several warps: query fragments wait here for the next tile (16 registers that the moments need more)
+  static constexpr int Q_FRAG = RW > 1 ? DP * 32 : 0;   // bytes of a warp
+  static constexpr int QF_AT = NST * STAGE + RW * WARP_HALO;
+  static constexpr int DESC_AT = QF_AT + RW * Q_FRAG;
   static constexpr int BAR_AT = DESC_AT + RING * 48;
   static constexpr int GROUP_STRIDE = (BAR_AT + 2 * NST * 8 + 16 + 127) / 128 * 128;
   static constexpr int SMEM = GROUPS * GROUP_STRIDE;    // and the prefix sums behind it
@@ -287,16 +290,21 @@ struct Desc {   // one tile of the stream
   int start, n, len;  // the sequence
   int h, rt;          // key head, row tile
   int bad;            // the sequence's length or one of the tile's pages is out of range
-  int fill[2];
+  int halo_page;      // of the key before a piece that does not start at key 0
+  int end;            // 1: the worker's last tile; 2: it has none
 };
 static_assert(sizeof(Desc) == 48, "");
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(C::THREADS, 1)
     mma_kernel(const __grid_constant__ Args a, const __grid_constant__ Plan plan, float* __restrict__ part_o,
-               float2* __restrict__ part_mz, Meta* __restrict__ meta) {
+               float2* __restrict__ part_mz, Meta* __restrict__ meta, int after_chunks) {
   extern __shared__ __align__(1024) uint8_t smem[];
-  pdl_wait();
+  // after_chunks: the kernel before this one in the stream is the chunks' launch of the same call.  Nothing
+  // here depends on it, and what both depend on was complete before it let this one start; so this one
+  // fills the SMs that it leaves, and waits for it at the end (every warp that leaves), since the merge
+  // that follows waits for this kernel only.
+  if (!after_chunks) pdl_wait();
   pdl_launch_dependents();
   constexpr int TK = C::TK, NJ = C::NJ, DP = C::DP, ROWB = C::ROWB, CH = C::CH, NST = C::NST;
   constexpr int NKK = DP / 16;                 // k-steps of Q K^T
@@ -330,26 +338,38 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   Schedule<C::BR, TK> sched(a, plan, prefix);   // a barrier of the block among other things
   const unsigned total = sched.total;
   const int worker = blockIdx.x * C::GROUPS + group, workers = gridDim.x * C::GROUPS;
-  const unsigned per = plan.tiles_per_worker(total, workers);
-  const unsigned long long x0l = (unsigned long long)worker * per;
-  const unsigned x0 = (unsigned)min(x0l, (unsigned long long)total), x1 = min(total, x0 + per);
+  const unsigned per = plan.places_per_worker(total, workers);
+  const unsigned x0 = (unsigned)min((unsigned long long)worker * per, (unsigned long long)total);
+  const unsigned x1 = (unsigned)min((unsigned long long)x0 + per, (unsigned long long)total);
 
   if (producer) {
     if constexpr (C::REGS_C > 0) regs_down<C::REGS_P>();
-    if (group >= C::GROUPS || x0 >= x1) {
-      if (group < C::GROUPS && lane == 0) meta[worker].pieces = 0;
+    if (group >= C::GROUPS) {
+      if (after_chunks) pdl_wait();
       return;
     }
-    // `cur` stands at tile xa, the next to be described; a tile's pages are fetched when it is described, one
-    // tile before its copies are issued
-  typename Schedule<C::BR, TK>::Cursor cur = sched.locate(x0);
-  unsigned xa = x0;
-  int slot_a = 0;
-  constexpr int NP = TK / 32;
-  int pg[NP];
+    // `cur` stands at the next tile to be described; a tile's pages are fetched when it is described, one tile
+    // before its copies are issued
+    typename Schedule<C::BR, TK>::Cursor cur;
+    cur.at = x1;
+    if (x0 < x1) cur = sched.locate(x0);
+    if (cur.at >= x1) {            // no tile's place lies in this range
+      if (lane == 0) {
+        meta[worker].pieces = 0;
+        descs[0].end = 2;
+        bar_expect(full, 0);
+      }
+      if (after_chunks) pdl_wait();
+      return;
+    }
+    int slot_a = 0, kt0 = 0;       // kt0: the first tile of the piece
+    bool more = true, first = true, in_first = true;
+    constexpr int NP = TK / 32;
+    int pg[NP];
 
   auto describe = [&]() {
-    if (xa < x1) {
+    if (more) {
+      const int seq_now = cur.s;
 #pragma unroll
       for (int k = 0; k < NP; ++k) {
         const int row = plan.unit_rows == 1 ? lane + 32 * k : (k == 0 && lane < 8 ? lane * NJ : TK);
@@ -357,26 +377,48 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         pg[k] = -1;
         if (row < TK && key < cur.len) pg[k] = a.page_table[(size_t)cur.s * a.page_table_stride + plan.page_of(key)];
       }
-      if (lane == 0) {
-        Desc d;
-        d.kt = cur.kt;
-        d.nt = cur.nt;
-        d.first = xa == x0 || cur.kt == 0;
-        d.last = xa + 1 == x1 || cur.kt + 1 == cur.nt;
-        d.start = cur.start;
-        d.n = cur.n;
-        d.len = cur.len;
-        d.h = cur.h;
-        d.rt = cur.rt;
-        d.bad = cur.bad;
-        // the page of the key before the piece
-        d.fill[0] = d.first && cur.kt > 0
-                        ? a.page_table[(size_t)cur.s * a.page_table_stride + plan.page_of(cur.kt * TK - 1)] : -1;
-        descs[slot_a] = d;
+      if (first || cur.kt == 0) {
+        kt0 = cur.kt;
+        in_first = first;
       }
-      if (xa + 1 < x1) sched.advance(cur);
+      more = cur.at + 1 < x1;
+      Desc d;
+      d.kt = cur.kt;
+      d.nt = cur.nt;
+      d.first = first || cur.kt == 0;
+      d.last = !more || cur.kt + 1 == cur.nt;
+      d.start = cur.start;
+      d.n = cur.n;
+      d.len = cur.len;
+      d.h = cur.h;
+      d.rt = cur.rt;
+      d.bad = cur.bad;
+      first = false;
+      const unsigned at = cur.at;
+      if (more) {
+        sched.advance(cur);
+        more = cur.at < x1;        // the next unit's first tile may lie behind the range
+      }
+      d.end = more ? 0 : 1;
+      if (lane == 0) {
+        d.halo_page = -1;
+        if (d.first && d.kt > 0) {
+          d.halo_page = a.page_table[(size_t)seq_now * a.page_table_stride + plan.page_of(d.kt * TK - 1)];
+        }
+        descs[slot_a] = d;
+        if (!more) {
+          // this worker joins the unit that starts in its range and goes on behind it
+          Meta mt;
+          mt.pieces = kt0 == 0 && d.kt + 1 < d.nt ? 1 + (int)((at + (d.nt - 1 - d.kt)) / per) - worker : 0;
+          mt.slot = in_first ? 0 : 1;
+          mt.start = d.start;
+          mt.rows = d.n * plan.group;
+          mt.h = d.h;
+          mt.rt = d.rt;
+          meta[worker] = mt;
+        }
+      }
     }
-    ++xa;
     if (++slot_a == C::RING) slot_a = 0;
     __syncwarp();
   };
@@ -389,8 +431,8 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   int slot_b = 0, stage_b = 0;
   uint32_t empty_parity = 1;      // of the stage's previous use
   describe();
-  for (unsigned xb = x0; xb < x1; ++xb) {
-    if (xb >= x0 + NST && !bar_wait(empty + 8 * stage_b, empty_parity, gave_up)) {
+  for (int k = 0, end = 0; !end; ++k) {
+    if (k >= NST && !bar_wait(empty + 8 * stage_b, empty_parity, gave_up)) {
       // copies may still be on their way: leave no sooner than they land, or another limit runs out
       *gave_up = 0;
       __syncwarp();
@@ -401,12 +443,14 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           empty_parity ^= 1;
         }
       }
+      if (after_chunks) pdl_wait();
       return;
     }
     {
       Desc& d = descs[slot_b];
       const uint32_t st = g0 + stage_b * C::STAGE, bar = full + 8 * stage_b;
       const int base = d.kt * TK, len = d.len, h = d.h, first = d.first;
+      end = d.end;
       const uint32_t row_bytes = (uint32_t)a.D * 2;
       const uint32_t unit_bytes = plan.unit_rows * row_bytes;
       bool go[NP], bad = false;
@@ -420,7 +464,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         go[k] = go[k] && in;
         bytes += __popc(__ballot_sync(0xffffffffu, go[k])) * 2 * unit_bytes;
       }
-      const int halo_page = d.fill[0];
+      const int halo_page = d.halo_page;
       const bool halo = first && base > 0 && base - 1 < len;
       const bool halo_go = halo && halo_page >= 0 && halo_page < a.num_pages;
       bad |= halo && !halo_go;
@@ -467,8 +511,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       stage_b = 0;
       empty_parity ^= 1;
     }
-    describe();
+    if (!end) describe();
   }
+  if (after_chunks) pdl_wait();
   return;
   }
 
@@ -491,14 +536,16 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   const uint32_t my_halo = g0 + NST * C::STAGE + warp * C::WARP_HALO + 112;
   uint8_t* my_halo_p = gsm + NST * C::STAGE + warp * C::WARP_HALO + 112;
 
+  uint8_t* my_qf = gsm + C::QF_AT + warp * C::Q_FRAG + 16 * lane;
+
   int slot = 0, stage = 0;
   uint32_t parity = 0;
-  for (unsigned x = x0; x < x1; ++x) {
-    if (!bar_wait(full + 8 * stage, parity, gave_up)) {
-      if (warp == 0 && lane == 0) meta[worker].pieces = 0;
-      return;
-    }
+  bool first_tile = true;
+  for (int end = 0; !end;) {
+    if (!bar_wait(full + 8 * stage, parity, gave_up)) break;
     const Desc& d = descs[slot];
+    end = d.end;
+    if (end == 2) break;
     uint8_t* sm = gsm + stage * C::STAGE;
     const uint32_t st = g0 + stage * C::STAGE;
     const int base = d.kt * TK;
@@ -506,7 +553,8 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     if (d.first) {
       kt0 = d.kt;
       piece_bad = 0;
-      in_first = x == x0;
+      in_first = first_tile;
+      first_tile = false;
       const int row0 = d.rt * C::BR + warp * C::RPW;
       const int row_last = min(rows, row0 + C::RPW) - 1;    // < row0: the warp has no row
       const int lead = d.len - d.n;                         // position of the sequence's first row
@@ -550,6 +598,11 @@ __global__ void __launch_bounds__(C::THREADS, 1)
           if (RS == 1) qf[k][1] = qf[k][3] = 0u;
         }
       }
+      if constexpr (C::Q_FRAG > 0) {
+#pragma unroll
+        for (int k = 0; k < NKK; ++k)
+          *reinterpret_cast<uint4*>(my_qf + 512 * k) = make_uint4(qf[k][0], qf[k][1], qf[k][2], qf[k][3]);
+      }
       if (d.kt > 0 && base - 1 <= i_max) {
         // the score of key base - 1, in every column of one score tile
         float s[4] = {0.f, 0.f, 0.f, 0.f};
@@ -586,6 +639,16 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     if (base - 1 <= i_max && i_max >= 0) {
       float2 s[RS][NJ];
       const uint32_t ka = st + k_lane;
+      if constexpr (C::Q_FRAG > 0) {
+#pragma unroll
+        for (int k = 0; k < NKK; ++k) {
+          const uint4 t = *reinterpret_cast<const uint4*>(my_qf + 512 * k);
+          qf[k][0] = t.x;
+          qf[k][1] = t.y;
+          qf[k][2] = t.z;
+          qf[k][3] = t.w;
+        }
+      }
       // score tiles side by side, so that no product waits for the one before it
       float acc[NJ][4];
 #pragma unroll
@@ -744,17 +807,6 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       __syncwarp();
       if (lane < CH) *reinterpret_cast<uint4*>(my_halo_p + 16 * lane) = *reinterpret_cast<const uint4*>(vlast + 16 * lane);
     }
-    if (x + 1 == x1 && warp == 0 && lane == 0) {
-      // this worker joins the unit that starts in its range and goes on behind it
-      Meta mt;
-      mt.pieces = kt0 == 0 && d.kt + 1 < d.nt ? 1 + (d.nt - d.kt - 2 + (int)per) / (int)per : 0;
-      mt.slot = in_first ? 0 : 1;
-      mt.start = d.start;
-      mt.rows = rows;
-      mt.h = d.h;
-      mt.rt = d.rt;
-      meta[worker] = mt;
-    }
     __syncwarp();
     if (lane == 0) bar_arrive(empty + 8 * stage);
     if (++slot == C::RING) slot = 0;
@@ -763,6 +815,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       parity ^= 1;
     }
   }
+  if (after_chunks) pdl_wait();
 }
 
 // Joins the pieces of a cut unit: piece 0 is in this worker's slot, the others are the first pieces of the
@@ -787,17 +840,30 @@ struct Sum {
   }
 };
 
-template <typename T, int DP, int BR>
-__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(Args a, int group, const float* __restrict__ part_o,
-                                                                 const float2* __restrict__ part_mz,
-                                                                 const Meta* __restrict__ meta) {
+// the pieces of one launch: units of br rows
+struct Pieces {
+  float* o;
+  float2* mz;
+  Meta* meta;
+  int br, workers;
+};
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ Args a, int group,
+                                                                 const __grid_constant__ Pieces one,
+                                                                 const __grid_constant__ Pieces two) {
   pdl_wait();
   pdl_launch_dependents();
+  const bool second = (int)blockIdx.x >= one.workers;
+  const Pieces& pc = second ? two : one;
+  const float* part_o = pc.o;
+  const float2* part_mz = pc.mz;
+  const int BR = pc.br;
   constexpr int VL = DP / 32;                        // values per lane: 2 or 4
   __shared__ float4 sum_y[kMergeWarps][32];
   __shared__ float2 sum_mz[kMergeWarps];
-  const int w = blockIdx.x;
-  const Meta mt = meta[w];
+  const int w = (int)blockIdx.x - (second ? one.workers : 0);
+  const Meta mt = pc.meta[w];
   if (mt.pieces == 0) return;
   const int nrows = min(BR, mt.rows - mt.rt * BR);
   int share = 1;                                     // warps per row
@@ -846,14 +912,27 @@ namespace {
 // The forms: decoding with 8 or 16 rows a warp, and chunks
 template <int DP> using Decode8 = std::conditional_t<DP == 64, Config<64, 32, 8, 1, 8, 2, 200, 56>, Config<128, 32, 8, 1, 4, 2, 0, 0>>;
 template <int DP> using Decode16 = std::conditional_t<DP == 64, Config<64, 32, 16, 1, 8, 2, 200, 56>, Config<128, 32, 16, 1, 4, 2, 0, 0>>;
-template <int DP> using Chunk = Config<DP, DP == 64 ? 64 : 32, 16, 4, 3, 4, 152, 56>;
+template <int DP> using Chunk = Config<DP, DP == 64 ? 64 : 32, 16, 4, 3, 3, 152, 56>;
 
-size_t part_bytes(long long workers, int br, int dp) {
-  return (size_t)workers * 2 * br * (dp * sizeof(float) + sizeof(float2)) + (size_t)workers * sizeof(Meta) + 768;
+constexpr int kDecodeUnitCost = 2, kChunkUnitCost = 2;
+
+size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+template <typename C>
+size_t pieces_bytes() {
+  const size_t w = (size_t)num_sms_cached() * C::GROUPS;
+  return up256(w * 2 * C::BR * C::DP * sizeof(float)) + up256(w * 2 * C::BR * sizeof(float2)) + up256(w * sizeof(Meta));
+}
+
+template <typename C>
+Pieces carve(char* ws) {
+  const size_t w = (size_t)num_sms_cached() * C::GROUPS;
+  const size_t o = up256(w * 2 * C::BR * C::DP * sizeof(float)), mz = up256(w * 2 * C::BR * sizeof(float2));
+  return Pieces{(float*)ws, (float2*)(ws + o), (Meta*)(ws + o + mz), C::BR, (int)w};
 }
 
 template <typename T, typename C>
-cudaError_t launch(const Args& a, Plan plan, void* workspace) {
+cudaError_t launch_main(const Args& a, Plan plan, const Pieces& pc, bool after_chunks) {
   static_assert(C::SMEM + (kMaxSeqs + 1) * (int)sizeof(unsigned) <= 232448, "shared memory of a block");
   const size_t smem = C::SMEM + (size_t)(a.seqs + 1) * sizeof(unsigned);
   static thread_local int set_dev = -1;    // the attribute belongs to the device
@@ -866,38 +945,45 @@ cudaError_t launch(const Args& a, Plan plan, void* workspace) {
     if (e != cudaSuccess) return e;
     set_dev = dev;
   }
-  const int blocks = num_sms_cached();
   plan.unit_rows = a.D == C::DP && a.slot_stride == C::DP && a.page_size % C::NJ == 0 ? C::NJ : 1;
-  const long long workers = (long long)blocks * C::GROUPS;
-  char* ws = (char*)workspace;
-  auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-  float* po = (float*)ws;
-  float2* mz = (float2*)(ws + up((size_t)workers * 2 * C::BR * C::DP * sizeof(float)));
-  Meta* meta = (Meta*)((char*)mz + up((size_t)workers * 2 * C::BR * sizeof(float2)));
-  e = launch_pdl(mma_kernel<T, C>, dim3(blocks), dim3(C::THREADS), smem, a.stream, a, plan, po, mz, meta);
-  if (e != cudaSuccess) return e;
-  return launch_pdl(merge_kernel<T, C::DP, C::BR>, dim3((unsigned)workers), dim3(kMergeWarps * 32), 0, a.stream, a, plan.group,
-                    (const float*)po, (const float2*)mz, (const Meta*)meta);
+  return launch_pdl(mma_kernel<T, C>, dim3(num_sms_cached()), dim3(C::THREADS), smem, a.stream, a, plan, pc.o, pc.mz,
+                    pc.meta, (int)after_chunks);
+}
+
+template <typename T, int DP>
+cudaError_t launch_merge(const Args& a, const Plan& plan, const Pieces& one, const Pieces& two) {
+  return launch_pdl(merge_kernel<T, DP>, dim3((unsigned)(one.workers + two.workers)), dim3(kMergeWarps * 32), 0,
+                    a.stream, a, plan.group, one, two);
 }
 
 template <typename T, int DP>
 cudaError_t forward_dp(const Args& a, void* workspace) {
   Plan plan = make_plan(a);
+  char* ws = (char*)workspace;
   const long long rows = (long long)a.max_q_len * plan.group;
+  plan.unit_cost = kDecodeUnitCost;
   if (rows <= 16) {
     // every sequence, whatever its rows: max_q_len may be wrong
-    return rows <= 8 ? launch<T, Decode8<DP>>(a, plan, workspace) : launch<T, Decode16<DP>>(a, plan, workspace);
+    const Pieces pc = rows <= 8 ? carve<Decode8<DP>>(ws) : carve<Decode16<DP>>(ws);
+    cudaError_t e = rows <= 8 ? launch_main<T, Decode8<DP>>(a, plan, pc, false)
+                              : launch_main<T, Decode16<DP>>(a, plan, pc, false);
+    return e != cudaSuccess ? e : launch_merge<T, DP>(a, plan, pc, Pieces{});
   }
-  // sequences of up to 16 rows in the decoding form, the others as chunks; both use the workspace, one
-  // after the other
-  plan.min_tiles = 4;
-  plan.row_lo = 17;
-  cudaError_t e = launch<T, Chunk<DP>>(a, plan, workspace);
-  if (e != cudaSuccess || a.seqs == 1) return e;
-  plan.min_tiles = 1;
-  plan.row_lo = 0;
+  // sequences of up to 16 rows in the decoding form, the others as chunks
+  Plan chunks = plan;
+  chunks.min_places = 4;
+  chunks.unit_cost = kChunkUnitCost;
+  chunks.row_lo = 17;
+  // (a single sequence is all in one form, whatever its rows)
+  if (a.seqs == 1) chunks.row_lo = 0;
+  const Pieces pc = carve<Chunk<DP>>(ws);
+  cudaError_t e = launch_main<T, Chunk<DP>>(a, chunks, pc, false);
+  if (e != cudaSuccess) return e;
+  if (a.seqs == 1) return launch_merge<T, DP>(a, plan, pc, Pieces{});
   plan.row_hi = 16;
-  return launch<T, Decode16<DP>>(a, plan, workspace);
+  const Pieces few = carve<Decode16<DP>>(ws + pieces_bytes<Chunk<DP>>());
+  e = launch_main<T, Decode16<DP>>(a, plan, few, true);
+  return e != cudaSuccess ? e : launch_merge<T, DP>(a, plan, pc, few);
 }
 
 }  // namespace
@@ -905,12 +991,10 @@ cudaError_t forward_dp(const Args& a, void* workspace) {
 size_t mma_workspace_bytes(long long max_q_len, long long H, long long G, long long D) {
   const long long rows = max_q_len * (H / G);
   auto bytes = [&](auto d8, auto d16, auto chunk) {
-    auto part = [](auto c) {
-      using C = decltype(c);
-      return part_bytes((long long)num_sms_cached() * C::GROUPS, C::BR, C::DP);
-    };
-    const size_t decode = std::max(part(d8), part(d16));
-    return rows <= 16 ? decode : std::max(decode, part(chunk));
+    using D8 = decltype(d8);
+    using D16 = decltype(d16);
+    using Ck = decltype(chunk);
+    return rows <= 8 ? pieces_bytes<D8>() : rows <= 16 ? pieces_bytes<D16>() : pieces_bytes<Ck>() + pieces_bytes<D16>();
   };
   return D <= 64 ? bytes(Decode8<64>{}, Decode16<64>{}, Chunk<64>{}) : bytes(Decode8<128>{}, Decode16<128>{}, Chunk<128>{});
 }
@@ -924,7 +1008,7 @@ cudaError_t mma_read_status(int* out, bool reset) {
 
 int mma_launches(const Args& a) {
   const long long rows = (long long)a.max_q_len * (a.H / a.G);
-  return rows <= 16 || a.seqs == 1 ? 2 : 4;
+  return rows <= 16 || a.seqs == 1 ? 2 : 3;
 }
 
 cudaError_t mma_forward(const Args& a, int dtype, void* workspace) {

@@ -17,7 +17,7 @@ from typing import Optional, Sequence
 import torch
 
 from . import _native
-from .attention import _DTYPE_CODE, _stream, ctypes_ptr
+from .attention import _DTYPE_CODE, on_device, raw_stream
 
 
 def check_cache(what, k_cache, v_cache, page_table, kv_lens, q_starts, dtype, device):
@@ -32,25 +32,28 @@ def check_cache(what, k_cache, v_cache, page_table, kv_lens, q_starts, dtype, de
     P, G, page, D = k_cache.shape
     if G < 1 or page < 1:
         raise ValueError(f"{what}: the cache needs kv_heads and page_size >= 1; got {tuple(k_cache.shape)}")
-    if k_cache.stride() != v_cache.stride():
+    strides = k_cache.stride()
+    if strides != v_cache.stride():
         raise ValueError(f"{what}: k_cache and v_cache must share strides")
-    if k_cache.stride(3) != 1 or any((s * k_cache.element_size()) % 16 for s in k_cache.stride()[:3]) \
+    unit = 16 // k_cache.element_size()
+    if strides[3] != 1 or strides[0] % unit or strides[1] % unit or strides[2] % unit \
             or k_cache.data_ptr() % 16 or v_cache.data_ptr() % 16:
         raise ValueError(f"{what}: the cache's D values must be contiguous, its strides and start multiples of "
                          "16 bytes")
+    S = kv_lens.numel()
     if page_table.dim() != 2 or kv_lens.dim() != 1 or q_starts.dim() != 1 \
-            or page_table.shape[0] != kv_lens.shape[0] or q_starts.shape[0] != kv_lens.shape[0] + 1:
+            or page_table.shape[0] != S or q_starts.numel() != S + 1:
         raise ValueError(f"{what}: expected page_table [S, pages], kv_lens [S], q_starts [S+1]; got "
                          f"{tuple(page_table.shape)}, {tuple(kv_lens.shape)}, {tuple(q_starts.shape)}")
-    if any(t.dtype != torch.int32 for t in (page_table, kv_lens, q_starts)):
+    if page_table.dtype != torch.int32 or kv_lens.dtype != torch.int32 or q_starts.dtype != torch.int32:
         raise TypeError(f"{what}: page_table, kv_lens and q_starts must be int32")
-    if (page_table.shape[1] > 1 and page_table.stride(1) != 1) or \
-            (page_table.shape[0] > 1 and page_table.stride(0) < page_table.shape[1]) or \
-            not kv_lens.is_contiguous() or not q_starts.is_contiguous():
+    if not (kv_lens.is_contiguous() and q_starts.is_contiguous()) or \
+            (not page_table.is_contiguous() and ((page_table.shape[1] > 1 and page_table.stride(1) != 1) or
+                                                 (S > 1 and page_table.stride(0) < page_table.shape[1]))):
         raise ValueError(f"{what}: page_table rows, kv_lens and q_starts must be contiguous")
     if device.type != "cuda":
         raise RuntimeError("continuum_attention_b200 runs on CUDA tensors only (no CPU fallback)")
-    if any(t.device != device for t in (k_cache, v_cache, page_table, kv_lens, q_starts)):
+    if not (k_cache.device == v_cache.device == page_table.device == kv_lens.device == q_starts.device == device):
         raise RuntimeError(f"{what}: every tensor must be on {device}")
     return P, G, page, D
 
@@ -98,8 +101,11 @@ def continuum_attention_paged(q, k_cache, v_cache, page_table, kv_lens, q_starts
         raise ValueError(f"max_q_len must be >= 1, got {max_q_len}")
     if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
         raise RuntimeError("continuum_attention_paged has no backward; call it under torch.no_grad()")
-    lg = log_gain.detach().to(device=q.device, dtype=torch.float32).contiguous()
-    if q.stride(2) != 1 or any((s * q.element_size()) % 16 for s in q.stride()[:2]) or q.data_ptr() % 16:
+    lg = log_gain.detach()
+    if lg.dtype != torch.float32 or lg.device != q.device or not lg.is_contiguous():
+        lg = lg.to(device=q.device, dtype=torch.float32).contiguous()
+    unit = 16 // q.element_size()
+    if q.stride(2) != 1 or q.stride(0) % unit or q.stride(1) % unit or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
     if out is None:
         out = torch.empty(N, H, D, dtype=q.dtype, device=q.device)
@@ -107,26 +113,27 @@ def continuum_attention_paged(q, k_cache, v_cache, page_table, kv_lens, q_starts
             or out.data_ptr() % 16:
         raise ValueError(f"continuum_attention_paged: out must be a contiguous, 16-byte aligned {q.dtype} "
                          f"[{N}, {H}, {D}] on {q.device}")
-    S = kv_lens.shape[0]
+    S = kv_lens.numel()
     if N == 0 or S == 0:
         return out
     lib = _native.lib()
     code = _DTYPE_CODE[q.dtype]
     max_q_len = min(int(max_q_len), N)
-    with torch.cuda.device(q.device):
-        nbytes = int(lib.ca_paged_workspace_size(S, max_q_len, H, G, D, code))
-    if workspace is None:
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    elif workspace.device != q.device or workspace.numel() * workspace.element_size() < nbytes \
-            or not workspace.is_contiguous():
-        raise ValueError(f"continuum_attention_paged: workspace must be {nbytes} contiguous bytes on {q.device}")
-    with torch.cuda.device(q.device):
+    with on_device(q.device):
+        nbytes = lib.ca_paged_workspace_size(S, max_q_len, H, G, D, code)
+        if workspace is None:
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            given = nbytes
+        else:
+            given = workspace.numel() * workspace.element_size()
+            if workspace.device != q.device or given < nbytes or not workspace.is_contiguous():
+                raise ValueError(f"continuum_attention_paged: workspace must be {nbytes} contiguous bytes on {q.device}")
+        ks, ps, ss, _ = k_cache.stride()
         st = lib.ca_paged_forward(
-            ctypes_ptr(q), q.stride(0), q.stride(1), ctypes_ptr(k_cache), ctypes_ptr(v_cache), k_cache.stride(0),
-            k_cache.stride(1), k_cache.stride(2), ctypes_ptr(page_table), page_table.stride(0), ctypes_ptr(kv_lens),
-            ctypes_ptr(q_starts), ctypes_ptr(lg), ctypes_ptr(out), ctypes_ptr(workspace),
-            workspace.numel() * workspace.element_size(), N, S, max_q_len, H, G, D, P, page, page_table.shape[1], code,
-            _stream(q.device))
+            q.data_ptr(), q.stride(0), q.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), ks, ps, ss,
+            page_table.data_ptr(), page_table.stride(0), kv_lens.data_ptr(), q_starts.data_ptr(), lg.data_ptr(),
+            out.data_ptr(), workspace.data_ptr(), given, N, S, max_q_len, H, G, D, P, page, page_table.shape[1], code,
+            raw_stream(q.device))
     _native.check("ca_paged_forward", st)
     return out
 

@@ -27,7 +27,7 @@ from typing import Optional
 import torch
 
 from . import _native
-from .attention import _DTYPE_CODE, _stream, ctypes_ptr
+from .attention import _DTYPE_CODE, ctypes_ptr, on_device, raw_stream
 from .paged import check_cache
 
 _LAYOUTS = {"interleaved": _native.CA_ROTARY_INTERLEAVED, "half": _native.CA_ROTARY_HALF}
@@ -137,11 +137,11 @@ class RotaryQKVFunction(torch.autograd.Function):
         k = torch.empty(B, kv_heads, T, D, dtype=qkv.dtype, device=qkv.device)
         v = torch.empty_like(k)
         stride = 0 if positions is None or positions.dim() == 1 else positions.stride(0)
-        with torch.cuda.device(qkv.device):
+        with on_device(qkv.device):
             st = _native.lib().ca_rotary_qkv_forward(
                 ctypes_ptr(qkv), width, ctypes_ptr(cos_sin), None if positions is None else ctypes_ptr(positions),
                 stride, ctypes_ptr(q), ctypes_ptr(k), ctypes_ptr(v), B, T, heads, kv_heads, D, 2 * cos_sin.shape[1],
-                cos_sin.shape[0], layout, _DTYPE_CODE[qkv.dtype], _stream(qkv.device))
+                cos_sin.shape[0], layout, _DTYPE_CODE[qkv.dtype], raw_stream(qkv.device))
         _native.check("ca_rotary_qkv_forward", st)
         ctx.save_for_backward(cos_sin, positions)
         ctx.meta = (B, T, heads, kv_heads, D, stride, layout, qkv.dtype)
@@ -157,11 +157,11 @@ class RotaryQKVFunction(torch.autograd.Function):
         grads = [torch.zeros((B, h, T, D), dtype=dtype, device=ref.device) if g is None
                  else _aligned(g.to(dtype).contiguous()) for g, h in zip((dq, dk, dv), (heads, kv_heads, kv_heads))]
         dqkv = torch.empty(B, T, (heads + 2 * kv_heads) * D, dtype=dtype, device=ref.device)
-        with torch.cuda.device(ref.device):
+        with on_device(ref.device):
             st = _native.lib().ca_rotary_qkv_backward(
                 ctypes_ptr(grads[0]), ctypes_ptr(grads[1]), ctypes_ptr(grads[2]), ctypes_ptr(cos_sin),
                 None if positions is None else ctypes_ptr(positions), stride, ctypes_ptr(dqkv), B, T, heads, kv_heads,
-                D, 2 * cos_sin.shape[1], cos_sin.shape[0], layout, _DTYPE_CODE[dtype], _stream(ref.device))
+                D, 2 * cos_sin.shape[1], cos_sin.shape[0], layout, _DTYPE_CODE[dtype], raw_stream(ref.device))
         _native.check("ca_rotary_qkv_backward", st)
         return dqkv, None, None, None, None, None
 
@@ -220,11 +220,11 @@ def rotary_append(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise ValueError(f"rotary_append: out must be a contiguous, 16-byte aligned {qkv.dtype} "
                          f"[{N}, {heads}, {D}] on {qkv.device}")
     cs = table.cos_sin
-    with torch.cuda.device(qkv.device):
+    with on_device(qkv.device):
         st = _native.lib().ca_rotary_append(
             ctypes_ptr(qkv), qkv.stride(0), ctypes_ptr(cs), ctypes_ptr(out), ctypes_ptr(k_cache), ctypes_ptr(v_cache),
             k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), ctypes_ptr(page_table), page_table.stride(0),
             ctypes_ptr(kv_lens), ctypes_ptr(q_starts), N, kv_lens.shape[0], heads, G, D, table.rotary_dim, cs.shape[0],
-            P, page, page_table.shape[1], _LAYOUTS[layout], _DTYPE_CODE[qkv.dtype], _stream(qkv.device))
+            P, page, page_table.shape[1], _LAYOUTS[layout], _DTYPE_CODE[qkv.dtype], raw_stream(qkv.device))
     _native.check("ca_rotary_append", st)
     return out
