@@ -12,9 +12,10 @@
 //
 // HBM-bound: each element of [tokens][H + 2G][D] is read once and written once.  An item
 // is two vectors of W elements of one head: the two that a turn in halves combines, else
-// two adjacent ones, so either layout keeps two independent loads of 16 bytes (16-bit
-// types) or 32 (fp32) in flight per item.  A block takes one token and its threads stride over the token's
-// heads by whole heads, so that a thread keeps its item and reads the table once.
+// two adjacent ones.  A thread keeps its item for several heads, so that it reads the
+// table once, and loads kHeads heads before it stores the first.
+#include <algorithm>
+
 #include "ca_common.cuh"
 #include "ca_internal.h"
 
@@ -25,24 +26,28 @@ namespace rotary {
 __device__ int g_status = 0;
 __device__ __forceinline__ void record_invalid() { atomicCAS(&g_status, 0, 1); }
 
-// W consecutive elements in 32 bits; p aligned to W elements (at least; 16 bytes where W is 8)
+// W consecutive elements as they are; p aligned to W elements (at least; 16 bytes where W is 8)
 template <typename T, int W>
-__device__ __forceinline__ void load_vec(const T* p, float (&x)[W]) {
-  constexpr int kBytes = W * (int)sizeof(T);
-  alignas(16) T e[W];
-  if constexpr (kBytes >= 16) {
+struct Raw {
+  static constexpr int kBytes = W * (int)sizeof(T);
+  alignas(kBytes < 16 ? kBytes : 16) T e[W];
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (kBytes >= 16) {
 #pragma unroll
-    for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(p)[i];
-  } else if constexpr (kBytes == 8) {
-    *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(p);
-  } else if constexpr (kBytes == 4) {
-    *reinterpret_cast<uint32_t*>(e) = *reinterpret_cast<const uint32_t*>(p);
-  } else {
-    e[0] = p[0];
+      for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4*>(e)[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else if constexpr (kBytes == 8) {
+      *reinterpret_cast<uint2*>(e) = *reinterpret_cast<const uint2*>(p);
+    } else if constexpr (kBytes == 4) {
+      *reinterpret_cast<uint32_t*>(e) = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+      e[0] = p[0];
+    }
   }
+  __device__ __forceinline__ void get(float (&x)[W]) const {
 #pragma unroll
-  for (int i = 0; i < W; ++i) x[i] = to_f32<T>(e[i]);
-}
+    for (int i = 0; i < W; ++i) x[i] = to_f32<T>(e[i]);
+  }
+};
 
 template <typename T, int W>
 __device__ __forceinline__ void store_vec(T* p, const float (&x)[W]) {
@@ -132,10 +137,15 @@ __device__ __forceinline__ const float2* table_row(const float2* cs, long long p
   return cs + (bad ? 0 : (size_t)pos * (R / 2));
 }
 
+// heads of a thread whose loads are in flight at once: one is 50% slower on a training batch, four are as
+// fast as two in 32 bits and 60% slower in 16 (registers)
+constexpr int kHeads = 2;
+
 // training, forward: qkv [B*T rows][(H+2G) D] -> q [B,H,T,D], k, v [B,G,T,D] (q, k turned);
-// backward: the other way with the transposed turn
+// backward: the other way with the transposed turn.  A block takes a token: four, whose
+// rows of one head lie side by side in q, k and v, ran 4 to 9% slower.
 template <typename T, int W, bool kHalf, bool kBack>
-__global__ void qkv_kernel(QkvArgs a) {
+__global__ void qkv_kernel(const __grid_constant__ QkvArgs a) {
   pdl_wait();
   pdl_launch_dependents();
   const int ni = items_per_head(a.D, W), heads = a.H + 2 * a.G;
@@ -147,127 +157,155 @@ __global__ void qkv_kernel(QkvArgs a) {
   const float2* row = table_row((const float2*)a.cos_sin, pos, a.table_rows, a.R, bad);
   if (bad && threadIdx.x == 0) record_invalid();
   Item<W, kHalf> item(it, a.D, a.R);
-  item.angles(row, bad, kBack ? -1.f : 1.f, a.R);
   T* packed = (T*)a.qkv + (size_t)token * a.qkv_stride;
-  for (int h = (int)threadIdx.x / ni; h < heads; h += step) {
-    T* split;
-    if (h < a.H) split = (T*)a.q + (((size_t)b * a.H + h) * a.T + t) * a.D;
-    else if (h < a.H + a.G) split = (T*)a.k + (((size_t)b * a.G + (h - a.H)) * a.T + t) * a.D;
-    else split = (T*)a.v + (((size_t)b * a.G + (h - a.H - a.G)) * a.T + t) * a.D;
-    T* flat = packed + (size_t)h * a.D;
-    const T* src = kBack ? split : flat;
-    T* dst = kBack ? flat : split;
-    if (h < a.H + a.G) {
-      float x[W], y[W];
-      load_vec<T, W>(src + item.a, x);
-      if (item.b >= 0) load_vec<T, W>(src + item.b, y);
-      item.apply(x, y, a.R);
-      store_vec<T, W>(dst + item.a, x);
-      if (item.b >= 0) store_vec<T, W>(dst + item.b, y);
-    } else {
-      float x[W];
-      load_vec<T, W>(src + item.a, x);
-      store_vec<T, W>(dst + item.a, x);
-      if (item.b >= 0) {
-        load_vec<T, W>(src + item.b, x);
-        store_vec<T, W>(dst + item.b, x);
-      }
+  auto split = [&](int h) {
+    if (h < a.H) return (T*)a.q + (((size_t)b * a.H + h) * a.T + t) * a.D;
+    if (h < a.H + a.G) return (T*)a.k + (((size_t)b * a.G + (h - a.H)) * a.T + t) * a.D;
+    return (T*)a.v + (((size_t)b * a.G + (h - a.H - a.G)) * a.T + t) * a.D;
+  };
+  bool angles = false;
+  for (int h0 = (int)threadIdx.x / ni; h0 < heads; h0 += step * kHeads) {
+    Raw<T, W> x[kHeads], y[kHeads];
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      const int h = h0 + u * step;
+      if (h >= heads) continue;
+      const T* src = kBack ? split(h) : packed + (size_t)h * a.D;
+      x[u].load(src + item.a);
+      if (item.b >= 0) y[u].load(src + item.b);
+    }
+    if (!angles) item.angles(row, bad, kBack ? -1.f : 1.f, a.R);
+    angles = true;
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      const int h = h0 + u * step;
+      if (h >= heads) continue;
+      float v[W], w[W];
+      x[u].get(v);
+      y[u].get(w);
+      if (h < a.H + a.G) item.apply(v, w, a.R);
+      T* dst = kBack ? packed + (size_t)h * a.D : split(h);
+      store_vec<T, W>(dst + item.a, v);
+      if (item.b >= 0) store_vec<T, W>(dst + item.b, w);
     }
   }
 }
 
 // serving: token n of sequence s (q_starts[s] <= n < q_starts[s+1]) sits at position
 // kv_lens[s] - (q_starts[s+1] - n); its queries go to q [N,H,D], its keys and values to
-// slot pos % page_size of page page_table[s][pos / page_size]
+// slot pos % page_size of page page_table[s][pos / page_size].  The first heads' loads are
+// issued before the sequence is looked up.
 template <typename T, int W, bool kHalf>
-__global__ void append_kernel(AppendArgs a) {
+__global__ void append_kernel(const __grid_constant__ AppendArgs a) {
   pdl_wait();
   pdl_launch_dependents();
   const int ni = items_per_head(a.D, W), heads = a.H + 2 * a.G;
   const int it = (int)threadIdx.x % ni, step = (int)blockDim.x / ni;
   const int n = (int)blockIdx.x;
-  __shared__ int s_seq;
-  if (threadIdx.x == 0) s_seq = -1;
-  __syncthreads();
-  for (int s = threadIdx.x; s < a.seqs; s += blockDim.x)
-    if (a.q_starts[s] <= n && n < a.q_starts[s + 1]) atomicMax(&s_seq, s);
-  __syncthreads();
-  const int s = s_seq;
-  if (s < 0) return;   // a row behind the last sequence
-  const long long pos = (long long)a.kv_lens[s] - a.q_starts[s + 1] + n;
-  const bool none = pos < 0;   // more rows than keys: no key to write, no row to answer
-  bool bad = false;
-  const float2* row = table_row((const float2*)a.cos_sin, none ? 0 : pos, a.table_rows, a.R, bad);
-  size_t cache = 0;
-  if (!none && !bad) {
-    const long long col = pos / a.page_size;
-    int page = -1;
-    if (col < a.pages_per_seq) page = a.page_table[(size_t)s * a.page_table_stride + col];
-    bad = page < 0 || page >= a.num_pages;
-    if (!bad) cache = (size_t)page * a.page_stride + (size_t)(pos - col * a.page_size) * a.slot_stride;
-  }
-  if (bad && threadIdx.x == 0) record_invalid();
   Item<W, kHalf> item(it, a.D, a.R);
-  item.angles(row, bad, 1.f, a.R);
   const T* src0 = (const T*)a.qkv + (size_t)n * a.qkv_stride;
-  for (int h = (int)threadIdx.x / ni; h < heads; h += step) {
-    if (h >= a.H && (none || bad)) break;
-    const T* src = src0 + (size_t)h * a.D;
-    T* dst;
-    if (h < a.H) dst = (T*)a.q + ((size_t)n * a.H + h) * a.D;
-    else if (h < a.H + a.G) dst = (T*)a.k_cache + cache + (size_t)(h - a.H) * a.head_stride;
-    else dst = (T*)a.v_cache + cache + (size_t)(h - a.H - a.G) * a.head_stride;
-    float x[W], y[W];
-    load_vec<T, W>(src + item.a, x);
-    if (item.b >= 0) load_vec<T, W>(src + item.b, y);
-    if (none || bad) {
-      const float fill = bad ? __int_as_float(0x7fffffff) : 0.f;
+  Raw<T, W> x[kHeads], y[kHeads];
+  auto fetch = [&](int h0) {
 #pragma unroll
-      for (int i = 0; i < W; ++i) x[i] = y[i] = fill;
-    } else if (h < a.H + a.G) {
-      item.apply(x, y, a.R);
+    for (int u = 0; u < kHeads; ++u) {
+      const int h = h0 + u * step;
+      if (h >= heads) continue;
+      x[u].load(src0 + (size_t)h * a.D + item.a);
+      if (item.b >= 0) y[u].load(src0 + (size_t)h * a.D + item.b);
     }
-    store_vec<T, W>(dst + item.a, x);
-    if (item.b >= 0) store_vec<T, W>(dst + item.b, y);
+  };
+  int h0 = (int)threadIdx.x / ni;
+  fetch(h0);
+  // The thread that finds the token's sequence looks its place up.  (Starts that decrease could let
+  // several find one; each writes a place that is in range.)
+  __shared__ long long s_pos, s_cache;   // s_pos = -1: no key; s_cache = -1: a page or position out of range
+  __shared__ int s_found;
+  if (threadIdx.x == 0) s_found = 0;
+  __syncthreads();
+  for (int s = threadIdx.x; s < a.seqs; s += blockDim.x) {
+    const int start = a.q_starts[s], end = a.q_starts[s + 1], len = a.kv_lens[s];
+    if (start > n || n >= end) continue;
+    const long long p = (long long)len - end + n;
+    long long cache = -1;
+    if (p >= 0 && p < a.table_rows) {
+      const long long col = p / a.page_size;
+      int page = -1;
+      if (col < a.pages_per_seq) page = a.page_table[(size_t)s * a.page_table_stride + col];
+      if (page >= 0 && page < a.num_pages)
+        cache = (long long)page * a.page_stride + (p - col * a.page_size) * a.slot_stride;
+    }
+    s_pos = p < 0 ? -1 : cache < 0 ? 0 : p;   // in the table whoever wrote s_cache
+    s_cache = cache;
+    s_found = 1;
+  }
+  __syncthreads();
+  if (!s_found) return;   // a row behind the last sequence
+  const bool none = s_pos < 0;   // more rows than keys: no key to write, no row to answer
+  const bool bad = !none && s_cache < 0;
+  const size_t cache = none || bad ? 0 : (size_t)s_cache;
+  const float2* row = (const float2*)a.cos_sin + (none || bad ? 0 : (size_t)s_pos * (a.R / 2));
+  if (bad && threadIdx.x == 0) record_invalid();
+  item.angles(row, bad, 1.f, a.R);
+  for (; h0 < heads; h0 += step * kHeads, fetch(h0)) {
+#pragma unroll
+    for (int u = 0; u < kHeads; ++u) {
+      const int h = h0 + u * step;
+      if (h >= heads || (h >= a.H && (none || bad))) continue;
+      T* dst;
+      if (h < a.H) dst = (T*)a.q + ((size_t)n * a.H + h) * a.D;
+      else if (h < a.H + a.G) dst = (T*)a.k_cache + cache + (size_t)(h - a.H) * a.head_stride;
+      else dst = (T*)a.v_cache + cache + (size_t)(h - a.H - a.G) * a.head_stride;
+      float v[W], w[W];
+      x[u].get(v);
+      y[u].get(w);
+      if (none || bad) {
+        const float fill = bad ? __int_as_float(0x7fffffff) : 0.f;
+#pragma unroll
+        for (int i = 0; i < W; ++i) v[i] = w[i] = fill;
+      } else if (h < a.H + a.G) {
+        item.apply(v, w, a.R);
+      }
+      store_vec<T, W>(dst + item.a, v);
+      if (item.b >= 0) store_vec<T, W>(dst + item.b, w);
+    }
   }
 }
 
-// Elements per vector: the widest of 8, 4, 2, 1 that the layout's pairs divide into (halves start
-// at R/2, so a vector may not straddle it; interleaved pairs lie within a vector).
-int vector_width(int R, int half) {
+// Elements per vector: the widest of 8 (16-bit types), 4, 2, 1 that the layout's pairs divide into (halves
+// start at R/2, so a vector may not straddle it; interleaved pairs lie within a vector).  Eight f32 values
+// and their angles cost registers that four do not (5.1 against 3.9 us on 1731 tokens of 20 heads).
+int vector_width(int R, int half, bool f32) {
   const int m = half ? R / 2 : R;
-  return m % 8 == 0 ? 8 : m % 4 == 0 ? 4 : m % 2 == 0 ? 2 : 1;
+  return m % 8 == 0 && !f32 ? 8 : m % 4 == 0 ? 4 : m % 2 == 0 ? 2 : 1;
 }
 
-// threads per block: whole heads of items, about `want` threads at most
-static unsigned block_threads(int heads, int ni, int want) {
-  int per = want / ni;
-  if (per < 1) per = 1;
-  if (per > heads) per = heads;
-  // the same number of rounds with no more heads at a time than they need
-  const int rounds = (heads + per - 1) / per;
-  per = (heads + rounds - 1) / rounds;
-  return (unsigned)(per * ni);
+// threads per token: whole heads of items, about `want` threads at most, each with `at_once` heads a round, and
+// no more than the rounds need
+static int token_threads(int heads, int ni, int want, int at_once) {
+  int per = std::max(1, std::min(want / ni, (heads + at_once - 1) / at_once));
+  const int rounds = (heads + per * at_once - 1) / (per * at_once);
+  per = (heads + rounds * at_once - 1) / (rounds * at_once);
+  return per * ni;
 }
 
 template <typename T, int W, bool kHalf>
 static cudaError_t qkv_t(const QkvArgs& a, bool back) {
-  const unsigned threads = block_threads(a.H + 2 * a.G, items_per_head(a.D, W), 256);
-  const dim3 grid((unsigned)((long long)a.B * a.T));
-  return back ? launch_pdl(qkv_kernel<T, W, kHalf, true>, grid, dim3(threads), 0, a.stream, a)
-              : launch_pdl(qkv_kernel<T, W, kHalf, false>, grid, dim3(threads), 0, a.stream, a);
+  const int lanes = token_threads(a.H + 2 * a.G, items_per_head(a.D, W), 256, kHeads);
+  const dim3 grid((unsigned)((long long)a.B * a.T)), block((unsigned)lanes);
+  return back ? launch_pdl(qkv_kernel<T, W, kHalf, true>, grid, block, 0, a.stream, a)
+              : launch_pdl(qkv_kernel<T, W, kHalf, false>, grid, block, 0, a.stream, a);
 }
 
 template <typename T, int W, bool kHalf>
 static cudaError_t append_t(const AppendArgs& a) {
-  const unsigned threads = block_threads(a.H + 2 * a.G, items_per_head(a.D, W), 256);
-  return launch_pdl(append_kernel<T, W, kHalf>, dim3((unsigned)a.tokens), dim3(threads), 0, a.stream, a);
+  const int threads = token_threads(a.H + 2 * a.G, items_per_head(a.D, W), 256, kHeads);
+  return launch_pdl(append_kernel<T, W, kHalf>, dim3((unsigned)a.tokens), dim3((unsigned)threads), 0, a.stream, a);
 }
 
 // dispatch on type, layout and vector width; FN<T, W, kHalf>
 #define CA_ROTARY_W(FN, T, HALF, ...)                     \
-  switch (vector_width(a.R, a.half)) {                    \
-    case 8: return FN<T, 8, HALF>(__VA_ARGS__);           \
+  switch (vector_width(a.R, a.half, sizeof(T) == 4)) {    \
+    case 8: return FN<T, sizeof(T) == 4 ? 4 : 8, HALF>(__VA_ARGS__); \
     case 4: return FN<T, 4, HALF>(__VA_ARGS__);           \
     case 2: return FN<T, 2, HALF>(__VA_ARGS__);           \
     default: return FN<T, HALF ? 1 : 2, HALF>(__VA_ARGS__); \

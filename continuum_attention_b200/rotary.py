@@ -132,7 +132,8 @@ class RotaryQKVFunction(torch.autograd.Function):
     def forward(ctx, qkv, cos_sin, positions, heads, kv_heads, layout):
         B, T, width = qkv.shape
         D = width // (heads + 2 * kv_heads)
-        qkv = _aligned(qkv.contiguous())
+        if not qkv.is_contiguous() or qkv.data_ptr() % 16:
+            qkv = _aligned(qkv.contiguous())
         q = torch.empty(B, heads, T, D, dtype=qkv.dtype, device=qkv.device)
         k = torch.empty(B, kv_heads, T, D, dtype=qkv.dtype, device=qkv.device)
         v = torch.empty_like(k)
@@ -145,6 +146,7 @@ class RotaryQKVFunction(torch.autograd.Function):
         _native.check("ca_rotary_qkv_forward", st)
         ctx.save_for_backward(cos_sin, positions)
         ctx.meta = (B, T, heads, kv_heads, D, stride, layout, qkv.dtype)
+        ctx.set_materialize_grads(False)
         return q, k, v
 
     @staticmethod
@@ -153,15 +155,20 @@ class RotaryQKVFunction(torch.autograd.Function):
             raise RuntimeError("rotary_qkv supports first-order gradients only")
         cos_sin, positions = ctx.saved_tensors
         B, T, heads, kv_heads, D, stride, layout, dtype = ctx.meta
-        ref = next(g for g in (dq, dk, dv) if g is not None)
-        grads = [torch.zeros((B, h, T, D), dtype=dtype, device=ref.device) if g is None
-                 else _aligned(g.to(dtype).contiguous()) for g, h in zip((dq, dk, dv), (heads, kv_heads, kv_heads))]
-        dqkv = torch.empty(B, T, (heads + 2 * kv_heads) * D, dtype=dtype, device=ref.device)
-        with on_device(ref.device):
+        device = cos_sin.device
+        grads = []
+        for g, h in ((dq, heads), (dk, kv_heads), (dv, kv_heads)):
+            if g is None:
+                g = torch.zeros((B, h, T, D), dtype=dtype, device=device)
+            elif g.dtype != dtype or not g.is_contiguous() or g.data_ptr() % 16:
+                g = _aligned(g.to(dtype).contiguous())
+            grads.append(g)
+        dqkv = torch.empty(B, T, (heads + 2 * kv_heads) * D, dtype=dtype, device=device)
+        with on_device(device):
             st = _native.lib().ca_rotary_qkv_backward(
                 ctypes_ptr(grads[0]), ctypes_ptr(grads[1]), ctypes_ptr(grads[2]), ctypes_ptr(cos_sin),
                 None if positions is None else ctypes_ptr(positions), stride, ctypes_ptr(dqkv), B, T, heads, kv_heads,
-                D, 2 * cos_sin.shape[1], cos_sin.shape[0], layout, _DTYPE_CODE[dtype], raw_stream(ref.device))
+                D, 2 * cos_sin.shape[1], cos_sin.shape[0], layout, _DTYPE_CODE[dtype], raw_stream(device))
         _native.check("ca_rotary_qkv_backward", st)
         return dqkv, None, None, None, None, None
 
