@@ -52,16 +52,15 @@ inline Plan make_plan(const Args& a) {
   return p;
 }
 
-// bf16 and f16 (ca_paged_mma.cu)
+// bf16 and f16 (ca_paged_mma.cu), f32 (ca_paged_simt.cu)
 size_t mma_workspace_bytes(long long max_q_len, long long H, long long G, long long D);
 int mma_launches(const Args& a);
 cudaError_t mma_forward(const Args& a, int dtype, void* workspace);
 cudaError_t mma_read_status(int* out, bool reset);
-
-// a worker whose unit goes on behind its range: what merge_kernel joins
-struct Meta {
-  int pieces, slot, start, rows, h, rt;
-};
+size_t simt_workspace_bytes(long long max_q_len, long long H, long long G, long long D);
+int simt_launches(const Args& a);
+cudaError_t simt_forward(const Args& a, void* workspace);
+cudaError_t simt_read_status(int* out, bool reset);
 
 // Prefix sums of the sequences' places in shared memory (all threads of the block take part in the
 // constructor), and cursors into the stream of tiles: sequence, key head, row tile, key tile.
@@ -226,6 +225,142 @@ struct Schedule {
     c.nt = unit_tiles(c.rt, c.n * plan.group, c.len - c.n);
   }
 };
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float x, float y);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// two neighbouring outputs
+template <typename T>
+__device__ __forceinline__ void store2(T* p, float x, float y) {
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(p) = make_float2(x, y);
+  else *reinterpret_cast<uint32_t*>(p) = pack2<T>(x, y);
+}
+
+// A score that no exponential feels: what masked keys and the key before key 0 get.  Their segments'
+// moments vanish without a select: the closed form divides by 1e30, and between two of them both
+// exponentials are 0.  (Finite, since infinities would meet as NaN.)
+constexpr float kMasked = -1e30f;
+
+// a worker whose unit goes on behind its range: what merge_kernel joins
+struct Meta {
+  int pieces, slot, start, rows, h, rt;
+};
+
+// Joins the pieces of a cut unit: piece 0 is in this worker's slot, the others are the first pieces of the
+// workers that follow.  A warp takes a row; where rows are fewer than warps, several warps share a row's
+// pieces, each sums its own in order, and then the warps' sums are added in order.
+constexpr int kMergeWarps = 16;
+
+struct Sum {
+  float m = -INFINITY, z = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
+  // adds a piece with maximum m2, mass z2 and row y2.  A piece without a key that the row sees has m = -inf
+  // and no mass, or the NaN of a bad page or length.
+  __device__ __forceinline__ void add(float m2, float z2, float4 y2) {
+    const bool none = m2 == -INFINITY;
+    const float top = fmaxf(m, m2);
+    const float fa = none ? 1.f : exp_rel(m - top), fb = none ? 0.f : exp_rel(m2 - top);
+    z = none ? z + z2 : fmaf(z, fa, z2 * fb);
+    y[0] = fmaf(y[0], fa, none ? 0.f : y2.x * fb);
+    y[1] = fmaf(y[1], fa, none ? 0.f : y2.y * fb);
+    y[2] = fmaf(y[2], fa, none ? 0.f : y2.z * fb);
+    y[3] = fmaf(y[3], fa, none ? 0.f : y2.w * fb);
+    m = top;
+  }
+};
+
+// the pieces of one launch: units of br rows
+struct Pieces {
+  float* o;
+  float2* mz;
+  Meta* meta;
+  int br, workers;
+};
+
+template <typename T, int DP>
+static __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ Args a, int group,
+                                                                 const __grid_constant__ Pieces one,
+                                                                 const __grid_constant__ Pieces two) {
+  pdl_wait();
+  pdl_launch_dependents();
+  const bool second = (int)blockIdx.x >= one.workers;
+  const Pieces& pc = second ? two : one;
+  const float* part_o = pc.o;
+  const float2* part_mz = pc.mz;
+  const int BR = pc.br;
+  constexpr int VL = DP / 32;                        // values per lane: 2 or 4
+  __shared__ float4 sum_y[kMergeWarps][32];
+  __shared__ float2 sum_mz[kMergeWarps];
+  const int w = (int)blockIdx.x - (second ? one.workers : 0);
+  const Meta mt = pc.meta[w];
+  if (mt.pieces == 0) return;
+  const int nrows = min(BR, mt.rows - mt.rt * BR);
+  int share = 1;                                     // warps per row
+  while (share * 2 * nrows <= kMergeWarps && share * 4 <= mt.pieces) share *= 2;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % share;
+  for (int r = warp / share; r < nrows; r += kMergeWarps / share) {
+    Sum acc;
+#pragma unroll 4
+    for (int p = part; p < mt.pieces; p += share) {
+      const long long row = ((long long)(w + p) * 2 + (p == 0 ? mt.slot : 0)) * BR + r;
+      const float2 mz = part_mz[row];
+      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+      if constexpr (VL == 4) {
+        y = *reinterpret_cast<const float4*>(part_o + row * DP + 4 * lane);
+      } else {
+        const float2 t = *reinterpret_cast<const float2*>(part_o + row * DP + 2 * lane);
+        y.x = t.x;
+        y.y = t.y;
+      }
+      acc.add(mz.x, mz.y, y);
+    }
+    if (share > 1) {                                 // then every warp takes this loop once, or not at all
+      sum_y[warp][lane] = make_float4(acc.y[0], acc.y[1], acc.y[2], acc.y[3]);
+      if (lane == 0) sum_mz[warp] = make_float2(acc.m, acc.z);
+      asm volatile("bar.sync 1, %0;" ::"r"(nrows * share * 32) : "memory");
+      if (part > 0) return;
+      for (int q = 1; q < share; ++q) acc.add(sum_mz[warp + q].x, sum_mz[warp + q].y, sum_y[warp + q][lane]);
+    }
+    const float inv = acc.z == 0.f ? 0.f : 1.f / acc.z;   // y is 0 then
+    const int row = mt.rt * BR + r, t = row / group;
+    T* dst = (T*)a.o + ((size_t)(mt.start + t) * a.H + (size_t)mt.h * group + (row - t * group)) * a.D + VL * lane;
+    if (VL * lane < a.D) {
+      store2<T>(dst, acc.y[0] * inv, acc.y[1] * inv);
+      if constexpr (VL == 4) store2<T>(dst + 2, acc.y[2] * inv, acc.y[3] * inv);
+    }
+  }
+}
+
+// workspace of a launch of `per_sm` workers per SM whose units have br rows
+inline size_t up256(size_t x) { return (x + 255) / 256 * 256; }
+
+template <int DP>
+inline size_t pieces_bytes(int br, int per_sm) {
+  const size_t w = (size_t)num_sms_cached() * per_sm;
+  return up256(w * 2 * br * DP * sizeof(float)) + up256(w * 2 * br * sizeof(float2)) + up256(w * sizeof(Meta));
+}
+
+template <int DP>
+inline Pieces carve(char* ws, int br, int per_sm) {
+  const size_t w = (size_t)num_sms_cached() * per_sm;
+  const size_t o = up256(w * 2 * br * DP * sizeof(float)), mz = up256(w * 2 * br * sizeof(float2));
+  return Pieces{(float*)ws, (float2*)(ws + o), (Meta*)(ws + o + mz), br, (int)w};
+}
+
+template <typename T, int DP>
+inline cudaError_t launch_merge(const Args& a, const Plan& plan, const Pieces& one, const Pieces& two) {
+  return launch_pdl(merge_kernel<T, DP>, dim3((unsigned)(one.workers + two.workers)), dim3(kMergeWarps * 32), 0,
+                    a.stream, a, plan.group, one, two);
+}
 
 }  // namespace paged
 }  // namespace ca

@@ -150,24 +150,6 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
 }
 template <>
 __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float x, float y);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
-  const __half2 h = __floats2half2_rn(x, y);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// A score that no exponential feels: what masked keys and the key before key 0 get.  Their segments'
-// moments vanish without a select: the closed form divides by 1e30, and between two of them both
-// exponentials are 0.  (Finite, since infinities would meet as NaN.)
-constexpr float kMasked = -1e30f;
-
 // Weights of one lane's run of one row, as two 16-bit parts.  sv[j] = scaled scores of keys (kc + j, kc + NJ + j),
 // sL that of key kc - 1, m2 the reference maximum in log2 units.  Parts j weigh keys (kc - 1 + j, kc + NJ - 1 + j);
 // first is the pair of place 0, unsplit, but for the mass that ends at key kc - 1, which is the lane's to
@@ -818,91 +800,6 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   if (after_chunks) pdl_wait();
 }
 
-// Joins the pieces of a cut unit: piece 0 is in this worker's slot, the others are the first pieces of the
-// workers that follow.  A warp takes a row; where rows are fewer than warps, several warps share a row's
-// pieces, each sums its own in order, and then the warps' sums are added in order.
-constexpr int kMergeWarps = 16;
-
-struct Sum {
-  float m = -INFINITY, z = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
-  // adds a piece with maximum m2, mass z2 and row y2.  A piece without a key that the row sees has m = -inf
-  // and no mass, or the NaN of a bad page or length.
-  __device__ __forceinline__ void add(float m2, float z2, float4 y2) {
-    const bool none = m2 == -INFINITY;
-    const float top = fmaxf(m, m2);
-    const float fa = none ? 1.f : exp_rel(m - top), fb = none ? 0.f : exp_rel(m2 - top);
-    z = none ? z + z2 : fmaf(z, fa, z2 * fb);
-    y[0] = fmaf(y[0], fa, none ? 0.f : y2.x * fb);
-    y[1] = fmaf(y[1], fa, none ? 0.f : y2.y * fb);
-    y[2] = fmaf(y[2], fa, none ? 0.f : y2.z * fb);
-    y[3] = fmaf(y[3], fa, none ? 0.f : y2.w * fb);
-    m = top;
-  }
-};
-
-// the pieces of one launch: units of br rows
-struct Pieces {
-  float* o;
-  float2* mz;
-  Meta* meta;
-  int br, workers;
-};
-
-template <typename T, int DP>
-__global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ Args a, int group,
-                                                                 const __grid_constant__ Pieces one,
-                                                                 const __grid_constant__ Pieces two) {
-  pdl_wait();
-  pdl_launch_dependents();
-  const bool second = (int)blockIdx.x >= one.workers;
-  const Pieces& pc = second ? two : one;
-  const float* part_o = pc.o;
-  const float2* part_mz = pc.mz;
-  const int BR = pc.br;
-  constexpr int VL = DP / 32;                        // values per lane: 2 or 4
-  __shared__ float4 sum_y[kMergeWarps][32];
-  __shared__ float2 sum_mz[kMergeWarps];
-  const int w = (int)blockIdx.x - (second ? one.workers : 0);
-  const Meta mt = pc.meta[w];
-  if (mt.pieces == 0) return;
-  const int nrows = min(BR, mt.rows - mt.rt * BR);
-  int share = 1;                                     // warps per row
-  while (share * 2 * nrows <= kMergeWarps && share * 4 <= mt.pieces) share *= 2;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % share;
-  for (int r = warp / share; r < nrows; r += kMergeWarps / share) {
-    Sum acc;
-#pragma unroll 4
-    for (int p = part; p < mt.pieces; p += share) {
-      const long long row = ((long long)(w + p) * 2 + (p == 0 ? mt.slot : 0)) * BR + r;
-      const float2 mz = part_mz[row];
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-      if constexpr (VL == 4) {
-        y = *reinterpret_cast<const float4*>(part_o + row * DP + 4 * lane);
-      } else {
-        const float2 t = *reinterpret_cast<const float2*>(part_o + row * DP + 2 * lane);
-        y.x = t.x;
-        y.y = t.y;
-      }
-      acc.add(mz.x, mz.y, y);
-    }
-    if (share > 1) {                                 // then every warp takes this loop once, or not at all
-      sum_y[warp][lane] = make_float4(acc.y[0], acc.y[1], acc.y[2], acc.y[3]);
-      if (lane == 0) sum_mz[warp] = make_float2(acc.m, acc.z);
-      asm volatile("bar.sync 1, %0;" ::"r"(nrows * share * 32) : "memory");
-      if (part > 0) return;
-      for (int q = 1; q < share; ++q) acc.add(sum_mz[warp + q].x, sum_mz[warp + q].y, sum_y[warp + q][lane]);
-    }
-    const float inv = acc.z == 0.f ? 0.f : 1.f / acc.z;   // y is 0 then
-    const int row = mt.rt * BR + r, t = row / group;
-    T* dst = (T*)a.o + ((size_t)(mt.start + t) * a.H + (size_t)mt.h * group + (row - t * group)) * a.D + VL * lane;
-    if (VL * lane < a.D) {
-      const uint32_t u = pack2<T>(acc.y[0] * inv, acc.y[1] * inv);
-      if constexpr (VL == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(u, pack2<T>(acc.y[2] * inv, acc.y[3] * inv));
-      else *reinterpret_cast<uint32_t*>(dst) = u;
-    }
-  }
-}
-
 }  // namespace
 
 // ------------------------------------------------------------------ host side
@@ -915,21 +812,6 @@ template <int DP> using Decode16 = std::conditional_t<DP == 64, Config<64, 32, 1
 template <int DP> using Chunk = Config<DP, DP == 64 ? 64 : 32, 16, 4, 3, 3, 152, 56>;
 
 constexpr int kDecodeUnitCost = 2, kChunkUnitCost = 2;
-
-size_t up256(size_t x) { return (x + 255) / 256 * 256; }
-
-template <typename C>
-size_t pieces_bytes() {
-  const size_t w = (size_t)num_sms_cached() * C::GROUPS;
-  return up256(w * 2 * C::BR * C::DP * sizeof(float)) + up256(w * 2 * C::BR * sizeof(float2)) + up256(w * sizeof(Meta));
-}
-
-template <typename C>
-Pieces carve(char* ws) {
-  const size_t w = (size_t)num_sms_cached() * C::GROUPS;
-  const size_t o = up256(w * 2 * C::BR * C::DP * sizeof(float)), mz = up256(w * 2 * C::BR * sizeof(float2));
-  return Pieces{(float*)ws, (float2*)(ws + o), (Meta*)(ws + o + mz), C::BR, (int)w};
-}
 
 template <typename T, typename C>
 cudaError_t launch_main(const Args& a, Plan plan, const Pieces& pc, bool after_chunks) {
@@ -951,12 +833,6 @@ cudaError_t launch_main(const Args& a, Plan plan, const Pieces& pc, bool after_c
 }
 
 template <typename T, int DP>
-cudaError_t launch_merge(const Args& a, const Plan& plan, const Pieces& one, const Pieces& two) {
-  return launch_pdl(merge_kernel<T, DP>, dim3((unsigned)(one.workers + two.workers)), dim3(kMergeWarps * 32), 0,
-                    a.stream, a, plan.group, one, two);
-}
-
-template <typename T, int DP>
 cudaError_t forward_dp(const Args& a, void* workspace) {
   Plan plan = make_plan(a);
   char* ws = (char*)workspace;
@@ -964,7 +840,7 @@ cudaError_t forward_dp(const Args& a, void* workspace) {
   plan.unit_cost = kDecodeUnitCost;
   if (rows <= 16) {
     // every sequence, whatever its rows: max_q_len may be wrong
-    const Pieces pc = rows <= 8 ? carve<Decode8<DP>>(ws) : carve<Decode16<DP>>(ws);
+    const Pieces pc = rows <= 8 ? carve<DP>(ws, Decode8<DP>::BR, Decode8<DP>::GROUPS) : carve<DP>(ws, Decode16<DP>::BR, Decode16<DP>::GROUPS);
     cudaError_t e = rows <= 8 ? launch_main<T, Decode8<DP>>(a, plan, pc, false)
                               : launch_main<T, Decode16<DP>>(a, plan, pc, false);
     return e != cudaSuccess ? e : launch_merge<T, DP>(a, plan, pc, Pieces{});
@@ -976,12 +852,12 @@ cudaError_t forward_dp(const Args& a, void* workspace) {
   chunks.row_lo = 17;
   // (a single sequence is all in one form, whatever its rows)
   if (a.seqs == 1) chunks.row_lo = 0;
-  const Pieces pc = carve<Chunk<DP>>(ws);
+  const Pieces pc = carve<DP>(ws, Chunk<DP>::BR, Chunk<DP>::GROUPS);
   cudaError_t e = launch_main<T, Chunk<DP>>(a, chunks, pc, false);
   if (e != cudaSuccess) return e;
   if (a.seqs == 1) return launch_merge<T, DP>(a, plan, pc, Pieces{});
   plan.row_hi = 16;
-  const Pieces few = carve<Decode16<DP>>(ws + pieces_bytes<Chunk<DP>>());
+  const Pieces few = carve<DP>(ws + pieces_bytes<DP>(Chunk<DP>::BR, Chunk<DP>::GROUPS), Decode16<DP>::BR, Decode16<DP>::GROUPS);
   e = launch_main<T, Decode16<DP>>(a, plan, few, true);
   return e != cudaSuccess ? e : launch_merge<T, DP>(a, plan, pc, few);
 }
@@ -994,7 +870,10 @@ size_t mma_workspace_bytes(long long max_q_len, long long H, long long G, long l
     using D8 = decltype(d8);
     using D16 = decltype(d16);
     using Ck = decltype(chunk);
-    return rows <= 8 ? pieces_bytes<D8>() : rows <= 16 ? pieces_bytes<D16>() : pieces_bytes<Ck>() + pieces_bytes<D16>();
+    constexpr int DP = D8::DP;
+    const size_t few = pieces_bytes<DP>(D16::BR, D16::GROUPS);
+    return rows <= 8 ? pieces_bytes<DP>(D8::BR, D8::GROUPS)
+                     : rows <= 16 ? few : pieces_bytes<DP>(Ck::BR, Ck::GROUPS) + few;
   };
   return D <= 64 ? bytes(Decode8<64>{}, Decode16<64>{}, Chunk<64>{}) : bytes(Decode8<128>{}, Decode16<128>{}, Chunk<128>{});
 }

@@ -1,0 +1,461 @@
+// ca_paged_simt.cu -- Continuum Attention over a paged cache in f32, on the FMA pipes.
+//
+// Work is divided as in ca_paged_mma.cu (units, places, pieces, merge); a worker is a block.
+// A tile of TK keys is three steps between barriers: scores S = Q K^T in register tiles, the
+// rows' moments (a few threads per row, consecutive keys each), O += P V in register tiles.
+// Tiles arrive by cp.async, one ahead, gathered row by row through the page table, V one
+// row early so that the weights of keys a-1 .. a+TK-2 meet it where they lie.
+//
+// What bounds it: decoding reads 2 D f32 values a key and key head, at most 16 rows' FMAs
+// for them; chunks are bound by the FMA pipe and the shared-memory reads that feed it
+// (scores: 6 16-byte reads for 32 FMAs of a thread; P V: 8 for 64).
+#include "ca_paged.cuh"
+
+namespace ca {
+namespace paged {
+
+namespace {
+
+__device__ float4 g_nan16 = {__builtin_nanf(""), __builtin_nanf(""), __builtin_nanf(""), __builtin_nanf("")};
+
+__device__ __forceinline__ void cp_async16(float* dst, const float* src, bool zero) {
+  const uint32_t d = (uint32_t)__cvta_generic_to_shared(dst);
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(zero ? 0 : 16) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// DP padded head values; BR rows of a unit; threads in TR x TC: scores are RT rows x KT keys a thread (row
+// tr + TR i, key tc + TC j), outputs RT rows x DP/TC neighbouring columns
+template <int DP_, int BR_, int TR_, int TC_, int PER_SM_>
+struct Config {
+  static constexpr int DP = DP_, BR = BR_, TR = TR_, TC = TC_, PER_SM = PER_SM_, TK = 32;
+  static constexpr int NT = TR * TC, RT = BR / TR, KT = TK / TC, CT = DP / TC;
+  static constexpr int TPR = NT / BR, KPT = TK / TPR;   // the moments: threads per row, keys per thread
+  static constexpr int LD = DP + 4, LS = TK + 4;        // rows of tiles and of scores, on 16 bytes
+  static constexpr int TILE = (TK + 1) * LD;            // floats; row TK is the halo
+  static constexpr int FLOATS = 4 * TILE + BR * LD + BR * LS + 4 * BR;
+  static constexpr int SMEM = FLOATS * 4 + 3 * (TK + 1) * 8;   // and the prefix sums behind it
+  static_assert(TPR >= 1 && 32 % TPR == 0 && KPT % 4 == 0 && CT % 4 == 0, "");
+};
+
+struct Tile {      // what the block knows of a tile (the same in all threads)
+  int kt, nt, start, n, len, h, rt, bad;
+  bool first, last, end;
+};
+
+template <typename C>
+__global__ void __launch_bounds__(C::NT, C::PER_SM)
+    simt_kernel(const __grid_constant__ Args a, const __grid_constant__ Plan plan, float* __restrict__ part_o,
+                float2* __restrict__ part_mz, Meta* __restrict__ meta) {
+  extern __shared__ __align__(16) uint8_t smem[];
+  pdl_wait();
+  pdl_launch_dependents();
+  constexpr int TK = C::TK, DP = C::DP, BR = C::BR, LD = C::LD, LS = C::LS, RT = C::RT, KT = C::KT, CT = C::CT;
+  float* kv = reinterpret_cast<float*>(smem);            // stages: K, V, K, V
+  float* sq = kv + 4 * C::TILE;                          // Q [BR][LD]
+  float* ss = sq + BR * LD;                              // S, then P [BR][LS]
+  float* row_f = ss + BR * LS;                           // per row: factor on O, then weight of the last key
+  float* row_m = row_f + BR;
+  float* row_z = row_m + BR;
+  long long* offs = reinterpret_cast<long long*>(smem + C::FLOATS * 4);   // [3][TK + 1]: rows a-1 .. a+TK-1
+  unsigned* prefix = reinterpret_cast<unsigned*>(smem + C::SMEM);
+  const int tid = threadIdx.x, tr = tid / C::TC, tc = tid % C::TC;
+
+  Schedule<BR, TK> sched(a, plan, prefix);
+  const unsigned total = sched.total;
+  const int worker = blockIdx.x;
+  const unsigned per = plan.places_per_worker(total, gridDim.x);
+  const unsigned x0 = (unsigned)min((unsigned long long)worker * per, (unsigned long long)total);
+  const unsigned x1 = (unsigned)min((unsigned long long)x0 + per, (unsigned long long)total);
+  typename Schedule<BR, TK>::Cursor cur;
+  cur.at = x1;
+  if (x0 < x1) cur = sched.locate(x0);
+  if (cur.at >= x1) {
+    if (tid == 0) meta[worker].pieces = 0;
+    return;
+  }
+
+  // the next tile of the stream, and its rows' offsets in the cache (-1: none, -2: a bad page)
+  int ring = 0;
+  bool more = true, opening = true;
+  unsigned at = 0;
+  auto describe = [&](Tile& t) {
+    const int base = cur.kt * TK;
+    for (int r = tid; r <= TK; r += C::NT) {
+      const int key = base - 1 + r;
+      long long off = -1;
+      if (key >= 0 && key < cur.len) {
+        const int col = plan.page_of(key);
+        const int page = a.page_table[(size_t)cur.s * a.page_table_stride + col];
+        if (page < 0 || page >= a.num_pages) {
+          off = -2;
+          record_invalid();
+        } else {
+          off = (long long)page * a.page_stride + (long long)cur.h * a.head_stride +
+                (long long)(key - col * a.page_size) * a.slot_stride;
+        }
+      }
+      offs[ring * (TK + 1) + r] = off;
+    }
+    at = cur.at;
+    more = cur.at + 1 < x1;
+    t.kt = cur.kt;
+    t.nt = cur.nt;
+    t.start = cur.start;
+    t.n = cur.n;
+    t.len = cur.len;
+    t.h = cur.h;
+    t.rt = cur.rt;
+    t.bad = cur.bad;
+    t.first = opening || cur.kt == 0;
+    t.last = !more || cur.kt + 1 == cur.nt;
+    opening = false;
+    if (more) {
+      sched.advance(cur);
+      more = cur.at < x1;
+    }
+    t.end = !more;
+  };
+  auto copy = [&](const Tile& t, int stage, int slot) {
+    const long long* of = offs + slot * (TK + 1);
+    float* kd = kv + stage * 2 * C::TILE;
+    float* vd = kd + C::TILE;
+    constexpr int C4 = DP / 4;
+    const float* kc = (const float*)a.k_cache;
+    const float* vc = (const float*)a.v_cache;
+    for (int x = tid; x < (TK + 1) * C4; x += C::NT) {
+      const int r = x / C4, c = (x - r * C4) * 4;
+      const bool pad = c >= a.D;
+      // K row r is key a + r, the halo (row TK) key a - 1; V row r is key a - 1 + r
+      const long long ok = of[r < TK ? r + 1 : 0], ov = of[r];
+      const float* nan = reinterpret_cast<const float*>(&g_nan16);
+      cp_async16(kd + r * LD + c, ok < -1 ? nan : kc + (ok < 0 ? 0 : ok + c), ok == -1 || pad);
+      cp_async16(vd + r * LD + c, ov < -1 ? nan : vc + (ov < 0 ? 0 : ov + c), ov == -1 || pad);
+    }
+  };
+
+  // a row's moments: threads [row][part] in one warp
+  const int mrow = tid / C::TPR, mpart = tid % C::TPR;
+  float m = -INFINITY, z = 0.f, carry_s = kMasked, carry_b = 0.f, scale = 0.f;
+  int pos = -1, kt0 = 0;
+  bool in_first = true, first_piece = true;
+  float o[RT][CT];
+
+  Tile cur_t, next_t;
+  describe(cur_t);
+  __syncthreads();
+  copy(cur_t, 0, 0);
+  cp_commit();
+  int stage = 0, slot = 0;
+  unsigned at_now = at;
+  while (true) {
+    const Tile t = cur_t;
+    const unsigned at_t = at_now;
+    ring = slot == 2 ? 0 : slot + 1;
+    if (!t.end) {
+      describe(next_t);
+      at_now = at;
+    }
+    const int base = t.kt * TK, rows = t.n * plan.group, row0 = t.rt * BR;
+    if (t.first) {
+      kt0 = t.kt;
+      in_first = first_piece;
+      first_piece = false;
+      for (int x = tid; x < BR * (DP / 4); x += C::NT) {
+        const int r = x / (DP / 4), c = (x % (DP / 4)) * 4, row = row0 + r;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (row < rows && c < a.D) {
+          const int tk = row / plan.group;
+          v = *reinterpret_cast<const float4*>((const float*)a.q + (size_t)(t.start + tk) * a.q_token_stride +
+                                               (size_t)(t.h * plan.group + row - tk * plan.group) * a.q_head_stride + c);
+        }
+        *reinterpret_cast<float4*>(sq + r * LD + c) = v;
+      }
+      const int row = row0 + mrow;
+      pos = -1;
+      scale = 0.f;
+      if (row < rows) {
+        const int tk = row / plan.group;
+        pos = t.len - t.n + tk;
+        scale = expf(a.log_gain[t.h * plan.group + row - tk * plan.group]) * a.inv_sqrt_d;
+      }
+      m = -INFINITY;
+      z = 0.f;
+      carry_s = kMasked;
+      carry_b = 0.f;
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int c = 0; c < CT; ++c) o[i][c] = 0.f;
+    }
+    cp_wait<0>();
+    __syncthreads();                 // this tile, Q and the next tile's offsets are there
+    if (!t.end) copy(next_t, stage ^ 1, ring);
+    cp_commit();
+    const float* ks = kv + stage * 2 * C::TILE;
+    const float* vs = ks + C::TILE;
+
+    {
+      // scores: even and odd positions of the head in the two halves of packed FMAs
+      float2 acc[RT][KT];
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < KT; ++j) acc[i][j] = splat2(0.f);
+#pragma unroll 4
+      for (int d = 0; d < DP; d += 4) {
+        float4 q[RT], k[KT];
+#pragma unroll
+        for (int i = 0; i < RT; ++i) q[i] = *reinterpret_cast<const float4*>(sq + (tr + C::TR * i) * LD + d);
+#pragma unroll
+        for (int j = 0; j < KT; ++j) k[j] = *reinterpret_cast<const float4*>(ks + (tc + C::TC * j) * LD + d);
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+          for (int j = 0; j < KT; ++j) {
+            acc[i][j] = fma2(make_float2(q[i].x, q[i].y), make_float2(k[j].x, k[j].y), acc[i][j]);
+            acc[i][j] = fma2(make_float2(q[i].z, q[i].w), make_float2(k[j].z, k[j].w), acc[i][j]);
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < KT; ++j) ss[(tr + C::TR * i) * LS + tc + C::TC * j] = acc[i][j].x + acc[i][j].y;
+    }
+    if (t.first && t.kt > 0) {
+      // the score that the first segment starts from, by the row's threads
+      float s = 0.f;
+      for (int d = 4 * mpart; d < DP; d += 4 * C::TPR) {
+        const float4 q = *reinterpret_cast<const float4*>(sq + mrow * LD + d);
+        const float4 k = *reinterpret_cast<const float4*>(ks + TK * LD + d);
+        s = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, s))));
+      }
+#pragma unroll
+      for (int off = C::TPR / 2; off; off >>= 1) s += __shfl_xor_sync(0xffffffffu, s, off);
+      if (base - 1 <= pos) m = carry_s = s * scale;
+    }
+    __syncthreads();
+
+    {
+      // the row's weights
+      float* sr = ss + mrow * LS + mpart * C::KPT;
+      const int kc = base + mpart * C::KPT;
+      float s[C::KPT];
+      float top = kMasked;
+#pragma unroll
+      for (int x = 0; x < C::KPT; x += 4) {
+        const float4 v = *reinterpret_cast<const float4*>(sr + x);
+        s[x] = v.x;
+        s[x + 1] = v.y;
+        s[x + 2] = v.z;
+        s[x + 3] = v.w;
+      }
+#pragma unroll
+      for (int x = 0; x < C::KPT; ++x) {
+        s[x] = kc + x <= pos ? s[x] * scale : kMasked;
+        top = fmaxf(top, s[x]);
+      }
+#pragma unroll
+      for (int off = C::TPR / 2; off; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+      float f = 1.f;
+      if (top > kMasked && top > m) {
+        f = exp_rel(m - top);
+        m = top;
+        z *= f;
+        carry_b *= f;
+      }
+      const float mm = m == -INFINITY ? 0.f : m;
+      float got = __shfl_up_sync(0xffffffffu, s[C::KPT - 1], 1, C::TPR);
+      float sa = mpart == 0 ? carry_s : got;
+      float ea = exp_rel(sa - mm), right = 0.f, p[C::KPT];
+      const int lowest = t.first ? base : base - 1;      // key `pos` has its cap here from this key on
+#pragma unroll
+      for (int x = 0; x < C::KPT; ++x) {
+        const float eb = exp_rel(s[x] - mm);
+        float M0, M1;
+        seg_moments01(ea, eb, s[x] - sa, M0, M1);
+        z += M0;
+        p[x] = right + (M0 - M1);
+        const int key = kc + x - 1;                      // the key this weight belongs to
+        if (key == 0 && pos >= 0) {
+          p[x] = fmaf(0.5f, ea, p[x]);
+          z = fmaf(0.5f, ea, z);
+        }
+        if (key == pos && key >= lowest) {
+          p[x] = fmaf(0.5f, ea, p[x]);
+          z = fmaf(0.5f, ea, z);
+        }
+        right = M1;
+        sa = s[x];
+        ea = eb;
+      }
+      got = __shfl_up_sync(0xffffffffu, right, 1, C::TPR);
+      p[0] += mpart == 0 ? carry_b : got;
+      carry_s = __shfl_sync(0xffffffffu, sa, C::TPR - 1, C::TPR);
+      carry_b = __shfl_sync(0xffffffffu, right, C::TPR - 1, C::TPR);
+#pragma unroll
+      for (int x = 0; x < C::KPT; x += 4)
+        *reinterpret_cast<float4*>(sr + x) = make_float4(p[x], p[x + 1], p[x + 2], p[x + 3]);
+      if (mpart == 0) row_f[mrow] = f;
+    }
+    __syncthreads();
+
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const float f = row_f[tr + C::TR * i];
+#pragma unroll
+      for (int c = 0; c < CT; ++c) o[i][c] *= f;
+    }
+#pragma unroll 2
+    for (int k = 0; k < TK; k += 4) {
+      float4 p[RT];
+#pragma unroll
+      for (int i = 0; i < RT; ++i) p[i] = *reinterpret_cast<const float4*>(ss + (tr + C::TR * i) * LS + k);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+#pragma unroll
+        for (int c = 0; c < CT; c += 4) {
+          const float4 v = *reinterpret_cast<const float4*>(vs + (k + u) * LD + tc * CT + c);
+#pragma unroll
+          for (int i = 0; i < RT; ++i) {
+            const float w = u == 0 ? p[i].x : u == 1 ? p[i].y : u == 2 ? p[i].z : p[i].w;
+            float2 lo = make_float2(o[i][c], o[i][c + 1]), hi = make_float2(o[i][c + 2], o[i][c + 3]);
+            lo = fma2(splat2(w), make_float2(v.x, v.y), lo);
+            hi = fma2(splat2(w), make_float2(v.z, v.w), hi);
+            o[i][c] = lo.x;
+            o[i][c + 1] = lo.y;
+            o[i][c + 2] = hi.x;
+            o[i][c + 3] = hi.y;
+          }
+        }
+      }
+    }
+
+    if (t.last) {
+      const bool whole = kt0 == 0 && t.kt + 1 == t.nt;
+      const int key = base + TK - 1;                     // the key whose weight is still carried
+      const long long slot_row = ((long long)worker * 2 + (in_first ? 0 : 1)) * BR;
+      const float mm = m == -INFINITY ? 0.f : m;
+      const float cap = key == pos ? 0.5f * exp_rel(carry_s - mm) : 0.f;
+      float zz = z;
+#pragma unroll
+      for (int off = C::TPR / 2; off; off >>= 1) zz += __shfl_xor_sync(0xffffffffu, zz, off);
+      zz += cap;
+      if (t.bad) zz = __int_as_float(0x7fffffff);
+      __syncthreads();                                   // row_f has been read
+      if (mpart == 0) {
+        // a key beyond the row's own has no weight, and its V may hold anything
+        row_f[mrow] = key <= pos ? carry_b + cap : 0.f;
+        row_m[mrow] = m;
+        row_z[mrow] = zz;
+        if (!whole && row0 + mrow < rows) part_mz[slot_row + mrow] = make_float2(m, zz);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const int r = tr + C::TR * i, row = row0 + r;
+        if (row >= rows) continue;
+        const float w = row_f[r], zr = row_z[r], inv = 1.f / zr;
+        const int tk = row / plan.group;
+        float* dst = (float*)a.o +
+                     ((size_t)(t.start + tk) * a.H + (size_t)t.h * plan.group + (row - tk * plan.group)) * a.D;
+#pragma unroll
+        for (int c = 0; c < CT; c += 4) {
+          const int col = tc * CT + c;
+          float4 y = make_float4(o[i][c], o[i][c + 1], o[i][c + 2], o[i][c + 3]);
+          if (w != 0.f) {
+            const float4 v = *reinterpret_cast<const float4*>(vs + TK * LD + col);
+            y = make_float4(fmaf(w, v.x, y.x), fmaf(w, v.y, y.y), fmaf(w, v.z, y.z), fmaf(w, v.w, y.w));
+          }
+          if (!whole) {
+            *reinterpret_cast<float4*>(part_o + (slot_row + r) * DP + col) = y;
+          } else if (col < a.D) {
+            // z = 0: the row sees no key
+            *reinterpret_cast<float4*>(dst + col) =
+                zr == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+          }
+        }
+      }
+      if (t.end && tid == 0) {
+        // this worker joins the unit that starts in its range and goes on behind it
+        Meta mt;
+        mt.pieces = kt0 == 0 && t.kt + 1 < t.nt ? 1 + (int)((at_t + (t.nt - 1 - t.kt)) / per) - worker : 0;
+        mt.slot = in_first ? 0 : 1;
+        mt.start = t.start;
+        mt.rows = rows;
+        mt.h = t.h;
+        mt.rt = t.rt;
+        meta[worker] = mt;
+      }
+    }
+    if (t.end) break;
+    __syncthreads();                 // scores, Q and this tile's stage are free
+    cur_t = next_t;
+    stage ^= 1;
+    slot = ring;
+  }
+  cp_wait<0>();
+}
+
+// rows of a unit: 16 for decoding, 64 for chunks
+template <int DP> using Few = Config<DP, 16, 16, 8, DP == 64 ? 5 : 2>;
+template <int DP> using Many = Config<DP, 64, 16, 16, DP == 64 ? 2 : 1>;
+constexpr int kUnitCost = 1;
+
+template <typename C>
+cudaError_t launch_main(const Args& a, const Plan& plan, const Pieces& pc) {
+  // (with the prefix sums of 200 sequences; with more, fewer blocks run at once)
+  static_assert((C::SMEM + 200 * 4 + 1024) * C::PER_SM <= 233472, "shared memory of an SM");
+  const size_t smem = C::SMEM + (size_t)(a.seqs + 1) * sizeof(unsigned);
+  static thread_local int set_dev = -1;    // the attribute belongs to the device
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (set_dev != dev) {
+    e = cudaFuncSetAttribute(simt_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             C::SMEM + (kMaxSeqs + 1) * (int)sizeof(unsigned));
+    if (e != cudaSuccess) return e;
+    set_dev = dev;
+  }
+  return launch_pdl(simt_kernel<C>, dim3((unsigned)pc.workers), dim3(C::NT), smem, a.stream, a, plan, pc.o, pc.mz,
+                    pc.meta);
+}
+
+template <int DP>
+cudaError_t forward_dp(const Args& a, void* workspace) {
+  Plan plan = make_plan(a);
+  plan.unit_cost = kUnitCost;
+  char* ws = (char*)workspace;
+  // every sequence in the form that suits the longest: 64-row units leave threads of a short one idle, but
+  // in 32 bits the loads and FMAs of a tile are the same whatever its rows
+  const bool few = (long long)a.max_q_len * plan.group <= 16;
+  const Pieces pc = few ? carve<DP>(ws, Few<DP>::BR, Few<DP>::PER_SM) : carve<DP>(ws, Many<DP>::BR, Many<DP>::PER_SM);
+  cudaError_t e = few ? launch_main<Few<DP>>(a, plan, pc) : launch_main<Many<DP>>(a, plan, pc);
+  return e != cudaSuccess ? e : launch_merge<float, DP>(a, plan, pc, Pieces{});
+}
+
+}  // namespace
+
+size_t simt_workspace_bytes(long long max_q_len, long long H, long long G, long long D) {
+  const bool few = max_q_len * (H / G) <= 16;
+  if (D <= 64) return few ? pieces_bytes<64>(Few<64>::BR, Few<64>::PER_SM) : pieces_bytes<64>(Many<64>::BR, Many<64>::PER_SM);
+  return few ? pieces_bytes<128>(Few<128>::BR, Few<128>::PER_SM) : pieces_bytes<128>(Many<128>::BR, Many<128>::PER_SM);
+}
+
+int simt_launches(const Args&) { return 2; }
+
+cudaError_t simt_forward(const Args& a, void* workspace) {
+  return a.D <= 64 ? forward_dp<64>(a, workspace) : forward_dp<128>(a, workspace);
+}
+
+cudaError_t simt_read_status(int* out, bool reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(out, g_status, sizeof(int));
+  if (e != cudaSuccess || !reset || *out == 0) return e;
+  const int zero = 0;
+  return cudaMemcpyToSymbol(g_status, &zero, sizeof(int));
+}
+
+}  // namespace paged
+}  // namespace ca
