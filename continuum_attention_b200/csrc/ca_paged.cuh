@@ -307,29 +307,17 @@ static __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __
   int share = 1;                                     // warps per row
   while (share * 2 * nrows <= kMergeWarps && share * 4 <= mt.pieces) share *= 2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % share;
-  for (int r = warp / share; r < nrows; r += kMergeWarps / share) {
-    Sum acc;
-#pragma unroll 4
-    for (int p = part; p < mt.pieces; p += share) {
-      const long long row = ((long long)(w + p) * 2 + (p == 0 ? mt.slot : 0)) * BR + r;
-      const float2 mz = part_mz[row];
-      float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-      if constexpr (VL == 4) {
-        y = *reinterpret_cast<const float4*>(part_o + row * DP + 4 * lane);
-      } else {
-        const float2 t = *reinterpret_cast<const float2*>(part_o + row * DP + 2 * lane);
-        y.x = t.x;
-        y.y = t.y;
-      }
-      acc.add(mz.x, mz.y, y);
+  auto load = [&](int p, int r, float2& mz, float4& y) {
+    const long long row = ((long long)(w + p) * 2 + (p == 0 ? mt.slot : 0)) * BR + r;
+    mz = part_mz[row];
+    if constexpr (VL == 4) {
+      y = *reinterpret_cast<const float4*>(part_o + row * DP + 4 * lane);
+    } else {
+      const float2 t = *reinterpret_cast<const float2*>(part_o + row * DP + 2 * lane);
+      y = make_float4(t.x, t.y, 0.f, 0.f);
     }
-    if (share > 1) {                                 // then every warp takes this loop once, or not at all
-      sum_y[warp][lane] = make_float4(acc.y[0], acc.y[1], acc.y[2], acc.y[3]);
-      if (lane == 0) sum_mz[warp] = make_float2(acc.m, acc.z);
-      asm volatile("bar.sync 1, %0;" ::"r"(nrows * share * 32) : "memory");
-      if (part > 0) return;
-      for (int q = 1; q < share; ++q) acc.add(sum_mz[warp + q].x, sum_mz[warp + q].y, sum_y[warp + q][lane]);
-    }
+  };
+  auto store = [&](const Sum& acc, int r) {
     const float inv = acc.z == 0.f ? 0.f : 1.f / acc.z;   // y is 0 then
     const int row = mt.rt * BR + r, t = row / group;
     T* dst = (T*)a.o + ((size_t)(mt.start + t) * a.H + (size_t)mt.h * group + (row - t * group)) * a.D + VL * lane;
@@ -337,7 +325,44 @@ static __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __
       store2<T>(dst, acc.y[0] * inv, acc.y[1] * inv);
       if constexpr (VL == 4) store2<T>(dst + 2, acc.y[2] * inv, acc.y[3] * inv);
     }
+  };
+  if (share == 1) {
+    // four rows of a warp side by side: one after the other each would wait for its own loads
+    for (int r0 = warp; r0 < nrows; r0 += 4 * kMergeWarps) {
+      Sum acc[4];
+#pragma unroll 2
+      for (int p = 0; p < mt.pieces; ++p) {
+        float2 mz[4];
+        float4 y[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (r0 + u * kMergeWarps < nrows) load(p, r0 + u * kMergeWarps, mz[u], y[u]);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (r0 + u * kMergeWarps < nrows) acc[u].add(mz[u].x, mz[u].y, y[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (r0 + u * kMergeWarps < nrows) store(acc[u], r0 + u * kMergeWarps);
+    }
+    return;
   }
+  const int r = warp / share;                        // nrows * share <= kMergeWarps
+  if (r >= nrows) return;
+  Sum acc;
+#pragma unroll 4
+  for (int p = part; p < mt.pieces; p += share) {
+    float2 mz;
+    float4 y;
+    load(p, r, mz, y);
+    acc.add(mz.x, mz.y, y);
+  }
+  sum_y[warp][lane] = make_float4(acc.y[0], acc.y[1], acc.y[2], acc.y[3]);
+  if (lane == 0) sum_mz[warp] = make_float2(acc.m, acc.z);
+  asm volatile("bar.sync 1, %0;" ::"r"(nrows * share * 32) : "memory");
+  if (part > 0) return;
+  for (int q = 1; q < share; ++q) acc.add(sum_mz[warp + q].x, sum_mz[warp + q].y, sum_y[warp + q][lane]);
+  store(acc, r);
 }
 
 // workspace of a launch of `per_sm` workers per SM whose units have br rows

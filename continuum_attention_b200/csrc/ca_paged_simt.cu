@@ -269,28 +269,33 @@ __global__ void __launch_bounds__(C::NT, C::PER_SM)
       const float mm = m == -INFINITY ? 0.f : m;
       float got = __shfl_up_sync(0xffffffffu, s[C::KPT - 1], 1, C::TPR);
       float sa = mpart == 0 ? carry_s : got;
-      float ea = exp_rel(sa - mm), right = 0.f, p[C::KPT];
+      float ea = exp_rel(sa - mm), right = 0.f, p[C::KPT], eb[C::KPT], M0[C::KPT], M1[C::KPT];
       const int lowest = t.first ? base : base - 1;      // key `pos` has its cap here from this key on
+      // both forms of each moment, selected: a branch would run both for a warp anyway, key after key
+#pragma unroll
+      for (int x = 0; x < C::KPT; ++x) eb[x] = exp_rel(s[x] - mm);
 #pragma unroll
       for (int x = 0; x < C::KPT; ++x) {
-        const float eb = exp_rel(s[x] - mm);
-        float M0, M1;
-        seg_moments01(ea, eb, s[x] - sa, M0, M1);
-        z += M0;
-        p[x] = right + (M0 - M1);
-        const int key = kc + x - 1;                      // the key this weight belongs to
-        if (key == 0 && pos >= 0) {
-          p[x] = fmaf(0.5f, ea, p[x]);
-          z = fmaf(0.5f, ea, z);
-        }
-        if (key == pos && key >= lowest) {
-          p[x] = fmaf(0.5f, ea, p[x]);
-          z = fmaf(0.5f, ea, z);
-        }
-        right = M1;
-        sa = s[x];
-        ea = eb;
+        const float a0 = x ? eb[x - 1] : ea, d = s[x] - (x ? s[x - 1] : sa);
+        const float r = rcp_approx(d);
+        const float m0 = (eb[x] - a0) * r, near = a0 * series_j1(d);
+        const bool use = fabsf(d) < kSeriesMax;
+        M1[x] = use ? near : (eb[x] - m0) * r;
+        M0[x] = use ? fmaf(-d, near, eb[x]) : m0;
       }
+#pragma unroll
+      for (int x = 0; x < C::KPT; ++x) {
+        z += M0[x];
+        p[x] = right + (M0[x] - M1[x]);
+        const int key = kc + x - 1;                      // the key this weight belongs to
+        const float half = (key == 0 && pos >= 0 ? 0.5f : 0.f) + (key == pos && key >= lowest ? 0.5f : 0.f);
+        if (half > 0.f) {
+          p[x] = fmaf(half, x ? eb[x - 1] : ea, p[x]);
+          z = fmaf(half, x ? eb[x - 1] : ea, z);
+        }
+        right = M1[x];
+      }
+      sa = s[C::KPT - 1];
       got = __shfl_up_sync(0xffffffffu, right, 1, C::TPR);
       p[0] += mpart == 0 ? carry_b : got;
       carry_s = __shfl_sync(0xffffffffu, sa, C::TPR - 1, C::TPR);
