@@ -13,6 +13,13 @@ pass a CPU stand-in with the same signature.  On CUDA the attention block's
 input side is one native kernel (``rope.rope_qkv``: QKV unpacking fused with the
 rotary embedding), the attention output is stored in the projection's input
 order, and each norm is one native kernel forward (``rmsnorm``).
+
+Answering (no reference counterpart: the reference trains and evaluates only):
+``forward_paged`` runs new tokens of several sequences against a ``PagedKVCache``
+(``rotary.rotary_append`` into the cache, ``paged.continuum_attention_paged`` over it),
+``generate`` continues prompts with it, one token of every sequence per CUDA-graph
+replay.  The ``rope_*`` options beyond theta select the general rotary positions
+(``rotary``): layout, part of the head, stretched contexts.
 """
 from __future__ import annotations
 
@@ -30,7 +37,9 @@ from .gelu import supported as gelu_supported
 from .rmsnorm import add_rms_norm, add_supported
 from .rmsnorm import rms_norm as native_rms_norm
 from .rmsnorm import supported as native_rms_norm_supported
-from .rope import apply_rope_torch, rope_qkv
+from .paged import PagedKVCache, PagedStep, continuum_attention_paged
+from .rope import apply_rope_torch, cos_sin_table, rope_qkv
+from .rotary import RotaryTable, rotary_append, rotary_frequencies, rotary_qkv, rotary_table
 
 
 @dataclass
@@ -47,6 +56,12 @@ class ContinuumDecoderConfig:
     rope_theta: float = 10000.0
     grad_checkpointing: bool = False
     ca_query_tile: int = 64
+    # rotary positions beyond the reference's interleaved pairs of the whole head (rotary.py)
+    rope_layout: str = "interleaved"
+    rope_dim: Optional[int] = None              # leading head values that turn (None: all)
+    rope_scaling: Optional[str] = None          # None, "linear", "ntk", "yarn"
+    rope_factor: float = 1.0
+    rope_original: Optional[int] = None         # "yarn": the context length before it was stretched
 
     def __post_init__(self):
         if self.d_model % self.n_heads:
@@ -57,6 +72,26 @@ class ContinuumDecoderConfig:
             raise ValueError("Invalid layer, context or CA query tile count")
         if self.dropout != 0:
             raise ValueError("The CA operator has no attention dropout; use --dropout 0.0")
+        if self.rope_layout not in ("interleaved", "half"):
+            raise ValueError("rope_layout must be 'interleaved' or 'half'")
+        if self.rope_dim is not None and not 2 <= self.rope_dim <= self.d_model // self.n_heads:
+            raise ValueError("rope_dim must be even and at most the head dimension")
+        if self.rope_general:
+            rotary_frequencies(self.rope_dim or self.d_model // self.n_heads, self.rope_theta, self.rope_scaling,
+                               self.rope_factor, self.rope_original)
+
+    @property
+    def rope_general(self) -> bool:
+        """Rotary positions that only rotary.py covers."""
+        return (self.rope_layout != "interleaved" or self.rope_dim is not None or self.rope_scaling is not None)
+
+    def rope_table(self, device) -> RotaryTable:
+        """The table of positions 0 .. block_size - 1: the reference's own 32-bit angles in its own case."""
+        head_dim = self.d_model // self.n_heads
+        if not self.rope_general:
+            return RotaryTable.from_cos_sin(cos_sin_table(self.block_size, head_dim, self.rope_theta, device))
+        return rotary_table(self.rope_dim or head_dim, self.block_size, self.rope_theta, self.rope_scaling,
+                            self.rope_factor, self.rope_original, device)
 
 
 class RMSNorm(nn.Module):
@@ -89,8 +124,9 @@ def apply_rope(q, k, theta: float):
 
 class ContinuumSelfAttention(nn.Module):
     def __init__(self, dim: int, heads: int, rope_theta: float, ca_query_tile: int,
-                 attention_fn: Optional[Callable] = None):
+                 attention_fn: Optional[Callable] = None, cfg: Optional[ContinuumDecoderConfig] = None):
         super().__init__()
+        self.cfg = cfg
         self.heads = heads
         self.head_dim = dim // heads
         self.rope_theta = rope_theta
@@ -104,13 +140,25 @@ class ContinuumSelfAttention(nn.Module):
 
     def forward(self, x):
         B, T, C = x.shape
-        q, k, v = rope_qkv(self.qkv(x), self.heads, self.rope_theta)
+        if self.cfg is not None and self.cfg.rope_general:
+            q, k, v = rotary_qkv(self.qkv(x), self.heads, self.cfg.rope_table(x.device), layout=self.cfg.rope_layout)
+        else:
+            q, k, v = rope_qkv(self.qkv(x), self.heads, self.rope_theta)
         if self.attention_fn is continuum_attention:
             # the operator stores y [B,T,H,D]: the projection's input below is a view of it
             y = continuum_attention(q, k, v, self.log_qk_gain, self.ca_query_tile, out_layout="bthd")
         else:
             y = self.attention_fn(q, k, v, self.log_qk_gain, self.ca_query_tile)
         return self.out(y.transpose(1, 2).reshape(B, T, C))
+
+    def forward_paged(self, x, k_cache, v_cache, step: PagedStep, table: RotaryTable):
+        """Packed new tokens x [N, C]: their keys and values go to the cache, their queries attend over it."""
+        layout = self.cfg.rope_layout if self.cfg is not None else "interleaved"
+        q = rotary_append(self.qkv(x), k_cache, v_cache, step.page_table, step.kv_lens, step.q_starts, table,
+                          heads=self.heads, layout=layout)
+        y = continuum_attention_paged(q, k_cache, v_cache, step.page_table, step.kv_lens, step.q_starts,
+                                      self.log_qk_gain, max_q_len=step.max_q_len)
+        return self.out(y.flatten(1))
 
 
 class _WeightGradFp32(torch.autograd.Function):
@@ -169,7 +217,7 @@ class CADecoderBlock(nn.Module):
         super().__init__()
         d = cfg.d_model
         self.norm1 = RMSNorm(d, cfg.eps)
-        self.attn = ContinuumSelfAttention(d, cfg.n_heads, cfg.rope_theta, cfg.ca_query_tile, attention_fn)
+        self.attn = ContinuumSelfAttention(d, cfg.n_heads, cfg.rope_theta, cfg.ca_query_tile, attention_fn, cfg)
         self.norm2 = RMSNorm(d, cfg.eps)
         self.mlp = GELUMLP(d, cfg.mlp_ratio)
 
@@ -231,6 +279,82 @@ class ContinuumDecoderLM(nn.Module):
                                           targets[:, 1:].reshape(-1), reduction="mean")
         return out
 
+    def make_cache(self, max_seqs: int, *, pages: Optional[int] = None, page_size: int = 64) -> PagedKVCache:
+        """A paged cache for ``max_seqs`` sequences of up to ``block_size`` tokens (``pages`` of all sequences
+        together, by default enough for all at full length), in the dtype of the attention projection."""
+        cfg, weight = self.cfg, self.lm_head.weight
+        dtype = weight.dtype
+        if weight.is_cuda and torch.is_autocast_enabled("cuda"):
+            dtype = torch.get_autocast_dtype("cuda")
+        return PagedKVCache(cfg.n_layers, pages or max_seqs * -(-cfg.block_size // page_size), page_size, cfg.n_heads,
+                            cfg.d_model // cfg.n_heads, max_seqs=max_seqs, max_len=cfg.block_size, dtype=dtype,
+                            device=weight.device)
+
+    @torch.no_grad()
+    def forward_paged(self, input_ids, cache: PagedKVCache, step: PagedStep):
+        """Logits [N, vocab] of packed new tokens input_ids [N] (sequence after sequence, as ``step`` counts
+        them): the rows that ``forward`` gives for them behind what the cache holds of their sequences."""
+        if input_ids.dim() != 1:
+            raise ValueError("forward_paged takes packed ids [N]")
+        table = self.cfg.rope_table(input_ids.device)
+        x = self.byte_emb(input_ids)
+        h = self.blocks[0].norm1(x)
+        for i, block in enumerate(self.blocks):
+            x, h = self._add_norm(x, block.attn.forward_paged(h, cache.k[i], cache.v[i], step, table), block.norm2)
+            nxt = self.blocks[i + 1].norm1 if i + 1 < len(self.blocks) else self.norm_f
+            x, h = self._add_norm(x, block.mlp(h), nxt)
+        return self.lm_head(h)
+
+    @torch.no_grad()
+    def generate(self, prompts, max_new_tokens: int, *, temperature: float = 0.0, generator=None,
+                 page_size: int = 64):
+        """Continue each prompt (1-D ids, of any lengths) by ``max_new_tokens`` tokens; returns their new ids
+        [len(prompts), max_new_tokens].  temperature 0 takes the likeliest token, else tokens are drawn.  The
+        prompts run as one packed step, then every step of one token a sequence replays one CUDA graph."""
+        if not prompts or min(len(p) for p in prompts) < 1 or max_new_tokens < 1:
+            raise ValueError("generate needs prompts of one token at least and max_new_tokens >= 1")
+        if temperature < 0:
+            raise ValueError("temperature must be >= 0")
+        device = self.lm_head.weight.device
+        lens = [len(p) for p in prompts]
+        if max(lens) + max_new_tokens - 1 > self.cfg.block_size:
+            raise ValueError(f"prompt and new tokens exceed block_size={self.cfg.block_size}")
+
+        def pick(logits):
+            if temperature == 0:
+                return logits.argmax(-1)
+            return torch.multinomial((logits.float() / temperature).softmax(-1), 1, generator=generator).squeeze(-1)
+
+        keys = [n + max_new_tokens - 1 for n in lens]
+        cache = self.make_cache(len(prompts), pages=sum(-(-n // page_size) for n in keys), page_size=page_size)
+        cache.reserve(keys)
+        step = cache.step(lens)
+        packed = torch.cat([torch.as_tensor(p, dtype=torch.long).flatten() for p in prompts]).to(device)
+        logits = self.forward_paged(packed, cache, step)
+        out = torch.empty(len(prompts), max_new_tokens, dtype=torch.long, device=device)
+        ids = pick(logits[step.q_starts[1:].long() - 1])
+        out[:, 0] = ids
+        if max_new_tokens == 1:
+            return out
+        # one token a sequence from here on: the same buffers every time, so the step is one graph
+        step = PagedStep(step.page_table, step.kv_lens.clone(),
+                         torch.arange(len(prompts) + 1, dtype=torch.int32, device=device), 1)
+        step.kv_lens += 1
+        side = torch.cuda.Stream(device)
+        side.wait_stream(torch.cuda.current_stream(device))
+        with torch.cuda.stream(side):
+            self.forward_paged(ids, cache, step)         # kernels and workspaces of the libraries, outside the graph
+        torch.cuda.current_stream(device).wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            logits = self.forward_paged(ids, cache, step)
+        for i in range(1, max_new_tokens):
+            graph.replay()                               # (the warm-up wrote the same keys to the same slots)
+            ids.copy_(pick(logits))
+            out[:, i] = ids
+            step.kv_lens += 1
+        return out
+
 
 def count_parameters(model: nn.Module) -> dict:
     params = list(model.parameters())
@@ -238,9 +362,31 @@ def count_parameters(model: nn.Module) -> dict:
             "trainable": sum(p.numel() for p in params if p.requires_grad)}
 
 
+def _main_generate(args):
+    """Tokens/s of ``generate`` (bf16 autocast, random weights and prompts), prompts and graph capture included."""
+    import json
+    dev = torch.device("cuda", torch.cuda.current_device())
+    torch.manual_seed(1337)
+    model = ContinuumDecoderLM(ContinuumDecoderConfig(block_size=args.seq_len)).to(dev)
+    g = torch.Generator(device="cpu").manual_seed(2000)
+    prompts = list(torch.randint(0, 256, (args.batch, args.seq_len - args.generate), generator=g))
+    e0, e1 = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        for i in range(max(args.warmup, 1) + 1):
+            e0.record()
+            model.generate(prompts, args.generate)
+            e1.record()
+            torch.cuda.synchronize()
+    ms = e0.elapsed_time(e1)
+    print(json.dumps({"metric": "CA-S decoder generated tokens/s", "value": args.batch * args.generate / (ms * 1e-3),
+                      "ms": ms, "batch": args.batch, "prompt": args.seq_len - args.generate,
+                      "new_tokens": args.generate}))
+
+
 def _main(argv=None):
     """Training-step throughput of the CA-S decoder on one GPU, synthetic bytes:
-    ``python -m continuum_attention_b200.decoder [--steps K] [--warmup W]``.
+    ``python -m continuum_attention_b200.decoder [--steps K] [--warmup W]``, or with ``--generate N`` the
+    throughput of generating N bytes behind prompts.
     Prints one JSON line (tokens/s, ms per step, last loss)."""
     import argparse
     import json
@@ -251,7 +397,11 @@ def _main(argv=None):
     p.add_argument("--warmup", type=int, default=3)
     p.add_argument("--batch", type=int, default=8)
     p.add_argument("--seq-len", type=int, default=2048)
+    p.add_argument("--generate", type=int, default=0, metavar="N",
+                   help="time the generation of N bytes behind prompts of seq-len - N bytes instead")
     args = p.parse_args(argv)
+    if args.generate:
+        return _main_generate(args)
     dev = torch.device("cuda", torch.cuda.current_device())
     torch.manual_seed(1337)
     model = ContinuumDecoderLM(ContinuumDecoderConfig(block_size=args.seq_len)).to(dev)

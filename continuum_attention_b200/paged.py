@@ -165,10 +165,31 @@ class PagedKVCache:
         self._table = torch.full((max_seqs, width), -1, dtype=torch.int32)   # host copy
         self._free = list(range(pages - 1, -1, -1))
         self.lens = [0] * max_seqs
+        self._held = [0] * max_seqs          # pages of each sequence
 
     @property
     def free_pages(self) -> int:
         return len(self._free)
+
+    def _grow(self, what: str, keys: Sequence[int]) -> None:
+        """Pages for keys[s] keys of each sequence; raises, and changes nothing, when they do not suffice."""
+        if max(keys) > self.max_len:
+            raise ValueError(f"{what}: a sequence of {max(keys)} tokens exceeds the cache's max_len={self.max_len}")
+        need = [max(-(-a // self.page_size), h) for a, h in zip(keys, self._held)]
+        more = sum(need) - sum(self._held)
+        if more > len(self._free):
+            raise RuntimeError(f"{what}: the cache is out of pages: {more} needed, {len(self._free)} free")
+        for s, (a, b) in enumerate(zip(self._held, need)):
+            for j in range(a, b):
+                self._table[s, j] = self._free.pop()
+        self._held = need
+
+    def reserve(self, keys: Sequence[int]) -> None:
+        """Hold pages for keys[s] keys of each sequence in advance, so that the page tables of later steps
+        (one captured into a graph, say) cover them."""
+        if len(keys) != len(self.lens):
+            raise ValueError(f"reserve takes one length for each of {len(self.lens)} sequences")
+        self._grow("reserve", keys)
 
     def step(self, new: Sequence[int]) -> PagedStep:
         """Make room for new[s] more tokens of each sequence s; the step that appends them.  Raises, and
@@ -176,30 +197,21 @@ class PagedKVCache:
         if len(new) != len(self.lens) or min(new) < 0:
             raise ValueError(f"step takes one count >= 0 for each of {len(self.lens)} sequences")
         after = [a + n for a, n in zip(self.lens, new)]
-        if max(after) > self.max_len:
-            raise ValueError(f"a sequence of {max(after)} tokens exceeds the cache's max_len={self.max_len}")
-        held = [-(-a // self.page_size) for a in self.lens]
-        need = [-(-a // self.page_size) for a in after]
-        if sum(need) - sum(held) > len(self._free):
-            raise RuntimeError(f"the cache is out of pages: {sum(need) - sum(held)} needed, {len(self._free)} free")
-        for s, (a, b) in enumerate(zip(held, need)):
-            for j in range(a, b):
-                self._table[s, j] = self._free.pop()
+        self._grow("step", after)
         self.lens = after
         starts = [0]
         for n in new:
             starts.append(starts[-1] + n)
-        device = self.k.device
         # one copy to the device for the three
         host = torch.cat((self._table.flatten(), torch.tensor(after + starts, dtype=torch.int32)))
-        dev = host.to(device)
+        dev = host.to(self.k.device)
         S, width = self._table.shape
-        return PagedStep(dev[:S * width].view(S, width), dev[S * width:S * width + S].clone(),
-                         dev[S * width + S:].clone(), max(max(new), 1))
+        return PagedStep(dev[:S * width].view(S, width), dev[S * width:S * width + S], dev[S * width + S:],
+                         max(max(new), 1))
 
     def release(self, seq: int) -> None:
         """Empty a sequence: its pages return to the free ones."""
-        for j in range(-(-self.lens[seq] // self.page_size)):
+        for j in range(self._held[seq]):
             self._free.append(int(self._table[seq, j]))
         self._table[seq] = -1
-        self.lens[seq] = 0
+        self._held[seq] = self.lens[seq] = 0

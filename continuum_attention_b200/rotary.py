@@ -22,6 +22,7 @@ cuda/continuum_attention.py:825-835) or ``"half"`` (pairs (p, p + R/2)).
 from __future__ import annotations
 
 import math
+import threading
 from typing import Optional
 
 import torch
@@ -96,6 +97,24 @@ class RotaryTable:
     @property
     def positions(self) -> int:
         return self.cos_sin.shape[0]
+
+
+_tables = {}
+_tables_lock = threading.Lock()
+
+
+def rotary_table(rotary_dim: int, max_positions: int, theta: float, scaling: Optional[str], factor: float,
+                 original_positions: Optional[int], device) -> RotaryTable:
+    """The ``RotaryTable`` of these settings, made once per device."""
+    key = (rotary_dim, max_positions, float(theta), scaling, float(factor), original_positions, str(device))
+    table = _tables.get(key)
+    if table is None:
+        with _tables_lock:
+            table = _tables.get(key)
+            if table is None:
+                table = _tables[key] = RotaryTable(rotary_dim, max_positions, theta=theta, scaling=scaling,
+                                                   factor=factor, original_positions=original_positions, device=device)
+    return table
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:

@@ -170,3 +170,33 @@ def test_cache_pages():
     s3 = c.step([0, 16, 0])
     assert c.free_pages == 1 and s3.kv_lens.tolist() == [0, 16, 2] and s3.max_q_len == 16
     assert len(set(s3.page_table[1, :4].tolist() + s3.page_table[2, :1].tolist())) == 5
+
+
+def test_cache_reserve():
+    c = PagedKVCache(1, 5, 4, 1, 8, max_seqs=2, max_len=16, dtype=torch.float32, device="cpu")
+    c.reserve([9, 2])
+    assert c.free_pages == 1 and c.lens == [0, 0]
+    s = c.step([1, 1])
+    assert c.free_pages == 1 and (s.page_table[0, :3] >= 0).all() and s.kv_lens.tolist() == [1, 1]
+    c.step([8, 0])                                          # within what is reserved
+    assert c.free_pages == 1
+    with pytest.raises(RuntimeError, match="out of pages"):
+        c.reserve([16, 16])
+    with pytest.raises(ValueError, match="max_len"):
+        c.reserve([17, 0])
+    c.release(0)
+    assert c.free_pages == 4 and c.lens == [0, 1]
+
+
+def test_decoder_options():
+    from continuum_attention_b200.decoder import ContinuumDecoderConfig
+    small = dict(d_model=64, n_heads=2)
+    assert not ContinuumDecoderConfig(**small).rope_general
+    assert ContinuumDecoderConfig(rope_dim=16, **small).rope_general
+    table = ContinuumDecoderConfig(rope_dim=16, rope_scaling="linear", rope_factor=2.0, block_size=10, **small).rope_table(
+        torch.device("cpu"))
+    assert table.rotary_dim == 16 and table.positions == 10
+    for bad in (dict(rope_layout="x"), dict(rope_dim=15), dict(rope_dim=34), dict(rope_scaling="y"),
+                dict(rope_scaling="yarn", rope_factor=2.0), dict(rope_scaling="linear", rope_factor=0.5)):
+        with pytest.raises(ValueError):
+            ContinuumDecoderConfig(**small, **bad)
