@@ -256,7 +256,7 @@ struct Config {
   static constexpr int Q_FRAG = RW > 1 ? DP * 32 : 0;   // bytes of a warp
   static constexpr int QF_AT = NST * STAGE + RW * WARP_HALO;
   static constexpr int DESC_AT = QF_AT + RW * Q_FRAG;
-  static constexpr int BAR_AT = DESC_AT + RING * 48;
+  static constexpr int BAR_AT = DESC_AT + RING * 32;
   static constexpr int GROUP_STRIDE = (BAR_AT + 2 * NST * 8 + 16 + 127) / 128 * 128;
   static constexpr int SMEM = GROUPS * GROUP_STRIDE;    // and the prefix sums behind it
   static_assert(KV_BYTES % 128 == 0 && STAGE % 128 == 0 && DESC_AT % 16 == 0, "");
@@ -266,16 +266,14 @@ struct Config {
                                                           THREADS / 32 * REGS_LAUNCH), "");
 };
 
-struct Desc {   // one tile of the stream
-  int kt, nt;         // tile in its unit, tiles of the unit
-  int first, last;    // of the piece
-  int start, n, len;  // the sequence
-  int h, rt;          // key head, row tile
-  int bad;            // the sequence's length or one of the tile's pages is out of range
-  int halo_page;      // of the key before a piece that does not start at key 0
-  int end;            // 1: the worker's last tile; 2: it has none
+// one tile of the stream; consumers read the first four words of every tile, the others at a piece's ends
+struct alignas(16) Desc {
+  int kt, flags, len, nt;   // tile in its unit, flags, keys of the sequence, tiles of the unit
+  int start, n, h, rt;      // the sequence's rows; key head; row tile
 };
-static_assert(sizeof(Desc) == 48, "");
+// of the piece: its first tile, its last; the sequence's length or a page is out of range; the worker's last
+// tile; the worker has none
+enum : int { kFirst = 1, kLast = 2, kBad = 4, kEnd = 8, kNone = 16 };
 
 template <typename T, typename C>
 __global__ void __launch_bounds__(C::THREADS, 1)
@@ -331,83 +329,80 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       return;
     }
     // `cur` stands at the next tile to be described; a tile's pages are fetched when it is described, one tile
-    // before its copies are issued
+    // before its copies are issued.  Every instruction here counts: the producer shares a scheduler with
+    // the consumers.
     typename Schedule<C::BR, TK>::Cursor cur;
     cur.at = x1;
     if (x0 < x1) cur = sched.locate(x0);
     if (cur.at >= x1) {            // no tile's place lies in this range
       if (lane == 0) {
         meta[worker].pieces = 0;
-        descs[0].end = 2;
+        descs[0].flags = kNone;
         bar_expect(full, 0);
       }
       if (after_chunks) pdl_wait();
       return;
     }
-    int slot_a = 0, kt0 = 0;       // kt0: the first tile of the piece
+    int kt0 = 0;                   // the first tile of the piece
     bool more = true, first = true, in_first = true;
     constexpr int NP = TK / 32;
-    int pg[NP];
+    int pg[NP];                    // page of a lane's rows
+    long long in_page[NP];         // and their offset in it
+    int halo_page = -1;            // of the key before a piece that does not start at key 0
+    Desc d;                        // the described tile
 
+  auto in_page_of = [&](int key, int col, int h) {
+    return (long long)h * a.head_stride + (long long)(key - col * a.page_size) * a.slot_stride;
+  };
   auto describe = [&]() {
-    if (more) {
-      const int seq_now = cur.s;
+    const int* pages = a.page_table + (size_t)cur.s * a.page_table_stride;
 #pragma unroll
-      for (int k = 0; k < NP; ++k) {
-        const int row = plan.unit_rows == 1 ? lane + 32 * k : (k == 0 && lane < 8 ? lane * NJ : TK);
-        const int key = cur.kt * TK + row;
-        pg[k] = -1;
-        if (row < TK && key < cur.len) pg[k] = a.page_table[(size_t)cur.s * a.page_table_stride + plan.page_of(key)];
-      }
-      if (first || cur.kt == 0) {
-        kt0 = cur.kt;
-        in_first = first;
-      }
-      more = cur.at + 1 < x1;
-      Desc d;
-      d.kt = cur.kt;
-      d.nt = cur.nt;
-      d.first = first || cur.kt == 0;
-      d.last = !more || cur.kt + 1 == cur.nt;
-      d.start = cur.start;
-      d.n = cur.n;
-      d.len = cur.len;
-      d.h = cur.h;
-      d.rt = cur.rt;
-      d.bad = cur.bad;
-      first = false;
-      const unsigned at = cur.at;
-      if (more) {
-        sched.advance(cur);
-        more = cur.at < x1;        // the next unit's first tile may lie behind the range
-      }
-      d.end = more ? 0 : 1;
-      if (lane == 0) {
-        d.halo_page = -1;
-        if (d.first && d.kt > 0) {
-          d.halo_page = a.page_table[(size_t)seq_now * a.page_table_stride + plan.page_of(d.kt * TK - 1)];
-        }
-        descs[slot_a] = d;
-        if (!more) {
-          // this worker joins the unit that starts in its range and goes on behind it
-          Meta mt;
-          mt.pieces = kt0 == 0 && d.kt + 1 < d.nt ? 1 + (int)((at + (d.nt - 1 - d.kt)) / per) - worker : 0;
-          mt.slot = in_first ? 0 : 1;
-          mt.start = d.start;
-          mt.rows = d.n * plan.group;
-          mt.h = d.h;
-          mt.rt = d.rt;
-          meta[worker] = mt;
-        }
+    for (int k = 0; k < NP; ++k) {
+      const int row = plan.unit_rows == 1 ? lane + 32 * k : (k == 0 && lane < 8 ? lane * NJ : TK);
+      const int key = cur.kt * TK + row;
+      pg[k] = -1;
+      if (row < TK && key < cur.len) {
+        const int col = plan.page_of(key);
+        pg[k] = pages[col];
+        in_page[k] = in_page_of(key, col, cur.h);
       }
     }
-    if (++slot_a == C::RING) slot_a = 0;
-    __syncwarp();
-  };
-
-  auto cache_at = [&](int page, int h, int key) {
-    return (size_t)page * a.page_stride + (size_t)h * a.head_stride +
-           (size_t)(key - plan.page_of(key) * a.page_size) * a.slot_stride;
+    d.kt = cur.kt;
+    d.nt = cur.nt;
+    d.flags = cur.bad ? kBad : 0;
+    if (first || cur.kt == 0) {
+      d.flags |= kFirst;
+      kt0 = cur.kt;
+      in_first = first;
+      first = false;
+      halo_page = cur.kt > 0 ? pages[plan.page_of(cur.kt * TK - 1)] : -1;
+    }
+    d.start = cur.start;
+    d.n = cur.n;
+    d.len = cur.len;
+    d.h = cur.h;
+    d.rt = cur.rt;
+    const unsigned at = cur.at;
+    more = at + 1 < x1;
+    if (!more || cur.kt + 1 == cur.nt) d.flags |= kLast;
+    if (more) {
+      sched.advance(cur);
+      more = cur.at < x1;        // the next unit's first tile may lie behind the range
+    }
+    if (!more) {
+      d.flags |= kEnd;
+      if (lane == 0) {
+        // this worker joins the unit that starts in its range and goes on behind it
+        Meta mt;
+        mt.pieces = kt0 == 0 && d.kt + 1 < d.nt ? 1 + (int)((at + (d.nt - 1 - d.kt)) / per) - worker : 0;
+        mt.slot = in_first ? 0 : 1;
+        mt.start = d.start;
+        mt.rows = d.n * plan.group;
+        mt.h = d.h;
+        mt.rt = d.rt;
+        meta[worker] = mt;
+      }
+    }
   };
 
   int slot_b = 0, stage_b = 0;
@@ -429,10 +424,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       return;
     }
     {
-      Desc& d = descs[slot_b];
       const uint32_t st = g0 + stage_b * C::STAGE, bar = full + 8 * stage_b;
-      const int base = d.kt * TK, len = d.len, h = d.h, first = d.first;
-      end = d.end;
+      const int base = d.kt * TK;
+      end = d.flags & kEnd;
       const uint32_t row_bytes = (uint32_t)a.D * 2;
       const uint32_t unit_bytes = plan.unit_rows * row_bytes;
       bool go[NP], bad = false;
@@ -440,28 +434,32 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 #pragma unroll
       for (int k = 0; k < NP; ++k) {
         const int row = plan.unit_rows == 1 ? lane + 32 * k : (k == 0 && lane < 8 ? lane * NJ : TK);
-        go[k] = row < TK && base + row < len;
-        const bool in = pg[k] >= 0 && pg[k] < a.num_pages;
-        bad |= go[k] && !in;
-        go[k] = go[k] && in;
+        go[k] = pg[k] >= 0 && pg[k] < a.num_pages;      // -1 where there is nothing to fetch
+        bad |= !go[k] && row < TK && base + row < d.len;
         bytes += __popc(__ballot_sync(0xffffffffu, go[k])) * 2 * unit_bytes;
       }
-      const int halo_page = d.halo_page;
-      const bool halo = first && base > 0 && base - 1 < len;
-      const bool halo_go = halo && halo_page >= 0 && halo_page < a.num_pages;
-      bad |= halo && !halo_go;
-      if (halo_go) bytes += 2 * row_bytes;
+      bool halo = false;
       int q_row = -1;
-      if constexpr (C::kStageQ) {
-        if (first && lane < C::RPW && d.rt * C::BR + lane < d.n * plan.group) q_row = d.rt * C::BR + lane;
-        bytes += __popc(__ballot_sync(0xffffffffu, q_row >= 0)) * row_bytes;
+      if (d.flags & kFirst) {
+        halo = base > 0 && base - 1 < d.len;
+        const bool in = halo_page >= 0 && halo_page < a.num_pages;
+        bad |= halo && !in;
+        halo = halo && in;
+        if (halo) bytes += 2 * row_bytes;
+        if constexpr (C::kStageQ) {
+          if (lane < C::RPW && d.rt * C::BR + lane < d.n * plan.group) q_row = d.rt * C::BR + lane;
+          bytes += __popc(__ballot_sync(0xffffffffu, q_row >= 0)) * row_bytes;
+        }
       }
       bad = __any_sync(0xffffffffu, bad);
       if (lane == 0) {
         if (bad) {
-          d.bad = 1;
+          d.flags |= kBad;
           record_invalid();
         }
+        int4* to = reinterpret_cast<int4*>(&descs[slot_b]);
+        to[0] = make_int4(d.kt, d.flags, d.len, d.nt);
+        to[1] = make_int4(d.start, d.n, d.h, d.rt);
         bar_expect(bar, bytes);
       }
       __syncwarp();
@@ -469,14 +467,15 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       for (int k = 0; k < NP; ++k) {
         if (go[k]) {
           const int row = plan.unit_rows == 1 ? lane + 32 * k : lane * NJ;
-          const size_t at = cache_at(pg[k], h, base + row);
+          const long long at = (long long)pg[k] * a.page_stride + in_page[k];
           const uint32_t dst = st + (row / NJ) * C::PITCH + (row % NJ) * ROWB;
           bulk_load(dst, (const T*)a.k_cache + at, unit_bytes, bar);
           bulk_load(dst + C::KV_BYTES, (const T*)a.v_cache + at, unit_bytes, bar);
         }
       }
-      if (halo_go && lane == 31) {
-        const size_t at = cache_at(halo_page, h, base - 1);
+      if (halo && lane == 31) {
+        const long long at = (long long)halo_page * a.page_stride +
+                             in_page_of(base - 1, plan.page_of(base - 1), d.h);
         bulk_load(st + C::HALO, (const T*)a.k_cache + at, row_bytes, bar);
         bulk_load(st + C::HALO + ROWB, (const T*)a.v_cache + at, row_bytes, bar);
       }
@@ -484,7 +483,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         const int t = q_row / plan.group;
         bulk_load(st + C::Q_AT + lane * ROWB,
                   (const T*)a.q + (size_t)(d.start + t) * a.q_token_stride +
-                      (size_t)(h * plan.group + q_row - t * plan.group) * a.q_head_stride,
+                      (size_t)(d.h * plan.group + q_row - t * plan.group) * a.q_head_stride,
                   row_bytes, bar);
       }
     }
@@ -526,20 +525,22 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   for (int end = 0; !end;) {
     if (!bar_wait(full + 8 * stage, parity, gave_up)) break;
     const Desc& d = descs[slot];
-    end = d.end;
-    if (end == 2) break;
+    const int4 head = *reinterpret_cast<const int4*>(&d);
+    const int kt = head.x, flags = head.y, len = head.z;
+    end = flags & (kEnd | kNone);
+    if (flags & kNone) break;
     uint8_t* sm = gsm + stage * C::STAGE;
     const uint32_t st = g0 + stage * C::STAGE;
-    const int base = d.kt * TK;
-    const int rows = d.n * plan.group;
-    if (d.first) {
-      kt0 = d.kt;
+    const int base = kt * TK;
+    if (flags & kFirst) {
+      kt0 = kt;
+      const int rows = d.n * plan.group;
       piece_bad = 0;
       in_first = first_tile;
       first_tile = false;
       const int row0 = d.rt * C::BR + warp * C::RPW;
       const int row_last = min(rows, row0 + C::RPW) - 1;    // < row0: the warp has no row
-      const int lead = d.len - d.n;                         // position of the sequence's first row
+      const int lead = len - d.n;                         // position of the sequence's first row
       i_min = lead + row0 / plan.group;
       i_max = row_last >= row0 ? lead + row_last / plan.group : -1;
       const T* qrow[RS];
@@ -585,7 +586,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         for (int k = 0; k < NKK; ++k)
           *reinterpret_cast<uint4*>(my_qf + 512 * k) = make_uint4(qf[k][0], qf[k][1], qf[k][2], qf[k][3]);
       }
-      if (d.kt > 0 && base - 1 <= i_max) {
+      if (kt > 0 && base - 1 <= i_max) {
         // the score of key base - 1, in every column of one score tile
         float s[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -602,13 +603,13 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       }
       if (lane < CH)
         *reinterpret_cast<uint4*>(my_halo_p + 16 * lane) =
-            d.kt > 0 ? *reinterpret_cast<const uint4*>(sm + C::HALO + ROWB + 16 * lane) : make_uint4(0u, 0u, 0u, 0u);
+            kt > 0 ? *reinterpret_cast<const uint4*>(sm + C::HALO + ROWB + 16 * lane) : make_uint4(0u, 0u, 0u, 0u);
     }
-    piece_bad |= d.bad;
-    if (base + TK > d.len) {
+    piece_bad |= flags & kBad;
+    if (base + TK > len) {
       // V behind the sequence's end may hold anything, and 0 times it has to be 0.  The warps of a group
       // write the same zeros.
-      for (int r = max(d.len - base, 0) * CH + lane; r < TK * CH; r += 32) {
+      for (int r = max(len - base, 0) * CH + lane; r < TK * CH; r += 32) {
         const int row = r / CH;
         *reinterpret_cast<uint4*>(sm + C::KV_BYTES + (row / NJ) * C::PITCH + (row % NJ) * ROWB + (r % CH) * 16) =
             make_uint4(0u, 0u, 0u, 0u);
@@ -702,7 +703,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         float2 first;
         float last;
         if (edge) {
-          weigh<T, true, NJ>(s[u], m2, sL, kc, pos[u], d.first ? base : base - 1, hi[u], lo[u], first, last, z2[u]);
+          weigh<T, true, NJ>(s[u], m2, sL, kc, pos[u], flags & kFirst ? base : base - 1, hi[u], lo[u], first, last, z2[u]);
         } else {
           weigh<T, false, NJ>(s[u], m2, sL, kc, pos[u], base, hi[u], lo[u], first, last, z2[u]);
         }
@@ -740,8 +741,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     }
 
     const uint8_t* vlast = sm + C::KV_BYTES + 7 * C::PITCH + (NJ - 1) * ROWB;   // V of the tile's last key
-    if (d.last) {
-      const bool whole = kt0 == 0 && d.kt + 1 == d.nt;
+    if (flags & kLast) {
+      const bool whole = kt0 == 0 && kt + 1 == head.w;
+      const int rows = d.n * plan.group;
       const int row0 = d.rt * C::BR + warp * C::RPW;
       const int key = base + TK - 1;             // the key whose weight is still carried
       const long long slot_row = ((long long)worker * 2 + (in_first ? 0 : 1)) * C::BR + warp * C::RPW;
@@ -807,9 +809,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 namespace {
 
 // The forms: decoding with 8 or 16 rows a warp, and chunks
-template <int DP> using Decode8 = std::conditional_t<DP == 64, Config<64, 32, 8, 1, 8, 2, 200, 56>, Config<128, 32, 8, 1, 4, 2, 0, 0>>;
-template <int DP> using Decode16 = std::conditional_t<DP == 64, Config<64, 32, 16, 1, 8, 2, 200, 56>, Config<128, 32, 16, 1, 4, 2, 0, 0>>;
-template <int DP> using Chunk = Config<DP, DP == 64 ? 64 : 32, 16, 4, 3, 3, 152, 56>;
+template <int DP> using Decode8 = std::conditional_t<DP == 64, Config<64, 32, 8, 1, 8, 2, 184, 72>, Config<128, 32, 8, 1, 4, 2, 0, 0>>;
+template <int DP> using Decode16 = std::conditional_t<DP == 64, Config<64, 32, 16, 1, 8, 2, 184, 72>, Config<128, 32, 16, 1, 4, 2, 0, 0>>;
+template <int DP> using Chunk = Config<DP, DP == 64 ? 64 : 32, 16, 4, 3, 3, 144, 80>;
 
 constexpr int kDecodeUnitCost = 2, kChunkUnitCost = 2;
 
