@@ -155,10 +155,11 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) { return __half22f
 // first is the pair of place 0, unsplit, but for the mass that ends at key kc - 1, which is the lane's to
 // the left; last is the mass that ends at the run's last key.  Pair by pair, each needing the one before:
 // a score's registers take its weight's parts.
-// kEdge adds the half caps of keys 0 and i where this run weighs them.  Key i's belongs to this piece when
-// i >= lowest: the piece before it has weighed its own last key to the end.
-template <typename T, bool kEdge, int NJ>
-__device__ __forceinline__ void weigh(const float2 (&sv)[NJ], float m2, float sL, int kc, int i, int lowest,
+// edge (of the whole warp) adds the half caps of keys 0 and i where this run weighs them.  Key i's belongs to
+// this piece when i >= lowest: the piece before it has weighed its own last key to the end.  (One body with
+// a jump around the caps: a second body for edges cost 30 moves a tile where the two meet.)
+template <typename T, int NJ>
+__device__ __forceinline__ void weigh(const float2 (&sv)[NJ], float m2, float sL, bool edge, int kc, int i, int lowest,
                                       uint32_t (&hi)[NJ], uint32_t (&lo)[NJ], float2& first, float& last, float2& z2) {
   const float2 l2e = splat2(kLog2e), nm2 = splat2(-m2);
   auto exps = [&](float2 v) {
@@ -203,9 +204,11 @@ __device__ __forceinline__ void weigh(const float2 (&sv)[NJ], float m2, float sL
       w[t] = sub2(w[t], m1[t]);
     }
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < 4; ++t)
       if (j0 + t > 0) w[t] = add2(w[t], t ? m1[t - 1] : m1_before);
-      if (kEdge) {
+    if (edge) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
         const float2 el = t ? e[t - 1] : el0;
         const int kx = kc + j0 + t - 1, ky = kx + NJ;      // the keys these weights belong to
         const float nx = (kx == 0 && i >= 0 ? 0.5f : 0.f) + (kx == i && i >= lowest ? 0.5f : 0.f);
@@ -702,11 +705,8 @@ __global__ void __launch_bounds__(C::THREADS, 1)
         carry_s[u] = got;                       // of use to the quad's first lane only
         float2 first;
         float last;
-        if (edge) {
-          weigh<T, true, NJ>(s[u], m2, sL, kc, pos[u], flags & kFirst ? base : base - 1, hi[u], lo[u], first, last, z2[u]);
-        } else {
-          weigh<T, false, NJ>(s[u], m2, sL, kc, pos[u], base, hi[u], lo[u], first, last, z2[u]);
-        }
+        weigh<T, NJ>(s[u], m2, sL, edge, kc, pos[u], flags & kFirst ? base : base - 1, hi[u], lo[u], first, last,
+                     z2[u]);
         got = __shfl_sync(0xffffffffu, last, left);
         first.x += c4 == 0 ? carry_b[u] : got;
         carry_b[u] = got;
@@ -811,7 +811,7 @@ namespace {
 // The forms: decoding with 8 or 16 rows a warp, and chunks
 template <int DP> using Decode8 = std::conditional_t<DP == 64, Config<64, 32, 8, 1, 8, 2, 184, 72>, Config<128, 32, 8, 1, 4, 2, 0, 0>>;
 template <int DP> using Decode16 = std::conditional_t<DP == 64, Config<64, 32, 16, 1, 8, 2, 184, 72>, Config<128, 32, 16, 1, 4, 2, 0, 0>>;
-template <int DP> using Chunk = Config<DP, DP == 64 ? 64 : 32, 16, 4, 3, 3, 144, 80>;
+template <int DP> using Chunk = Config<DP, DP == 64 ? 64 : 32, 16, 4, 3, 3, 152, 56>;
 
 constexpr int kDecodeUnitCost = 2, kChunkUnitCost = 2;
 
