@@ -819,16 +819,9 @@ template <typename T, typename C>
 cudaError_t launch_main(const Args& a, Plan plan, const Pieces& pc, bool after_chunks) {
   static_assert(C::SMEM + (kMaxSeqs + 1) * (int)sizeof(unsigned) <= 232448, "shared memory of a block");
   const size_t smem = C::SMEM + (size_t)(a.seqs + 1) * sizeof(unsigned);
-  static thread_local int set_dev = -1;    // the attribute belongs to the device
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  cudaError_t e = cudaFuncSetAttribute(mma_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       C::SMEM + (kMaxSeqs + 1) * (int)sizeof(unsigned));
   if (e != cudaSuccess) return e;
-  if (set_dev != dev) {
-    e = cudaFuncSetAttribute(mma_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             C::SMEM + (kMaxSeqs + 1) * (int)sizeof(unsigned));
-    if (e != cudaSuccess) return e;
-    set_dev = dev;
-  }
   plan.unit_rows = a.D == C::DP && a.slot_stride == C::DP && a.page_size % C::NJ == 0 ? C::NJ : 1;
   return launch_pdl(mma_kernel<T, C>, dim3(num_sms_cached()), dim3(C::THREADS), smem, a.stream, a, plan, pc.o, pc.mz,
                     pc.meta, (int)after_chunks);

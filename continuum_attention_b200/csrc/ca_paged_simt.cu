@@ -414,16 +414,9 @@ cudaError_t launch_main(const Args& a, const Plan& plan, const Pieces& pc) {
   // (with the prefix sums of 200 sequences; with more, fewer blocks run at once)
   static_assert((C::SMEM + 200 * 4 + 1024) * C::PER_SM <= 233472, "shared memory of an SM");
   const size_t smem = C::SMEM + (size_t)(a.seqs + 1) * sizeof(unsigned);
-  static thread_local int set_dev = -1;    // the attribute belongs to the device
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+  cudaError_t e = cudaFuncSetAttribute(simt_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       C::SMEM + (kMaxSeqs + 1) * (int)sizeof(unsigned));
   if (e != cudaSuccess) return e;
-  if (set_dev != dev) {
-    e = cudaFuncSetAttribute(simt_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             C::SMEM + (kMaxSeqs + 1) * (int)sizeof(unsigned));
-    if (e != cudaSuccess) return e;
-    set_dev = dev;
-  }
   return launch_pdl(simt_kernel<C>, dim3((unsigned)pc.workers), dim3(C::NT), smem, a.stream, a, plan, pc.o, pc.mz,
                     pc.meta);
 }

@@ -297,7 +297,7 @@ int ca_rotary_qkv_backward(const void* dq, const void* dk, const void* dv, const
  * (q_starts has num_seqs + 1 entries), and kv_lens counts them: row n sits at position
  * kv_lens[s] - (q_starts[s+1] - n).  Rows behind q_starts[num_seqs] are left as they
  * were.  kv_lens, q_starts and page_table are int32 on the device; entries of the page
- * table that no key needs are never used.  A page outside 0 .. num_pages-1, a length
+ * table that no key needs are never used; a row of it covers 2^30 keys at most.  A page outside 0 .. num_pages-1, a length
  * beyond pages_per_seq * page_size, or rows outside the buffers are recorded in
  * ca_device_status() as CA_ERR_INVALID_ARGUMENT; nothing is read or written there.
  *
@@ -320,10 +320,15 @@ int ca_rotary_append(const void* qkv, int64_t qkv_stride, const float* cos_sin, 
  * h / (heads / kv_heads), with the scores, trajectories and caps of ca_forward.  A row at a
  * negative position gives zeros.  q rows are q_token_stride and heads q_head_stride elements
  * apart; o is [num_rows][heads][D].  The rows of a sequence whose length is out of range, and
- * those that see a page out of range, come out NaN (see above).  max_q_len is the number of new
+ * those that see a page out of range, come out NaN (see above; other rows of that sequence
+ * may).  Keys and values behind a sequence's length, and pages that no sequence holds, may
+ * hold anything; a value that is not finite reaches the rows that see it, and may reach
+ * earlier rows of the same call and sequence (0 times it is NaN).  How a row's sum is cut
+ * depends on the other sequences of the call, so its last bit may; the same call gives the
+ * same bits every time.  max_q_len is the number of new
  * tokens of the longest sequence, by which the kernel is chosen; a wrong one costs time only.
- * heads a multiple of kv_heads; D a multiple of 8, at most 128; every buffer and stride a
- * multiple of 16 bytes (o and q included).  workspace holds
+ * heads a multiple of kv_heads; D a multiple of 8, at most 128; at most 2048 sequences; every
+ * buffer and stride a multiple of 16 bytes (o and q included).  workspace holds
  * ca_paged_workspace_size() bytes (256-byte aligned; its contents are ignored, and it
  * belongs to this call until the call's GPU work has finished).
  */

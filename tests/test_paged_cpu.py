@@ -30,7 +30,7 @@ def paged_args(**kw):
     (dict(G=0), 1, "multiple of kv_heads"), (dict(maxq=0), 1, "max_q_len"), (dict(q=None), 1, "null"),
     (dict(o=None), 1, "null"), (dict(table=None), 1, "null"), (dict(k=None), 1, "null"),
     (dict(q=ctypes.c_void_p(264)), 1, "aligned"), (dict(qt=260), 1, "strides"), (dict(ss=60), 1, "strides"),
-    (dict(ts=7), 1, "page table"), (dict(pps=1 << 27, ts=1 << 27, page=64), 2, "2^31-1"),
+    (dict(ts=7), 1, "page table"), (dict(pps=1 << 25, ts=1 << 25, page=64), 2, "2^30"),
     (dict(rows=1 << 31), 2, "2^31-1"), (dict(seqs=2049), 2, "2048"), (dict(maxq=1, rows=1 << 28, H=16), 2, "2^31-1"),
 ])
 def test_paged_forward_refusals(change, status, text):
