@@ -1,6 +1,7 @@
 // ca_paged.cu -- Continuum Attention of new tokens over a paged cache: the choice of kernels.
 //
-// bf16 and f16 run on the tensor cores (ca_paged_mma.cu), f32 on the FMA pipes
+// bf16 and f16 run on the tensor cores (decoding and wide heads ca_paged_mma.cu, other chunks
+// ca_paged_tc.cu), f32 on the FMA pipes
 // (ca_paged_simt.cu), whose scores are exact to 32 bits as f32 inputs ask.
 #include "ca_paged.cuh"
 
@@ -19,10 +20,11 @@ cudaError_t forward(const Args& a, int dtype, void* workspace) {
 }
 
 cudaError_t read_status(int* out, bool reset) {
-  int more = 0;
+  int more[2] = {0, 0};
   cudaError_t e = mma_read_status(out, reset);
-  if (e == cudaSuccess) e = simt_read_status(&more, reset);
-  if (*out == 0) *out = more;
+  if (e == cudaSuccess) e = tc_read_status(&more[0], reset);
+  if (e == cudaSuccess) e = simt_read_status(&more[1], reset);
+  if (*out == 0) *out = more[0] ? more[0] : more[1];
   return e;
 }
 

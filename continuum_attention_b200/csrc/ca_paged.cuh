@@ -62,6 +62,13 @@ int simt_launches(const Args& a);
 cudaError_t simt_forward(const Args& a, void* workspace);
 cudaError_t simt_read_status(int* out, bool reset);
 
+// chunks in bf16 and f16 with D <= 64 on tcgen05 (ca_paged_tc.cu): units of tc_br() rows, tc_groups() workers per SM
+struct Pieces;
+int tc_br();
+int tc_groups();
+cudaError_t tc_launch(const Args& a, const Plan& plan, int dtype, const Pieces& pc);
+cudaError_t tc_read_status(int* out, bool reset);
+
 // Prefix sums of the sequences' places in shared memory (all threads of the block take part in the
 // constructor), and cursors into the stream of tiles: sequence, key head, row tile, key tile.
 template <int BR, int TK>

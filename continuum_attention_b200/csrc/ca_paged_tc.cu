@@ -1,0 +1,605 @@
+// ca_paged_tc.cu -- Continuum Attention of chunks over a paged cache on tcgen05: bf16 and f16,
+// head values up to 64, units of 128 rows.
+//
+// Work is divided as in ca_paged_mma.cu (units, places, pieces, merge).  One block runs on an SM,
+// with three workers that share nothing but the tensor pipe: each has four math warps (a thread
+// is a row, its TMEM lane), a warp that issues the products and a warp that loads.
+//
+// A worker's tensor memory: three regions of 32 columns and O in 64.  Tile t of 32 keys has its
+// scores S = Q K^T in region t mod 3; its weights P overwrite them in place, each 16 keys as 8
+// columns of hi pairs and 8 of lo pairs (two 16-bit parts, see ca_paged_mma.cu); then
+// O += P_hi V + P_lo V with P as the A operand from tensor memory.  The products run in issue
+// order, so S of tile t + 3 is issued behind P V of tile t into the same region, and the math
+// warps find the next tiles' scores done.  O is rescaled in place, only when a row's maximum
+// has grown by more than 8 nats.
+//
+// Columns: S column 16 c + 2 j + s is key 16 c + j + 8 s (K rows are gathered in that order),
+// so a register pair of the score load is the pair (j, j + 8), whose left neighbours are the pair
+// before it, and every step of the moments is one packed instruction for two keys.  P keeps
+// the order, and V's rows are gathered in it, one key early (ca_paged_mma.cu: cutting keys).
+// Being one thread's, a row needs no exchange between lanes at all.
+//
+// The loader gathers rows through the page table with 16-byte cp.async in the 128-byte swizzle
+// that the matrix descriptors name, any page size and any strides; rows that no key fills are
+// zero.
+//
+// Against the mma.sync form the products take no issue slots of the math warps, and O no
+// registers, which leaves room for three math warps on a scheduler and less work in each.
+#include "ca_common.cuh"
+#include "ca_paged.cuh"
+#include "ca_paged_math.cuh"
+#include "ca_sm100_ptx.cuh"
+
+namespace ca {
+namespace paged {
+
+namespace {
+
+using namespace sm100;
+
+constexpr int TK = 32, BR = 128, NREG = 3, NST = 4, GROUPS = 3, RING = NST + 1;
+constexpr int MATH_WARPS = 4 * GROUPS, THREADS = (MATH_WARPS + 8) * 32;   // and a warpgroup of issuers, one of loaders
+constexpr int REGS_MATH = 112, REGS_OTHER = 72;
+static_assert(GROUPS * REGS_MATH + 2 * REGS_OTHER <= THREADS / 128 * (65536 / THREADS / 8 * 8), "registers of the launch");
+constexpr uint32_t COLS = 160, COL_O = 96;          // a worker's columns: regions at 0, 32, 64
+static_assert(GROUPS * COLS <= 512, "tensor memory");
+constexpr uint32_t Q_BYTES = BR * 128, KV_BYTES = TK * 128;
+
+enum : int { kFirst = 1, kLast = 2, kBad = 4, kEnd = 8, kNone = 16, kQ1 = 32 };   // kQ1: Q is in buffer 1
+
+struct alignas(16) Slot {     // what a tile's readers need beside its stage
+  int kt, flags, len, nt;     // tile in its unit, flags, keys of the sequence, tiles of the unit
+  int start, n, h, rt;        // the sequence's rows; key head; row tile
+  uint8_t k_before[128];      // K of the key before a piece
+  uint8_t v_last[128];        // V of a piece's last key
+};
+
+struct alignas(1024) Group {
+  uint8_t q[2][Q_BYTES];
+  uint8_t k[NST][KV_BYTES];
+  uint8_t v[NST][KV_BYTES];
+};
+
+struct alignas(16) Control {
+  uint64_t full[NST];         // a tile's rows and descriptor are there                 (1: the loader)
+  uint64_t free_[NST];        // its products have read them                              (1: commit)
+  uint64_t s_full[NREG];      // its scores are in tensor memory                          (1: commit)
+  uint64_t p_ready[NREG];     // its weights are                                          (4: math warps)
+  uint64_t pv_done[2];        // P V of tile t and all before it: barrier t & 1           (1: commit)
+  uint64_t drained;           // every product, where a wait gave up                      (1: commit)
+  int gave_up;
+  Slot ring[RING];
+};
+
+constexpr size_t kSmem = GROUPS * (sizeof(Group) + sizeof(Control)) + 16;   // and the prefix sums behind it
+
+template <int N>
+__device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool zero) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(zero ? 0 : 16) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// ------------------------------------------------------------------ the loader
+
+template <typename T>
+__device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const Schedule<BR, TK>& sched, int worker,
+                                          unsigned per, unsigned x0, unsigned x1, Group& gm, Control& ct,
+                                          Meta* __restrict__ meta) {
+  const int lane = threadIdx.x & 31;
+  volatile int* ab = &ct.gave_up;
+  typename Schedule<BR, TK>::Cursor cur;
+  cur.at = x1;
+  if (x0 < x1) cur = sched.locate(x0);
+  if (cur.at >= x1) {              // no tile's place lies in this range
+    if (lane == 0) {
+      meta[worker].pieces = 0;
+      ct.ring[0].flags = kNone;
+      mbar_arrive(&ct.full[0]);
+    }
+    return;
+  }
+  const uint32_t qs = smem_u32(gm.q), ks = smem_u32(gm.k), vs = smem_u32(gm.v);
+  const int row8 = lane >> 3, ch = lane & 7;          // a copy instruction: 4 rows of 8 chunks
+  const bool pad = ch * 8 >= a.D;
+  const T* kb = (const T*)a.k_cache + ch * 8;
+  const T* vb = (const T*)a.v_cache + ch * 8;
+
+  auto page_at = [&](int key) {                       // of this sequence, -1 beyond its keys
+    return key < cur.len ? a.page_table[(size_t)cur.s * a.page_table_stride + plan.page_of(key)] : -1;
+  };
+  auto offset = [&](int page, int key, int h) {
+    return (long long)page * a.page_stride + (long long)h * a.head_stride +
+           (long long)(key - plan.page_of(key) * a.page_size) * a.slot_stride;
+  };
+
+  int done = 0;                  // tiles signalled
+  // the oldest tiles' copies are there: tell the readers of tiles done .. upto - 1
+  auto signal = [&](int upto) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    for (; done < upto; ++done)
+      if (lane == 0) mbar_arrive(&ct.full[done % NST]);
+  };
+
+  bool first = true, in_first = true;
+  int kt0 = 0, qbuf = 1;
+  int last_tile[2] = {-1, -1};   // the last tiles of the units before this one and before that
+  long long before = -1;         // the row of the key before the tile (-1: none)
+  int pg = page_at(cur.kt * TK + lane);
+  int pg_before = cur.kt > 0 ? page_at(cur.kt * TK - 1) : -1;
+  bool end = false;
+  int t = 0;
+  for (; !end; ++t) {
+    const int st = t % NST;
+    if (t >= NST && !__all_sync(0xffffffffu, mbar_try_wait(&ct.free_[st], (t / NST - 1) & 1))) {
+      // the readers may be waiting for tiles that are there but not signalled
+      copy_wait<0>();
+      signal(t);
+      if (!mbar_wait_warp(&ct.free_[st], (t / NST - 1) & 1, ab)) break;
+    }
+    const int base = cur.kt * TK;
+    const bool opens = first || cur.kt == 0;
+    int flags = cur.bad ? kBad : 0;
+    if (opens) {
+      flags |= kFirst;
+      kt0 = cur.kt;
+      in_first = first;
+      qbuf ^= 1;
+      // Q of the unit before the last one lay in this buffer: its products have to be done (they are known to
+      // be where the stage of its last tile has been filled again since)
+      const int u = last_tile[1];
+      if (u >= 0 && u + NST > t && !__all_sync(0xffffffffu, mbar_try_wait(&ct.free_[u % NST], (u / NST) & 1))) {
+        copy_wait<0>();
+        signal(t);
+        if (!mbar_wait_warp(&ct.free_[u % NST], (u / NST) & 1, ab)) break;
+      }
+      const int rows = cur.n * plan.group, row0 = cur.rt * BR;
+#pragma unroll 4
+      for (int r0 = 0; r0 < BR; r0 += 4) {
+        const int r = r0 + row8, row = row0 + r;
+        const bool none = row >= rows || pad;
+        const int tk = none ? 0 : row / plan.group;
+        const T* src = (const T*)a.q + (none ? 0 : (size_t)(cur.start + tk) * a.q_token_stride +
+                                                        (size_t)(cur.h * plan.group + row - tk * plan.group) *
+                                                            a.q_head_stride + ch * 8);
+        copy16(qs + qbuf * Q_BYTES + r * 128 + ((ch ^ (r & 7)) << 4), src, none);
+      }
+    }
+    if (qbuf) flags |= kQ1;
+    Slot& slot = ct.ring[t % RING];
+
+    // this lane's key, and the one before the tile
+    const int key = base + lane;
+    bool bad = key < cur.len && (pg < 0 || pg >= a.num_pages);
+    const long long off = key < cur.len && !bad ? offset(pg, key, cur.h) : -1;
+    if (opens) {
+      before = -1;
+      if (base > 0 && base - 1 < cur.len) {
+        if (pg_before < 0 || pg_before >= a.num_pages) bad = true;
+        else before = offset(pg_before, base - 1, cur.h);
+      }
+      if (lane < 8 && base > 0)
+        copy16(smem_u32(slot.k_before) + ch * 16, before < 0 ? (const T*)a.k_cache : kb + before, before < 0 || pad);
+    }
+    // row r of the stage is the key at 16 (r / 16) + (r % 16) / 2 + 8 (r % 2): K of it, V of the key before it
+#pragma unroll
+    for (int r0 = 0; r0 < TK; r0 += 4) {
+      const int r = r0 + row8;
+      const int p = (r & 16) + ((r & 15) >> 1) + ((r & 1) << 3);
+      const long long ko = __shfl_sync(0xffffffffu, off, p);
+      long long vo = __shfl_sync(0xffffffffu, off, (p + 31) & 31);
+      if (p == 0) vo = before;
+      const uint32_t dst = st * KV_BYTES + r * 128 + ((ch ^ (r & 7)) << 4);
+      copy16(ks + dst, ko < 0 ? (const T*)a.k_cache : kb + ko, ko < 0 || pad);
+      copy16(vs + dst, vo < 0 ? (const T*)a.v_cache : vb + vo, vo < 0 || pad);
+    }
+    before = __shfl_sync(0xffffffffu, off, 31);
+
+    const int kt = cur.kt, nt = cur.nt, start = cur.start, n = cur.n, len = cur.len, h = cur.h, rt = cur.rt;
+    const unsigned at = cur.at;
+    bool more = at + 1 < x1;
+    const bool closes = !more || cur.kt + 1 == cur.nt;
+    if (closes) {
+      flags |= kLast;
+      if (lane < 8)
+        copy16(smem_u32(slot.v_last) + ch * 16, before < 0 ? (const T*)a.v_cache : vb + before, before < 0 || pad);
+      last_tile[1] = last_tile[0];
+      last_tile[0] = t;
+    }
+    copy_commit();
+    first = false;
+    if (more) {
+      sched.advance(cur);
+      more = cur.at < x1;        // the next unit's first tile may lie behind the range
+    }
+    if (more) {
+      pg = page_at(cur.kt * TK + lane);
+      pg_before = -1;            // a unit that is entered here starts at key 0
+    } else {
+      flags |= kEnd;
+      end = true;
+    }
+    bad = __any_sync(0xffffffffu, bad);
+    if (bad) flags |= kBad;
+    if (lane == 0) {
+      if (bad) record_invalid();
+      int4* to = reinterpret_cast<int4*>(&slot);
+      to[0] = make_int4(kt, flags, len, nt);
+      to[1] = make_int4(start, n, h, rt);
+      if (end) {
+        // this worker joins the unit that starts in its range and goes on behind it
+        Meta mt;
+        mt.pieces = kt0 == 0 && kt + 1 < nt ? 1 + (int)((at + (nt - 1 - kt)) / per) - worker : 0;
+        mt.slot = in_first ? 0 : 1;
+        mt.start = start;
+        mt.rows = n * plan.group;
+        mt.h = h;
+        mt.rt = rt;
+        meta[worker] = mt;
+      }
+    }
+    if (t >= 2) {                // two tiles stay on their way
+      copy_wait<2>();
+      signal(t - 1);
+    }
+  }
+  copy_wait<0>();
+  if (end) signal(t);
+}
+
+// ------------------------------------------------------------------ the issuer
+
+template <bool kBF16>
+__device__ __forceinline__ void issue_warp(Group& gm, Control& ct, uint32_t tmem) {
+  volatile int* ab = &ct.gave_up;
+  const uint32_t id_s = make_idesc(BR, TK, kBF16, false), id_o = make_idesc(BR, 64, kBF16, true);
+  const uint32_t q0 = smem_u32(gm.q), k0 = smem_u32(gm.k), v0 = smem_u32(gm.v);
+  int issued = 0;
+  bool more = true, good = true;
+  // S of tile `issued` into its region; its rows are there
+  auto issue_s = [&]() {
+    const int st = issued % NST, flags = ct.ring[issued % RING].flags;
+    if (flags & kNone) {
+      more = false;
+      return;
+    }
+    more = !(flags & kEnd);
+    const uint64_t qd = sdesc_sw128(q0 + (flags & kQ1 ? Q_BYTES : 0), 16, 1024);
+    const uint64_t kd = sdesc_sw128(k0 + st * KV_BYTES, 16, 1024);
+    tc_fence_after();
+#pragma unroll
+    for (int kk = 0; kk < 4; ++kk)
+      mma_ss(tmem + TK * (issued % NREG), qd + 2 * kk, kd + 2 * kk, id_s, kk > 0 ? 1u : 0u);
+    mma_commit(&ct.s_full[issued % NREG]);
+    ++issued;
+  };
+  // scores up to three tiles ahead of the weights, as far as rows are there.  Only where no weights are
+  // awaited may this wait for them: the loader itself waits for a unit's last products before it
+  // overwrites its Q, and with units of one tile those are the next that this warp issues.
+  auto scores = [&](int upto, int awaited) {
+    while (more && good && issued < upto) {
+      uint64_t* bar = &ct.full[issued % NST];
+      const uint32_t parity = (issued / NST) & 1;
+      if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+        if (issued > awaited) return;
+        good = mbar_wait_warp(bar, parity, ab);
+        if (!good) return;
+      }
+      issue_s();
+    }
+  };
+  scores(NREG, 0);
+  for (int t = 0; good && t < issued; ++t) {
+    good = mbar_wait_warp(&ct.p_ready[t % NREG], (t / NREG) & 1, ab);
+    if (!good) break;
+    const int st = t % NST;
+    const bool first = ct.ring[t % RING].flags & kFirst;
+    const uint64_t vd = sdesc_sw128(v0 + st * KV_BYTES, 16384, 1024);
+    const uint32_t p = tmem + TK * (t % NREG);
+    tc_fence_after();
+#pragma unroll
+    for (int part = 0; part < 2; ++part)
+#pragma unroll
+      for (int kk = 0; kk < TK / 16; ++kk)
+        mma_ts(tmem + COL_O, p + 16 * kk + 8 * part, vd + 128 * kk, id_o, first && part == 0 && kk == 0 ? 0u : 1u);
+    mma_commit(&ct.pv_done[t & 1]);
+    mma_commit(&ct.free_[st]);
+    scores(t + 1 + NREG, t + 1);
+  }
+  if (!good) {
+    // products may still be running: they end before tensor memory is given back
+    volatile int go = 0;
+    mma_commit(&ct.drained);
+    mbar_wait_warp(&ct.drained, 0, &go);
+  }
+}
+
+// ------------------------------------------------------------------ the math warps
+
+template <typename T>
+__device__ __forceinline__ void math_warp(const Args& a, const Plan& plan, int worker, Group& gm, Control& ct,
+                                          uint32_t tmem, float* __restrict__ part_o, float2* __restrict__ part_mz) {
+  volatile int* ab = &ct.gave_up;
+  const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, r = warp * 32 + lane;
+  const uint32_t lanes = (uint32_t)(warp * 32) << 16, t_o = tmem + COL_O + lanes;
+  float m = -INFINITY, carry_s = kMasked, carry_b = 0.f, scale = 0.f;
+  float2 z2 = splat2(0.f);
+  int pos = -1, i_min = 0, i_max = -1, kt0 = 0, bad = 0;
+  bool in_first = true, first_tile = true;
+  for (int t = 0;; ++t) {
+    if (!mbar_wait_warp(&ct.full[t % NST], (t / NST) & 1, ab)) return;
+    const Slot& d = ct.ring[t % RING];
+    const int4 head = *reinterpret_cast<const int4*>(&d);
+    const int kt = head.x, flags = head.y, base = kt * TK;
+    if (flags & kNone) return;
+    if (flags & kFirst) {
+      kt0 = kt;
+      bad = 0;
+      in_first = first_tile;
+      first_tile = false;
+      const int rows = d.n * plan.group, row0 = d.rt * BR + warp * 32, lead = head.z - d.n;
+      const int row_last = min(rows, row0 + 32) - 1;          // < row0: the warp has no row
+      i_min = lead + row0 / plan.group;
+      i_max = row_last >= row0 ? lead + row_last / plan.group : -1;
+      const int row = max(min(row0 + lane, row_last), 0);
+      const int tk = row / plan.group;
+      pos = lead + tk;
+      scale = expf(a.log_gain[d.h * plan.group + row - tk * plan.group]) * a.inv_sqrt_d;
+      m = -INFINITY;
+      z2 = splat2(0.f);
+      carry_s = kMasked;
+      carry_b = 0.f;
+      if (kt > 0 && base - 1 <= i_max) {
+        // the score of the key before the piece, this row's
+        const uint8_t* q = gm.q[flags & kQ1 ? 1 : 0] + r * 128;
+        float2 s = splat2(0.f);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const uint4 x = *reinterpret_cast<const uint4*>(q + ((c ^ (r & 7)) << 4));
+          const uint4 y = *reinterpret_cast<const uint4*>(d.k_before + 16 * c);
+          s = fma2(unpack2<T>(x.x), unpack2<T>(y.x), s);
+          s = fma2(unpack2<T>(x.y), unpack2<T>(y.y), s);
+          s = fma2(unpack2<T>(x.z), unpack2<T>(y.z), s);
+          s = fma2(unpack2<T>(x.w), unpack2<T>(y.w), s);
+        }
+        if (base - 1 <= pos) m = carry_s = (s.x + s.y) * scale;
+      }
+    }
+    bad |= flags & kBad;
+    if (!mbar_wait_warp(&ct.s_full[t % NREG], (t / NREG) & 1, ab)) return;
+    tc_fence_after();
+    const uint32_t t_s = tmem + TK * (t % NREG) + lanes;
+    if (base - 1 <= i_max && i_max >= 0) {
+      uint32_t raw[32];
+      tmem_ld32(t_s, raw);
+      tmem_ld_wait();
+      tmem_reg_fence(raw);
+      float2 s[2][8];
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        s[j >> 3][j & 7] = mul2(make_float2(__uint_as_float(raw[2 * j]), __uint_as_float(raw[2 * j + 1])), splat2(scale));
+      const bool edge = base == 0 || base + TK - 1 > i_min;     // keys beyond a row's own, or caps
+      if (edge) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int key = base + 16 * (j >> 3) + (j & 7);
+          if (key > pos) s[j >> 3][j & 7].x = kMasked;
+          if (key + 8 > pos) s[j >> 3][j & 7].y = kMasked;
+        }
+      }
+      float top = max3f(s[0][0].x, s[0][0].y, s[0][1].x);
+      top = fmaxf(top, s[0][1].y);
+#pragma unroll
+      for (int j = 2; j < 16; ++j) top = max3f(top, s[j >> 3][j & 7].x, s[j >> 3][j & 7].y);
+      const bool move = top > kMasked && top > m + kRescaleNats;
+      if (__any_sync(0xffffffffu, move)) {
+        const float to = move ? top : m, f = move ? exp_rel(m - to) : 1.f;
+        m = to;
+        carry_b *= f;
+        z2 = mul2(z2, splat2(f));
+        if (!(flags & kFirst)) {
+          // O holds P V of the piece's tiles so far: the last of them has to have landed.  Its barrier is
+          // neither a phase further on (that needs P of tile t + 1) nor behind (P V of tile t - 3
+          // completed before the scores of tile t)
+          if (!mbar_wait_warp(&ct.pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1, ab)) return;
+          tc_fence_after();
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            uint32_t o[32];
+            tmem_ld32(t_o + 32 * half, o);
+            tmem_ld_wait();
+            tmem_reg_fence(o);
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+            tmem_st32(t_o + 32 * half, o);
+          }
+          tmem_st_wait();
+        }
+      }
+      const float m2 = m == -INFINITY ? 0.f : m * kLog2e;
+      const int lowest = flags & kFirst ? base : base - 1;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t hi[8], lo[8];
+        float2 lead;
+        float last;
+        weigh<T, 8>(s[c], m2, carry_s, edge, base + 16 * c, pos, lowest, hi, lo, lead, last, z2);
+        lead.x += carry_b;
+        split2<T>(lead, hi[0], lo[0]);
+        carry_s = s[c][7].y;
+        carry_b = last;
+        tmem_st8(t_s + 16 * c, hi);
+        tmem_st8(t_s + 16 * c + 8, lo);
+      }
+    } else if (i_max >= 0) {
+      // no row of this warp sees a segment or a weight here
+      uint32_t zero[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_st8(t_s + 8 * c, zero);
+    }
+    tmem_st_wait();
+    tc_fence_before();
+    mbar_arrive_warp(&ct.p_ready[t % NREG]);
+
+    if (flags & kLast) {
+      // (P V of tile t - 1 first: only then can this tile's phase be told from the one before)
+      if (t > 0 && !mbar_wait_warp(&ct.pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1, ab)) return;
+      if (!mbar_wait_warp(&ct.pv_done[t & 1], (t >> 1) & 1, ab)) return;
+      tc_fence_after();
+      uint32_t o[2][32];
+      tmem_ld32(t_o, o[0]);
+      tmem_ld32(t_o + 32, o[1]);
+      tmem_ld_wait();
+      tmem_reg_fence(o[0]);
+      tmem_reg_fence(o[1]);
+      tc_fence_before();
+      const int rows = d.n * plan.group, row = d.rt * BR + r;
+      if (row < rows) {
+        const bool whole = kt0 == 0 && kt + 1 == head.w;
+        const int key = base + TK - 1;                      // the key whose weight is still carried
+        const float m2 = m == -INFINITY ? 0.f : m * kLog2e;
+        const float cap = key == pos ? 0.5f * ex2_approx(fmaf(carry_s, kLog2e, -m2)) : 0.f;
+        // beyond the row's own key the weight is 0, and V may hold anything
+        const float w = key <= pos ? carry_b + cap : 0.f;
+        float z = z2.x + z2.y + cap;
+        if (bad) z = __int_as_float(0x7fffffff);
+        const float inv = 1.f / z;
+        const long long prow = ((long long)worker * 2 + (in_first ? 0 : 1)) * BR + r;
+        const int tk = row / plan.group;
+        T* dst = (T*)a.o + ((size_t)(d.start + tk) * a.H + (size_t)d.h * plan.group + (row - tk * plan.group)) * a.D;
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          float y[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) y[x] = __uint_as_float(o[(8 * c + x) >> 5][(8 * c + x) & 31]);
+          if (w != 0.f) {
+            const uint4 v = *reinterpret_cast<const uint4*>(d.v_last + 16 * c);
+            const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const float2 vv = unpack2<T>(vw[x]);
+              y[2 * x] = fmaf(w, vv.x, y[2 * x]);
+              y[2 * x + 1] = fmaf(w, vv.y, y[2 * x + 1]);
+            }
+          }
+          if (!whole) {
+            *reinterpret_cast<float4*>(part_o + prow * 64 + 8 * c) = make_float4(y[0], y[1], y[2], y[3]);
+            *reinterpret_cast<float4*>(part_o + prow * 64 + 8 * c + 4) = make_float4(y[4], y[5], y[6], y[7]);
+          } else if (8 * c < a.D) {
+            // z = 0: the row sees no key
+            const bool none = z == 0.f;
+            *reinterpret_cast<uint4*>(dst + 8 * c) =
+                none ? make_uint4(0u, 0u, 0u, 0u)
+                     : make_uint4(pack2<T>(y[0] * inv, y[1] * inv), pack2<T>(y[2] * inv, y[3] * inv),
+                                  pack2<T>(y[4] * inv, y[5] * inv), pack2<T>(y[6] * inv, y[7] * inv));
+          }
+        }
+        if (!whole) part_mz[prow] = make_float2(m, z);
+      }
+      __syncwarp();
+    }
+    if (flags & kEnd) return;
+  }
+}
+
+// ------------------------------------------------------------------ the kernel
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS, 1)
+    tc_kernel(const __grid_constant__ Args a, const __grid_constant__ Plan plan, float* __restrict__ part_o,
+              float2* __restrict__ part_mz, Meta* __restrict__ meta) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  pdl_wait();
+  pdl_launch_dependents();
+  Group* groups = reinterpret_cast<Group*>(smem);
+  Control* controls = reinterpret_cast<Control*>(smem + GROUPS * sizeof(Group));
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + GROUPS * (sizeof(Group) + sizeof(Control)));
+  unsigned* prefix = reinterpret_cast<unsigned*>(smem + kSmem);
+  const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int role = wid < MATH_WARPS ? 0 : wid < MATH_WARPS + 4 ? 1 : 2;
+  const int group = role == 0 ? wid >> 2 : wid & 3;
+
+  if (role == 2 && group < GROUPS && lane == 0) {
+    Control& ct = controls[group];
+    for (int i = 0; i < NST; ++i) {
+      mbar_init(&ct.full[i], 1);
+      mbar_init(&ct.free_[i], 1);
+    }
+    for (int i = 0; i < NREG; ++i) {
+      mbar_init(&ct.s_full[i], 1);
+      mbar_init(&ct.p_ready[i], 4);
+    }
+    for (int i = 0; i < 2; ++i) mbar_init(&ct.pv_done[i], 1);
+    mbar_init(&ct.drained, 1);
+    ct.gave_up = 0;
+    fence_mbar_init();
+  }
+  if (role == 1 && group == 3) {
+    tmem_alloc(tmem_at, 512);
+    tmem_relinquish();
+  }
+  Schedule<BR, TK> sched(a, plan, prefix);   // a barrier of the block among other things
+  tc_fence_after();
+  const uint32_t tmem = *tmem_at + COLS * (group < GROUPS ? group : 0);
+  const unsigned total = sched.total;
+  const int worker = blockIdx.x * GROUPS + group, workers = gridDim.x * GROUPS;
+  const unsigned per = plan.places_per_worker(total, workers);
+
+  if (role == 0) {
+    regs_up<REGS_MATH>();
+    math_warp<T>(a, plan, worker, groups[group], controls[group], tmem, part_o, part_mz);
+  } else {
+    regs_down<REGS_OTHER>();
+    if (group < GROUPS) {
+      if (role == 1) {
+        issue_warp<sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value>(groups[group], controls[group], tmem);
+      } else {
+        const unsigned x0 = (unsigned)min((unsigned long long)worker * per, (unsigned long long)total);
+        const unsigned x1 = (unsigned)min((unsigned long long)x0 + per, (unsigned long long)total);
+        load_warp<T>(a, plan, sched, worker, per, x0, x1, groups[group], controls[group], meta);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (role == 1 && group == 3) {
+    tc_fence_after();
+    tmem_dealloc(*tmem_at, 512);
+  }
+}
+
+}  // namespace
+
+int tc_br() { return BR; }
+int tc_groups() { return GROUPS; }
+
+cudaError_t tc_launch(const Args& a, const Plan& plan, int dtype, const Pieces& pc) {
+  static_assert(kSmem + (kMaxSeqs + 1) * sizeof(unsigned) <= 232448, "shared memory of a block");
+  auto kern = dtype == 1 ? tc_kernel<__nv_bfloat16> : tc_kernel<__half>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       (int)(kSmem + (kMaxSeqs + 1) * sizeof(unsigned)));
+  if (e != cudaSuccess) return e;
+  const size_t smem = kSmem + (size_t)(a.seqs + 1) * sizeof(unsigned);
+  return launch_pdl(kern, dim3(num_sms_cached()), dim3(THREADS), smem, a.stream, a, plan, pc.o, pc.mz, pc.meta);
+}
+
+cudaError_t tc_read_status(int* out, bool reset) {
+  int word[2] = {0, 0};
+  cudaError_t e = cudaMemcpyFromSymbol(&word[0], g_status, sizeof(int));
+  if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&word[1], sm100::g_device_status, sizeof(int));
+  if (e != cudaSuccess) return e;
+  *out = word[1] ? word[1] : word[0];
+  if (!reset || *out == 0) return e;
+  const int zero = 0;
+  e = cudaMemcpyToSymbol(g_status, &zero, sizeof(int));
+  return e != cudaSuccess ? e : cudaMemcpyToSymbol(sm100::g_device_status, &zero, sizeof(int));
+}
+
+}  // namespace paged
+}  // namespace ca

@@ -16,8 +16,8 @@ namespace ca {
 namespace sm100 {
 
 // Kernels record CA_ERR_DEVICE_TIMEOUT (5) here when a bounded wait gives up.
-// Defined here: this header is included by exactly one translation unit (ca_sm100.cu).
-__device__ int g_device_status = 0;
+// One word per source file that includes this; read_device_status() reads them all.
+static __device__ int g_device_status = 0;
 
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // 2 s per wait
 
