@@ -78,6 +78,13 @@ __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.al
 template <int N>
 __device__ __forceinline__ void regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
+// whether the phase has completed, at once (a try_wait may sleep for microseconds before it says no); whole warp
+__device__ __forceinline__ bool mbar_test_warp(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+               "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  return __all_sync(0xffffffffu, done != 0);
+}
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool zero) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(zero ? 0 : 16) : "memory");
 }
@@ -137,7 +144,7 @@ __device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const
   int t = 0;
   for (; !end; ++t) {
     const int st = t % NST;
-    if (t >= NST && !__all_sync(0xffffffffu, mbar_try_wait(&ct.free_[st], (t / NST - 1) & 1))) {
+    if (t >= NST && !mbar_test_warp(&ct.free_[st], (t / NST - 1) & 1)) {
       // the readers may be waiting for tiles that are there but not signalled
       copy_wait<0>();
       signal(t);
@@ -154,7 +161,7 @@ __device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const
       // Q of the unit before the last one lay in this buffer: its products have to be done (they are known to
       // be where the stage of its last tile has been filled again since)
       const int u = last_tile[1];
-      if (u >= 0 && u + NST > t && !__all_sync(0xffffffffu, mbar_try_wait(&ct.free_[u % NST], (u / NST) & 1))) {
+      if (u >= 0 && u + NST > t && !mbar_test_warp(&ct.free_[u % NST], (u / NST) & 1)) {
         copy_wait<0>();
         signal(t);
         if (!mbar_wait_warp(&ct.free_[u % NST], (u / NST) & 1, ab)) break;
@@ -286,7 +293,7 @@ __device__ __forceinline__ void issue_warp(Group& gm, Control& ct, uint32_t tmem
     while (more && good && issued < upto) {
       uint64_t* bar = &ct.full[issued % NST];
       const uint32_t parity = (issued / NST) & 1;
-      if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) {
+      if (!mbar_test_warp(bar, parity)) {
         if (issued > awaited) return;
         good = mbar_wait_warp(bar, parity, ab);
         if (!good) return;
