@@ -66,7 +66,8 @@ cudaError_t simt_read_status(int* out, bool reset);
 struct Pieces;
 int tc_br();
 int tc_groups();
-cudaError_t tc_launch(const Args& a, const Plan& plan, int dtype, const Pieces& pc);
+// false where the caches' strides do not suit it: nothing was launched
+bool tc_launch(const Args& a, const Plan& plan, int dtype, const Pieces& pc, cudaError_t& e);
 cudaError_t tc_read_status(int* out, bool reset);
 
 // Prefix sums of the sequences' places in shared memory (all threads of the block take part in the

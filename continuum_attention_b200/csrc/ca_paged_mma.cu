@@ -738,11 +738,14 @@ cudaError_t forward_dp(const Args& a, void* workspace) {
   chunks.row_lo = 17;
   // (a single sequence is all in one form, whatever its rows)
   if (a.seqs == 1) chunks.row_lo = 0;
-  const bool tc = use_tc(rows, DP);
-  const int br = tc ? tc_br() : Chunk<DP>::BR, groups = tc ? tc_groups() : Chunk<DP>::GROUPS;
-  const Pieces pc = carve<DP>(ws, br, groups);
-  cudaError_t e = tc ? tc_launch(a, chunks, sizeof(T) == 2 && std::is_same_v<T, __nv_bfloat16> ? 1 : 2, pc)
-                     : launch_main<T, Chunk<DP>>(a, chunks, pc, false);
+  const bool wide = use_tc(rows, DP);
+  const int br = wide ? tc_br() : Chunk<DP>::BR, groups = wide ? tc_groups() : Chunk<DP>::GROUPS;
+  Pieces pc = carve<DP>(ws, br, groups);
+  cudaError_t e;
+  if (!wide || !tc_launch(a, chunks, std::is_same_v<T, __nv_bfloat16> ? 1 : 2, pc, e)) {
+    pc = carve<DP>(ws, Chunk<DP>::BR, Chunk<DP>::GROUPS);   // its units are the smaller ones
+    e = launch_main<T, Chunk<DP>>(a, chunks, pc, false);
+  }
   if (e != cudaSuccess) return e;
   if (a.seqs == 1) return launch_merge<T, DP>(a, plan, pc, Pieces{});
   plan.row_hi = 16;

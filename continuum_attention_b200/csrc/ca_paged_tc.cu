@@ -25,6 +25,10 @@
 //
 // Against the mma.sync form the products take no issue slots of the math warps, and O no
 // registers, which leaves room for three math warps on a scheduler and less work in each.
+#include <cuda.h>
+
+#include <numeric>
+
 #include "ca_common.cuh"
 #include "ca_paged.cuh"
 #include "ca_paged_math.cuh"
@@ -85,19 +89,26 @@ __device__ __forceinline__ bool mbar_test_warp(uint64_t* bar, uint32_t parity) {
                "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
   return __all_sync(0xffffffffu, done != 0);
 }
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool zero) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(zero ? 0 : 16) : "memory");
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar) : "memory");
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// The caches and q as 2-D maps of rows: the strides' greatest common divisor apart, so that a row's number
+// is a sum of products of small integers, whatever the strides.
+struct Maps {
+  CUtensorMap q, k, v;
+  int q_token, q_head;               // rows between tokens, heads
+  int page, slot, head;              // rows between pages, slots, key heads
+  long long unit;                    // values between a cache's rows
+};
 
 // ------------------------------------------------------------------ the loader
 
 template <typename T>
-__device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const Schedule<BR, TK>& sched, int worker,
-                                          unsigned per, unsigned x0, unsigned x1, Group& gm, Control& ct,
-                                          Meta* __restrict__ meta) {
+__device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const Maps& maps,
+                                          const Schedule<BR, TK>& sched, int worker, unsigned per, unsigned x0,
+                                          unsigned x1, Group& gm, Control& ct, Meta* __restrict__ meta) {
   const int lane = threadIdx.x & 31;
   volatile int* ab = &ct.gave_up;
   typename Schedule<BR, TK>::Cursor cur;
@@ -111,116 +122,71 @@ __device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const
     }
     return;
   }
-  const uint32_t qs = smem_u32(gm.q), ks = smem_u32(gm.k), vs = smem_u32(gm.v);
-  const int row8 = lane >> 3, ch = lane & 7;          // a copy instruction: 4 rows of 8 chunks
-  const bool pad = ch * 8 >= a.D;
-  const T* kb = (const T*)a.k_cache + ch * 8;
-  const T* vb = (const T*)a.v_cache + ch * 8;
-
   auto page_at = [&](int key) {                       // of this sequence, -1 beyond its keys
     return key < cur.len ? a.page_table[(size_t)cur.s * a.page_table_stride + plan.page_of(key)] : -1;
   };
-  auto offset = [&](int page, int key, int h) {
-    return (long long)page * a.page_stride + (long long)h * a.head_stride +
-           (long long)(key - plan.page_of(key) * a.page_size) * a.slot_stride;
+  auto row_of = [&](int page, int key, int h) {       // of the maps
+    return page * maps.page + (key - plan.page_of(key) * a.page_size) * maps.slot + h * maps.head;
   };
-
-  int done = 0;                  // tiles signalled
-  // the oldest tiles' copies are there: tell the readers of tiles done .. upto - 1
-  auto signal = [&](int upto) {
-    fence_proxy_async_smem();
-    __syncwarp();
-    for (; done < upto; ++done)
-      if (lane == 0) mbar_arrive(&ct.full[done % NST]);
-  };
+  // this lane's four rows of the stage: lanes 0 .. 7 of K, 8 .. 15 of V.  Row r is the key at
+  // 16 (r / 16) + (r % 16) / 2 + 8 (r % 2): K of it, V of the key before it
+  const bool is_v = lane >= 8;
+  const uint32_t dst = (is_v ? smem_u32(gm.v) : smem_u32(gm.k)) + (lane & 7) * 512;
+  const int p0 = ((lane & 4) << 2) + ((lane & 3) << 1);    // of its first row: + 0, 8, 1, 9 for the four
+  const CUtensorMap* map = is_v ? &maps.v : &maps.k;
+  const uint32_t row_bytes = a.D * sizeof(T);
 
   bool first = true, in_first = true;
   int kt0 = 0, qbuf = 1;
   int last_tile[2] = {-1, -1};   // the last tiles of the units before this one and before that
-  long long before = -1;         // the row of the key before the tile (-1: none)
+  int before = -1;               // the row of the key before the tile (-1: none)
   int pg = page_at(cur.kt * TK + lane);
   int pg_before = cur.kt > 0 ? page_at(cur.kt * TK - 1) : -1;
   bool end = false;
   int t = 0;
   for (; !end; ++t) {
     const int st = t % NST;
-    if (t >= NST && !mbar_test_warp(&ct.free_[st], (t / NST - 1) & 1)) {
-      // the readers may be waiting for tiles that are there but not signalled
-      copy_wait<0>();
-      signal(t);
-      if (!mbar_wait_warp(&ct.free_[st], (t / NST - 1) & 1, ab)) break;
-    }
+    if (t >= NST && !mbar_wait_warp(&ct.free_[st], (t / NST - 1) & 1, ab)) break;
     const int base = cur.kt * TK;
     const bool opens = first || cur.kt == 0;
     int flags = cur.bad ? kBad : 0;
+    Slot& slot = ct.ring[t % RING];
+    const uint32_t bar = smem_u32(&ct.full[st]);
+    uint32_t bytes = 2 * KV_BYTES;
+    const int key = base + lane;
+    bool bad = key < cur.len && (pg < 0 || pg >= a.num_pages);
+    const int row = key < cur.len && !bad ? row_of(pg, key, cur.h) : -1;
     if (opens) {
       flags |= kFirst;
       kt0 = cur.kt;
       in_first = first;
+      first = false;
       qbuf ^= 1;
       // Q of the unit before the last one lay in this buffer: its products have to be done (they are known to
       // be where the stage of its last tile has been filled again since)
       const int u = last_tile[1];
-      if (u >= 0 && u + NST > t && !mbar_test_warp(&ct.free_[u % NST], (u / NST) & 1)) {
-        copy_wait<0>();
-        signal(t);
-        if (!mbar_wait_warp(&ct.free_[u % NST], (u / NST) & 1, ab)) break;
-      }
-      const int rows = cur.n * plan.group, row0 = cur.rt * BR;
-#pragma unroll 4
-      for (int r0 = 0; r0 < BR; r0 += 4) {
-        const int r = r0 + row8, row = row0 + r;
-        const bool none = row >= rows || pad;
-        const int tk = none ? 0 : row / plan.group;
-        const T* src = (const T*)a.q + (none ? 0 : (size_t)(cur.start + tk) * a.q_token_stride +
-                                                        (size_t)(cur.h * plan.group + row - tk * plan.group) *
-                                                            a.q_head_stride + ch * 8);
-        copy16(qs + qbuf * Q_BYTES + r * 128 + ((ch ^ (r & 7)) << 4), src, none);
-      }
-    }
-    if (qbuf) flags |= kQ1;
-    Slot& slot = ct.ring[t % RING];
-
-    // this lane's key, and the one before the tile
-    const int key = base + lane;
-    bool bad = key < cur.len && (pg < 0 || pg >= a.num_pages);
-    const long long off = key < cur.len && !bad ? offset(pg, key, cur.h) : -1;
-    if (opens) {
+      if (u >= 0 && u + NST > t && !mbar_wait_warp(&ct.free_[u % NST], (u / NST) & 1, ab)) break;
+      bytes += Q_BYTES;
       before = -1;
       if (base > 0 && base - 1 < cur.len) {
         if (pg_before < 0 || pg_before >= a.num_pages) bad = true;
-        else before = offset(pg_before, base - 1, cur.h);
+        else before = row_of(pg_before, base - 1, cur.h);
       }
-      if (lane < 8 && base > 0)
-        copy16(smem_u32(slot.k_before) + ch * 16, before < 0 ? (const T*)a.k_cache : kb + before, before < 0 || pad);
+      if (before >= 0) bytes += row_bytes;
     }
-    // row r of the stage is the key at 16 (r / 16) + (r % 16) / 2 + 8 (r % 2): K of it, V of the key before it
-#pragma unroll
-    for (int r0 = 0; r0 < TK; r0 += 4) {
-      const int r = r0 + row8;
-      const int p = (r & 16) + ((r & 15) >> 1) + ((r & 1) << 3);
-      const long long ko = __shfl_sync(0xffffffffu, off, p);
-      long long vo = __shfl_sync(0xffffffffu, off, (p + 31) & 31);
-      if (p == 0) vo = before;
-      const uint32_t dst = st * KV_BYTES + r * 128 + ((ch ^ (r & 7)) << 4);
-      copy16(ks + dst, ko < 0 ? (const T*)a.k_cache : kb + ko, ko < 0 || pad);
-      copy16(vs + dst, vo < 0 ? (const T*)a.v_cache : vb + vo, vo < 0 || pad);
-    }
-    before = __shfl_sync(0xffffffffu, off, 31);
-
-    const int kt = cur.kt, nt = cur.nt, start = cur.start, n = cur.n, len = cur.len, h = cur.h, rt = cur.rt;
+    if (qbuf) flags |= kQ1;
+    bad = __any_sync(0xffffffffu, bad);
+    if (bad) flags |= kBad;
+    const int behind = __shfl_sync(0xffffffffu, row, 31);
     const unsigned at = cur.at;
     bool more = at + 1 < x1;
-    const bool closes = !more || cur.kt + 1 == cur.nt;
-    if (closes) {
+    if (!more || cur.kt + 1 == cur.nt) {
       flags |= kLast;
-      if (lane < 8)
-        copy16(smem_u32(slot.v_last) + ch * 16, before < 0 ? (const T*)a.v_cache : vb + before, before < 0 || pad);
       last_tile[1] = last_tile[0];
       last_tile[0] = t;
+      if (behind >= 0) bytes += row_bytes;
     }
-    copy_commit();
-    first = false;
+    const int kt = cur.kt, nt = cur.nt, start = cur.start, n = cur.n, len = cur.len, h = cur.h, rt = cur.rt;
     if (more) {
       sched.advance(cur);
       more = cur.at < x1;        // the next unit's first tile may lie behind the range
@@ -232,8 +198,6 @@ __device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const
       flags |= kEnd;
       end = true;
     }
-    bad = __any_sync(0xffffffffu, bad);
-    if (bad) flags |= kBad;
     if (lane == 0) {
       if (bad) record_invalid();
       int4* to = reinterpret_cast<int4*>(&slot);
@@ -251,13 +215,34 @@ __device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const
         meta[worker] = mt;
       }
     }
-    if (t >= 2) {                // two tiles stay on their way
-      copy_wait<2>();
-      signal(t - 1);
+    mbar_arrive_expect_tx(&ct.full[st], bytes);
+    __syncwarp();
+    int r[4];
+#pragma unroll
+    for (int x = 0; x < 4; ++x) {
+      const int p = p0 + (x >> 1) + 8 * (x & 1) - (is_v ? 1 : 0);
+      r[x] = __shfl_sync(0xffffffffu, row, p & 31);
+      if (p < 0) r[x] = before;
     }
+    if (lane < 16) tma_gather4(dst + st * KV_BYTES, map, bar, r[0], r[1], r[2], r[3]);
+    if (opens) {
+      const int rows = n * plan.group;
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int i = rt * BR + 4 * lane + x, tk = i / plan.group;
+        r[x] = i < rows ? (start + tk) * maps.q_token + (h * plan.group + i - tk * plan.group) * maps.q_head : -1;
+      }
+      tma_gather4(smem_u32(gm.q[qbuf]) + lane * 512, &maps.q, bar, r[0], r[1], r[2], r[3]);
+      if (lane == 0 && before >= 0)
+        bulk_load(smem_u32(slot.k_before), (const T*)a.k_cache + before * maps.unit, row_bytes, bar);
+    }
+    if (lane == 0 && (flags & kLast) && behind >= 0)
+      bulk_load(smem_u32(slot.v_last), (const T*)a.v_cache + behind * maps.unit, row_bytes, bar);
+    before = behind;
   }
-  copy_wait<0>();
-  if (end) signal(t);
+  // every copy has to land before this block's shared memory is another's
+  volatile int go = 0;
+  for (int u = max(t - NST, 0); u < t; ++u) mbar_wait_warp(&ct.full[u % NST], (u / NST) & 1, &go);
 }
 
 // ------------------------------------------------------------------ the issuer
@@ -519,8 +504,8 @@ __device__ __forceinline__ void math_warp(const Args& a, const Plan& plan, int w
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS, 1)
-    tc_kernel(const __grid_constant__ Args a, const __grid_constant__ Plan plan, float* __restrict__ part_o,
-              float2* __restrict__ part_mz, Meta* __restrict__ meta) {
+    tc_kernel(const __grid_constant__ Args a, const __grid_constant__ Plan plan, const __grid_constant__ Maps maps,
+              float* __restrict__ part_o, float2* __restrict__ part_mz, Meta* __restrict__ meta) {
   extern __shared__ __align__(1024) uint8_t smem[];
   pdl_wait();
   pdl_launch_dependents();
@@ -532,8 +517,20 @@ __global__ void __launch_bounds__(THREADS, 1)
   const int role = wid < MATH_WARPS ? 0 : wid < MATH_WARPS + 4 ? 1 : 2;
   const int group = role == 0 ? wid >> 2 : wid & 3;
 
+  if (role == 2 && group < GROUPS) {
+    // values behind D stay 0 (copies write D values a row)
+    Control& ct = controls[group];
+    for (int x = lane; x < RING * 8; x += 32) {
+      reinterpret_cast<uint4*>(ct.ring[x >> 3].k_before)[x & 7] = make_uint4(0u, 0u, 0u, 0u);
+      reinterpret_cast<uint4*>(ct.ring[x >> 3].v_last)[x & 7] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    fence_proxy_async_smem();
+  }
   if (role == 2 && group < GROUPS && lane == 0) {
     Control& ct = controls[group];
+    tma_prefetch_desc(&maps.q);
+    tma_prefetch_desc(&maps.k);
+    tma_prefetch_desc(&maps.v);
     for (int i = 0; i < NST; ++i) {
       mbar_init(&ct.full[i], 1);
       mbar_init(&ct.free_[i], 1);
@@ -569,7 +566,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       } else {
         const unsigned x0 = (unsigned)min((unsigned long long)worker * per, (unsigned long long)total);
         const unsigned x1 = (unsigned)min((unsigned long long)x0 + per, (unsigned long long)total);
-        load_warp<T>(a, plan, sched, worker, per, x0, x1, groups[group], controls[group], meta);
+        load_warp<T>(a, plan, maps, sched, worker, per, x0, x1, groups[group], controls[group], meta);
       }
     }
   }
@@ -586,14 +583,75 @@ __global__ void __launch_bounds__(THREADS, 1)
 int tc_br() { return BR; }
 int tc_groups() { return GROUPS; }
 
-cudaError_t tc_launch(const Args& a, const Plan& plan, int dtype, const Pieces& pc) {
+namespace {
+
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                             const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode_fn() {
+  static EncodeFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                    q == cudaDriverEntryPointSuccess;
+    return ok ? reinterpret_cast<EncodeFn>(p) : nullptr;
+  }();
+  return fn;
+}
+
+struct Axis {
+  long long count, stride;
+};
+
+// a map of rows of D values over the places that the axes reach, and how many rows a step along each is;
+// false where the rows are too many for a coordinate
+template <int N>
+bool make_rows(CUtensorMap* map, const void* base, long long D, bool bf16, const Axis (&axes)[N], int* const (&step)[N],
+               long long* unit) {
+  long long g = 0, rows = 1;
+  for (const Axis& x : axes) g = x.count > 1 ? std::gcd(g, x.stride) : g;
+  if (g == 0) g = D;
+  for (int i = 0; i < N; ++i) {
+    const long long s = axes[i].count > 1 ? axes[i].stride / g : 0;
+    if (s > 0x7fffffffll) return false;
+    *step[i] = (int)s;
+    rows += (axes[i].count - 1) * s;           // (counts are below 2^31)
+    if (rows > 0x7fffffffll) return false;
+  }
+  *unit = g;
+  const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)rows}, pitch[1] = {(cuuint64_t)(g * 2)};
+  const cuuint32_t box[2] = {64, 1}, one[2] = {1, 1};
+  return encode_fn()(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2,
+                     const_cast<void*>(base), dims, pitch, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool make_maps(const Args& a, bool bf16, Maps& m) {
+  if (!encode_fn() || a.num_pages < 1 || a.rows < 1) return false;
+  long long q_unit;
+  return make_rows(&m.q, a.q, a.D, bf16, {Axis{a.rows, a.q_token_stride}, {a.H, a.q_head_stride}},
+                   {&m.q_token, &m.q_head}, &q_unit) &&
+         make_rows(&m.k, a.k_cache, a.D, bf16, {Axis{a.num_pages, a.page_stride}, {a.page_size, a.slot_stride}, {a.G, a.head_stride}},
+                   {&m.page, &m.slot, &m.head}, &m.unit) &&
+         make_rows(&m.v, a.v_cache, a.D, bf16, {Axis{a.num_pages, a.page_stride}, {a.page_size, a.slot_stride}, {a.G, a.head_stride}},
+                   {&m.page, &m.slot, &m.head}, &m.unit);
+}
+
+}  // namespace
+
+bool tc_launch(const Args& a, const Plan& plan, int dtype, const Pieces& pc, cudaError_t& e) {
+  Maps maps;
+  if (!make_maps(a, dtype == 1, maps)) return false;
   static_assert(kSmem + (kMaxSeqs + 1) * sizeof(unsigned) <= 232448, "shared memory of a block");
   auto kern = dtype == 1 ? tc_kernel<__nv_bfloat16> : tc_kernel<__half>;
-  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)(kSmem + (kMaxSeqs + 1) * sizeof(unsigned)));
-  if (e != cudaSuccess) return e;
+  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                           (int)(kSmem + (kMaxSeqs + 1) * sizeof(unsigned)));
+  if (e != cudaSuccess) return true;
   const size_t smem = kSmem + (size_t)(a.seqs + 1) * sizeof(unsigned);
-  return launch_pdl(kern, dim3(num_sms_cached()), dim3(THREADS), smem, a.stream, a, plan, pc.o, pc.mz, pc.meta);
+  e = launch_pdl(kern, dim3(num_sms_cached()), dim3(THREADS), smem, a.stream, a, plan, maps, pc.o, pc.mz, pc.meta);
+  return true;
 }
 
 cudaError_t tc_read_status(int* out, bool reset) {
