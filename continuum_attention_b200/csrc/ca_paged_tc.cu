@@ -43,7 +43,7 @@ using namespace sm100;
 
 constexpr int TK = 32, BR = 128, NREG = 3, NST = 4, GROUPS = 3, RING = NST + 1;
 constexpr int MATH_WARPS = 4 * GROUPS, THREADS = (MATH_WARPS + 8) * 32;   // and a warpgroup of issuers, one of loaders
-constexpr int REGS_MATH = 112, REGS_OTHER = 72;
+constexpr int REGS_MATH = 128, REGS_OTHER = 48;
 static_assert(GROUPS * REGS_MATH + 2 * REGS_OTHER <= THREADS / 128 * (65536 / THREADS / 8 * 8), "registers of the launch");
 constexpr uint32_t COLS = 160, COL_O = 96;          // a worker's columns: regions at 0, 32, 64
 static_assert(GROUPS * COLS <= 512, "tensor memory");
