@@ -8,6 +8,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "ca_common.cuh"
 #include "ca_internal.h"
@@ -265,9 +266,9 @@ struct Meta {
 };
 
 // Joins the pieces of a cut unit: piece 0 is in this worker's slot, the others are the first pieces of the
-// workers that follow.  A warp takes a row; where rows are fewer than warps, several warps share a row's
-// pieces, each sums its own in order, and then the warps' sums are added in order.
-constexpr int kMergeWarps = 16;
+// workers that follow.  A block takes up to 4 W rows of a unit, a warp four of them; where rows are fewer than
+// warps, several warps share a row's pieces, each sums its own in order, and then the warps' sums are added
+// in order.
 
 struct Sum {
   float m = -INFINITY, z = 0.f, y[4] = {0.f, 0.f, 0.f, 0.f};
@@ -294,29 +295,33 @@ struct Pieces {
   int br, workers;
 };
 
-template <typename T, int DP>
-static __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __grid_constant__ Args a, int group,
+template <typename T, int DP, int W>
+static __global__ void __launch_bounds__(W * 32) merge_kernel(const __grid_constant__ Args a, int group,
                                                                  const __grid_constant__ Pieces one,
                                                                  const __grid_constant__ Pieces two) {
   pdl_wait();
   pdl_launch_dependents();
-  const bool second = (int)blockIdx.x >= one.workers;
+  constexpr int RB = 4 * W;
+  const int slices = (one.br + RB - 1) / RB;         // (the second launch's units have 16 rows at most)
+  const bool second = (int)blockIdx.x >= one.workers * slices;
   const Pieces& pc = second ? two : one;
   const float* part_o = pc.o;
   const float2* part_mz = pc.mz;
   const int BR = pc.br;
   constexpr int VL = DP / 32;                        // values per lane: 2 or 4
-  __shared__ float4 sum_y[kMergeWarps][32];
-  __shared__ float2 sum_mz[kMergeWarps];
-  const int w = (int)blockIdx.x - (second ? one.workers : 0);
+  __shared__ float4 sum_y[W][32];
+  __shared__ float2 sum_mz[W];
+  const int w = second ? (int)blockIdx.x - one.workers * slices : (int)blockIdx.x / slices;
+  const int row0 = second ? 0 : (int)blockIdx.x % slices * RB;   // of the unit
   const Meta mt = pc.meta[w];
   if (mt.pieces == 0) return;
-  const int nrows = min(BR, mt.rows - mt.rt * BR);
+  const int nrows = min(min(BR, mt.rows - mt.rt * BR) - row0, RB);
+  if (nrows <= 0) return;
   int share = 1;                                     // warps per row
-  while (share * 2 * nrows <= kMergeWarps && share * 4 <= mt.pieces) share *= 2;
+  while (share * 2 * nrows <= W && share * 4 <= mt.pieces) share *= 2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % share;
   auto load = [&](int p, int r, float2& mz, float4& y) {
-    const long long row = ((long long)(w + p) * 2 + (p == 0 ? mt.slot : 0)) * BR + r;
+    const long long row = ((long long)(w + p) * 2 + (p == 0 ? mt.slot : 0)) * BR + row0 + r;
     mz = part_mz[row];
     if constexpr (VL == 4) {
       y = *reinterpret_cast<const float4*>(part_o + row * DP + 4 * lane);
@@ -327,7 +332,7 @@ static __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __
   };
   auto store = [&](const Sum& acc, int r) {
     const float inv = acc.z == 0.f ? 0.f : 1.f / acc.z;   // y is 0 then
-    const int row = mt.rt * BR + r, t = row / group;
+    const int row = mt.rt * BR + row0 + r, t = row / group;
     T* dst = (T*)a.o + ((size_t)(mt.start + t) * a.H + (size_t)mt.h * group + (row - t * group)) * a.D + VL * lane;
     if (VL * lane < a.D) {
       store2<T>(dst, acc.y[0] * inv, acc.y[1] * inv);
@@ -336,26 +341,24 @@ static __global__ void __launch_bounds__(kMergeWarps * 32) merge_kernel(const __
   };
   if (share == 1) {
     // four rows of a warp side by side: one after the other each would wait for its own loads
-    for (int r0 = warp; r0 < nrows; r0 += 4 * kMergeWarps) {
-      Sum acc[4];
+    Sum acc[4];
 #pragma unroll 2
-      for (int p = 0; p < mt.pieces; ++p) {
-        float2 mz[4];
-        float4 y[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (r0 + u * kMergeWarps < nrows) load(p, r0 + u * kMergeWarps, mz[u], y[u]);
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-          if (r0 + u * kMergeWarps < nrows) acc[u].add(mz[u].x, mz[u].y, y[u]);
-      }
+    for (int p = 0; p < mt.pieces; ++p) {
+      float2 mz[4];
+      float4 y[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u)
-        if (r0 + u * kMergeWarps < nrows) store(acc[u], r0 + u * kMergeWarps);
+        if (warp + u * W < nrows) load(p, warp + u * W, mz[u], y[u]);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (warp + u * W < nrows) acc[u].add(mz[u].x, mz[u].y, y[u]);
     }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (warp + u * W < nrows) store(acc[u], warp + u * W);
     return;
   }
-  const int r = warp / share;                        // nrows * share <= kMergeWarps
+  const int r = warp / share;                        // nrows * share <= W
   if (r >= nrows) return;
   Sum acc;
 #pragma unroll 4
@@ -389,10 +392,16 @@ inline Pieces carve(char* ws, int br, int per_sm) {
   return Pieces{(float*)ws, (float2*)(ws + o), (Meta*)(ws + o + mz), br, (int)w};
 }
 
+// few rows a unit: sixteen warps share their pieces; else eight, more blocks, and all of a unit's rows at once
 template <typename T, int DP>
 inline cudaError_t launch_merge(const Args& a, const Plan& plan, const Pieces& one, const Pieces& two) {
-  return launch_pdl(merge_kernel<T, DP>, dim3((unsigned)(one.workers + two.workers)), dim3(kMergeWarps * 32), 0,
-                    a.stream, a, plan.group, one, two);
+  auto launch = [&](auto w) {
+    constexpr int W = decltype(w)::value;
+    const int slices = (one.br + 4 * W - 1) / (4 * W);
+    return launch_pdl(merge_kernel<T, DP, W>, dim3((unsigned)(one.workers * slices + two.workers)), dim3(W * 32), 0,
+                      a.stream, a, plan.group, one, two);
+  };
+  return one.br <= 16 ? launch(std::integral_constant<int, 16>{}) : launch(std::integral_constant<int, 8>{});
 }
 
 }  // namespace paged
