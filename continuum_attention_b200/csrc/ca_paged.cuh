@@ -392,7 +392,7 @@ inline Pieces carve(char* ws, int br, int per_sm) {
   return Pieces{(float*)ws, (float2*)(ws + o), (Meta*)(ws + o + mz), br, (int)w};
 }
 
-// few rows a unit: sixteen warps share their pieces; else eight, more blocks, and all of a unit's rows at once
+// few rows a unit: sixteen warps share their pieces; else blocks of four, 16 rows each
 template <typename T, int DP>
 inline cudaError_t launch_merge(const Args& a, const Plan& plan, const Pieces& one, const Pieces& two) {
   auto launch = [&](auto w) {
@@ -401,7 +401,7 @@ inline cudaError_t launch_merge(const Args& a, const Plan& plan, const Pieces& o
     return launch_pdl(merge_kernel<T, DP, W>, dim3((unsigned)(one.workers * slices + two.workers)), dim3(W * 32), 0,
                       a.stream, a, plan.group, one, two);
   };
-  return one.br <= 16 ? launch(std::integral_constant<int, 16>{}) : launch(std::integral_constant<int, 8>{});
+  return one.br <= 16 ? launch(std::integral_constant<int, 16>{}) : launch(std::integral_constant<int, 4>{});
 }
 
 }  // namespace paged

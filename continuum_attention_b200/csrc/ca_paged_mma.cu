@@ -733,7 +733,7 @@ cudaError_t forward_dp(const Args& a, void* workspace) {
   }
   // sequences of up to 16 rows in the decoding form, the others as chunks: on tcgen05 where D allows
   Plan chunks = plan;
-  chunks.min_places = 4;
+  chunks.min_places = 2;
   chunks.unit_cost = kChunkUnitCost;
   chunks.row_lo = 17;
   // (a single sequence is all in one form, whatever its rows)
