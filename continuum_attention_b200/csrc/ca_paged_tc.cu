@@ -19,12 +19,21 @@
 // the order, and V's rows are gathered in it, one key early (ca_paged_mma.cu: cutting keys).
 // Being one thread's, a row needs no exchange between lanes at all.
 //
-// The loader gathers rows through the page table with 16-byte cp.async in the 128-byte swizzle
-// that the matrix descriptors name, any page size and any strides; rows that no key fills are
-// zero.
+// The loader brings rows by TMA, four rows of any page a copy (tile::gather4), in the 128-byte swizzle
+// that the matrix descriptors name; the caches are maps of rows one common divisor of all strides
+// apart, so any page size and any strides do, and a row that no key fills is one outside the map,
+// zeros.  (One 16-byte cp.async per lane and a shuffled 64-bit address each took 2400 cycles a tile
+// and 16000 for a unit's queries: prompts of 2 x 2048 tokens 155 us, with TMA 126.)
 //
-// Against the mma.sync form the products take no issue slots of the math warps, and O no
-// registers, which leaves room for three math warps on a scheduler and less work in each.
+// What bounds it: the scalar work per score, 23.6 instructions with everything, of which the schedulers
+// issue one in 55% of the cycles, with three math warps on each (counters at 511 rows over
+// 16001 keys; tensor pipe 13% busy, transcendental pipe 35%, HBM 5%).  Without the moments that case
+// takes 127 us, without moments and copies 91.  Tried and slower: two workers with tiles of 64 keys (205
+// against 189 us at that case), four workers whose products and copies one warp does (220; registers
+// for two regions only), one such warp for each of three workers (187 against 179).
+// Measured (16 heads of 64): prompts of 2 x 2048 tokens 112 us (mma.sync form 148), 511 rows over
+// 16001 keys 171 us (235), 23 sequences of 0 .. 300 rows over up to 4000 keys, 4 query heads a key
+// head, 82 us (102).
 #include <cuda.h>
 
 #include <numeric>
@@ -43,6 +52,8 @@ using namespace sm100;
 
 constexpr int TK = 32, BR = 128, NREG = 3, NST = 4, GROUPS = 3, RING = NST + 1;
 constexpr int MATH_WARPS = 4 * GROUPS, THREADS = (MATH_WARPS + 8) * 32;   // and a warpgroup of issuers, one of loaders
+// the moments of 16 pairs want 120 registers (112: 189 us at 511 rows over 16001 keys, 120: 180, 128: 179), which the
+// loaders and issuers give up
 constexpr int REGS_MATH = 128, REGS_OTHER = 48;
 static_assert(GROUPS * REGS_MATH + 2 * REGS_OTHER <= THREADS / 128 * (65536 / THREADS / 8 * 8), "registers of the launch");
 constexpr uint32_t COLS = 160, COL_O = 96;          // a worker's columns: regions at 0, 32, 64
@@ -596,13 +607,14 @@ typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void
                              CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
 EncodeFn encode_fn() {
-  static EncodeFn fn = [] {
+  static EncodeFn fn = nullptr;
+  if (!fn) {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
-    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-                    q == cudaDriverEntryPointSuccess;
-    return ok ? reinterpret_cast<EncodeFn>(p) : nullptr;
-  }();
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeFn>(p);
+  }
   return fn;
 }
 
@@ -660,6 +672,11 @@ bool make_maps(const Args& a, bool bf16, Maps& m) {
 }  // namespace
 
 bool tc_launch(const Args& a, const Plan& plan, int dtype, const Pieces& pc, cudaError_t& e) {
+  // a thread that has made no runtime call yet has no context, which the encoder asks for
+  int dev;
+  e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaSetDevice(dev);
+  if (e != cudaSuccess) return true;
   Maps maps;
   if (!make_maps(a, dtype == 1, maps)) return false;
   static_assert(kSmem + (kMaxSeqs + 1) * sizeof(unsigned) <= 232448, "shared memory of a block");

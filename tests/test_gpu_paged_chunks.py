@@ -2,6 +2,7 @@
 ``test_gpu_paged.py`` asks of short ones, and units that end or start inside a tile, a page or a batch."""
 import math
 import random
+import threading
 
 import pytest
 import torch
@@ -253,3 +254,25 @@ def test_two_streams_at_once():
         for o in got:
             check("f16", o, *w, 221)
             assert torch.equal(o, got[0])               # same bits every time
+
+
+def test_from_a_thread_that_never_called_cuda():
+    """The same kernels, so the same bits, from a thread without a context of its own."""
+    lib = _native.lib()
+    case = make_case("bf16", 4, 2, 64, 16, [(150, 300), (1, 40)], seed=31)
+    want = run(case)
+    got = torch.zeros_like(want)
+    q, kc, vc, table, lens, starts, gain = arguments(case)
+    n = lib.ca_paged_workspace_size(2, 150, 4, 2, 64, 1)
+    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    args = (q.data_ptr(), q.stride(0), q.stride(1), kc.data_ptr(), vc.data_ptr(), *kc.stride()[:3], table.data_ptr(),
+            table.stride(0), lens.data_ptr(), starts.data_ptr(), gain.data_ptr(), got.data_ptr(), ws.data_ptr(), n,
+            q.shape[0], 2, 150, 4, 2, 64, kc.shape[0], 16, table.shape[1], 1, 0)
+    torch.cuda.synchronize()
+    status = []
+    t = threading.Thread(target=lambda: status.append(lib.ca_paged_forward(*args)))
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert status == [0]
+    assert torch.equal(got, want)
