@@ -315,6 +315,10 @@ class ContinuumDecoderLM(nn.Module):
             raise ValueError("generate needs prompts of one token at least and max_new_tokens >= 1")
         if temperature < 0:
             raise ValueError("temperature must be >= 0")
+        with torch.cuda.device_of(self.lm_head.weight):      # graphs are captured on the current device
+            return self._generate(prompts, max_new_tokens, temperature, generator, page_size)
+
+    def _generate(self, prompts, max_new_tokens, temperature, generator, page_size):
         device = self.lm_head.weight.device
         lens = [len(p) for p in prompts]
         if max(lens) + max_new_tokens - 1 > self.cfg.block_size:

@@ -39,8 +39,20 @@ def cos_sin_table(T: int, D: int, theta: float, device) -> torch.Tensor:
             if tab is None:
                 ph = rope_phase(T, D, theta, device)
                 tab = torch.stack((ph.cos(), ph.sin()), -1).contiguous()
-                _tables[key] = tab
+                if settled(tab):
+                    _tables[key] = tab
     return tab
+
+
+def settled(table: torch.Tensor) -> bool:
+    """Whether a table that was just computed may be kept for later calls: waits for it, since those may run on
+    other streams.  One that a CUDA graph computes is only that graph's."""
+    if table.is_cuda:
+        with torch.cuda.device(table.device):
+            if torch.cuda.is_current_stream_capturing():
+                return False
+            torch.cuda.current_stream().synchronize()
+    return True
 
 
 def apply_rope_torch(q, k, theta: float):

@@ -30,6 +30,7 @@ import torch
 from . import _native
 from .attention import _DTYPE_CODE, ctypes_ptr, on_device, raw_stream
 from .paged import check_cache
+from .rope import settled
 
 _LAYOUTS = {"interleaved": _native.CA_ROTARY_INTERLEAVED, "half": _native.CA_ROTARY_HALF}
 SCALINGS = (None, "linear", "ntk", "yarn")
@@ -105,15 +106,20 @@ _tables_lock = threading.Lock()
 
 def rotary_table(rotary_dim: int, max_positions: int, theta: float, scaling: Optional[str], factor: float,
                  original_positions: Optional[int], device) -> RotaryTable:
-    """The ``RotaryTable`` of these settings, made once per device."""
+    """The ``RotaryTable`` of these settings, made once per device; not while a CUDA graph is captured."""
     key = (rotary_dim, max_positions, float(theta), scaling, float(factor), original_positions, str(device))
     table = _tables.get(key)
     if table is None:
         with _tables_lock:
             table = _tables.get(key)
             if table is None:
-                table = _tables[key] = RotaryTable(rotary_dim, max_positions, theta=theta, scaling=scaling,
-                                                   factor=factor, original_positions=original_positions, device=device)
+                if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("rotary_table: the table of these settings has to be made before a CUDA graph "
+                                       "that uses it is captured (one call outside does)")
+                table = RotaryTable(rotary_dim, max_positions, theta=theta, scaling=scaling, factor=factor,
+                                    original_positions=original_positions, device=device)
+                settled(table.cos_sin)
+                _tables[key] = table
     return table
 
 

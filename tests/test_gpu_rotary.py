@@ -221,3 +221,22 @@ def test_captured_forward_and_backward():
         t.normal_()
     graph.replay()
     assert torch.equal(dx, step())
+
+
+def test_shared_tables_are_not_made_by_a_capture():
+    """A table kept for later calls must not be one that only a graph's replay fills."""
+    from continuum_attention_b200.rope import cos_sin_table
+    from continuum_attention_b200.rotary import rotary_table
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=side):
+        inside = cos_sin_table(57, 48, 777.0, torch.device("cuda", 0))
+        with pytest.raises(RuntimeError, match="before a CUDA graph"):
+            rotary_table(48, 57, 777.0, "ntk", 2.0, None, torch.device("cuda", 0))
+    after = cos_sin_table(57, 48, 777.0, torch.device("cuda", 0))
+    assert after is not inside and cos_sin_table(57, 48, 777.0, torch.device("cuda", 0)) is after
+    graph.replay()
+    assert torch.equal(inside, after)
+    table = rotary_table(48, 57, 777.0, "ntk", 2.0, None, torch.device("cuda", 0))
+    assert rotary_table(48, 57, 777.0, "ntk", 2.0, None, torch.device("cuda", 0)) is table
