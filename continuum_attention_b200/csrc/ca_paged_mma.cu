@@ -37,6 +37,14 @@
 // followed by 16 bytes: the eight land in different banks without any address arithmetic, and
 // each NJ rows (512 or 1024 bytes) are one bulk copy where the page holds them in one run,
 // else one copy per row.
+//
+// What bounds it.  Decoding reads every visible key's K and V once and is bound by that: 2 sequences
+// over 90001 .. 131071 keys (f16, 32 heads on 8 of 64, pages of 16) 90 us for 506 MB, 5.6 TB/s; 17
+// sequences of 1 .. 4 rows over up to 20000 keys (bf16, 32 heads on 8 of 128) 98 us for 484 MB, 4.9 TB/s;
+// 64 sequences over 1 .. 8192 keys (bf16, 16 heads of 64) 50 us for 231 MB, 4.6 TB/s; a single
+// sequence of 2048 keys is all latency, 12 us (launch, page look-ups, one round of copies, the join).
+// Chunks are bound by the scalar work and its dependences (885 issue slots a warp for 1024 scores, 40% of
+// the cycles issue); long ones of narrow heads are ca_paged_tc.cu's.
 #include <algorithm>
 #include <type_traits>
 
@@ -715,7 +723,10 @@ cudaError_t launch_main(const Args& a, Plan plan, const Pieces& pc, bool after_c
                     pc.meta, (int)after_chunks);
 }
 
-// 128-row units on tcgen05 for chunks whose longest sequence fills half of one
+// 128-row units on tcgen05 (ca_paged_tc.cu) for heads of up to 64 values, where the longest sequence fills more than
+// half of one; else units of 64 rows on mma.sync.  16 heads, tcgen05 against mma.sync: 16 sequences of 64 rows over
+// 4096 keys 173 and 136 us, of 80 rows 174 and 251; 1 of 128 rows over 16000 keys 77 and 81; 4 prompts of 256 of
+// 512 keys 35 and 31.
 bool use_tc(long long rows, int dp) { return dp == 64 && rows > 64; }
 
 template <typename T, int DP>

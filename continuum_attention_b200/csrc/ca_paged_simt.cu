@@ -8,7 +8,8 @@
 //
 // What bounds it: decoding reads 2 D f32 values a key and key head, at most 16 rows' FMAs
 // for them; chunks are bound by the FMA pipe and the shared-memory reads that feed it
-// (scores: 6 16-byte reads for 32 FMAs of a thread; P V: 8 for 64).
+// (scores: 6 16-byte reads for 32 FMAs of a thread; P V: 8 for 64).  8 prompts of 40 .. 192 tokens
+// (4 heads of 64) take 25 us, nearly all of it latency: launch, a unit's few tiles, the join.
 #include "ca_paged.cuh"
 
 namespace ca {
