@@ -28,7 +28,7 @@ from typing import Optional
 import torch
 
 from . import _native
-from .attention import _DTYPE_CODE, ctypes_ptr, on_device, raw_stream
+from .attention import _DTYPE_CODE, on_device, raw_stream
 from .paged import check_cache
 from .rope import settled
 
@@ -159,14 +159,13 @@ class RotaryQKVFunction(torch.autograd.Function):
         D = width // (heads + 2 * kv_heads)
         if not qkv.is_contiguous() or qkv.data_ptr() % 16:
             qkv = _aligned(qkv.contiguous())
-        q = torch.empty(B, heads, T, D, dtype=qkv.dtype, device=qkv.device)
-        k = torch.empty(B, kv_heads, T, D, dtype=qkv.dtype, device=qkv.device)
-        v = torch.empty_like(k)
+        q = qkv.new_empty(B, heads, T, D)
+        k, v = qkv.new_empty(B, kv_heads, T, D), qkv.new_empty(B, kv_heads, T, D)
         stride = 0 if positions is None or positions.dim() == 1 else positions.stride(0)
         with on_device(qkv.device):
             st = _native.lib().ca_rotary_qkv_forward(
-                ctypes_ptr(qkv), width, ctypes_ptr(cos_sin), None if positions is None else ctypes_ptr(positions),
-                stride, ctypes_ptr(q), ctypes_ptr(k), ctypes_ptr(v), B, T, heads, kv_heads, D, 2 * cos_sin.shape[1],
+                qkv.data_ptr(), width, cos_sin.data_ptr(), None if positions is None else positions.data_ptr(),
+                stride, q.data_ptr(), k.data_ptr(), v.data_ptr(), B, T, heads, kv_heads, D, 2 * cos_sin.shape[1],
                 cos_sin.shape[0], layout, _DTYPE_CODE[qkv.dtype], raw_stream(qkv.device))
         _native.check("ca_rotary_qkv_forward", st)
         ctx.save_for_backward(cos_sin, positions)
@@ -188,11 +187,11 @@ class RotaryQKVFunction(torch.autograd.Function):
             elif g.dtype != dtype or not g.is_contiguous() or g.data_ptr() % 16:
                 g = _aligned(g.to(dtype).contiguous())
             grads.append(g)
-        dqkv = torch.empty(B, T, (heads + 2 * kv_heads) * D, dtype=dtype, device=device)
+        dqkv = grads[0].new_empty(B, T, (heads + 2 * kv_heads) * D)
         with on_device(device):
             st = _native.lib().ca_rotary_qkv_backward(
-                ctypes_ptr(grads[0]), ctypes_ptr(grads[1]), ctypes_ptr(grads[2]), ctypes_ptr(cos_sin),
-                None if positions is None else ctypes_ptr(positions), stride, ctypes_ptr(dqkv), B, T, heads, kv_heads,
+                grads[0].data_ptr(), grads[1].data_ptr(), grads[2].data_ptr(), cos_sin.data_ptr(),
+                None if positions is None else positions.data_ptr(), stride, dqkv.data_ptr(), B, T, heads, kv_heads,
                 D, 2 * cos_sin.shape[1], cos_sin.shape[0], layout, _DTYPE_CODE[dtype], raw_stream(device))
         _native.check("ca_rotary_qkv_backward", st)
         return dqkv, None, None, None, None, None
@@ -254,9 +253,9 @@ def rotary_append(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     cs = table.cos_sin
     with on_device(qkv.device):
         st = _native.lib().ca_rotary_append(
-            ctypes_ptr(qkv), qkv.stride(0), ctypes_ptr(cs), ctypes_ptr(out), ctypes_ptr(k_cache), ctypes_ptr(v_cache),
-            k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), ctypes_ptr(page_table), page_table.stride(0),
-            ctypes_ptr(kv_lens), ctypes_ptr(q_starts), N, kv_lens.shape[0], heads, G, D, table.rotary_dim, cs.shape[0],
+            qkv.data_ptr(), qkv.stride(0), cs.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+            k_cache.stride(0), k_cache.stride(1), k_cache.stride(2), page_table.data_ptr(), page_table.stride(0),
+            kv_lens.data_ptr(), q_starts.data_ptr(), N, kv_lens.shape[0], heads, G, D, table.rotary_dim, cs.shape[0],
             P, page, page_table.shape[1], _LAYOUTS[layout], _DTYPE_CODE[qkv.dtype], raw_stream(qkv.device))
     _native.check("ca_rotary_append", st)
     return out
