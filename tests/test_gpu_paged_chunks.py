@@ -276,3 +276,34 @@ def test_from_a_thread_that_never_called_cuda():
     torch.cuda.synchronize()
     assert status == [0]
     assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_short_sequence_alone_in_a_long_buffer(dtype):
+    """max_q_len and the buffer say 100 rows, the sequence has three."""
+    case = make_case(dtype, 4, 2, 64, 16, [(3, 50)], seed=32, tail=97)
+    out = torch.full_like(case["q"], 7.0)
+    run(case, max_q_len=100, out=out)
+    check(dtype, out, *exact(case), 3)
+    assert (out[3:] == 7.0).all()
+    assert _native.lib().ca_device_status(0) == 0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_as_many_sequences_as_a_call_takes(dtype):
+    seqs = [(1, 1 + s % 40) for s in range(1500)] + [(0, 3)] * 500 + [(2, 5)] * 46 + [(70, 100), (80, 80)]
+    assert len(seqs) == 2048
+    run_and_check(dtype, make_case(dtype, 2, 2, 16, 16, seqs, seed=33))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n", [1, 20, 100])
+def test_a_cache_without_pages(dtype, n):
+    """No keys anywhere: every row is zero."""
+    q = torch.randn(n, 4, 64, device="cuda").to(DTYPES[dtype])
+    kc = torch.empty(0, 2, 16, 64, dtype=q.dtype, device="cuda")
+    ints = [torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([0], [0, n])]
+    table = torch.empty(1, 0, dtype=torch.int32, device="cuda")
+    out = continuum_attention_paged(q, kc, kc.clone(), table, *ints, torch.zeros(4, device="cuda"), max_q_len=n)
+    assert (out == 0).all()
+    assert _native.lib().ca_device_status(0) == 0
