@@ -6,8 +6,8 @@
 // Tiles arrive by cp.async, one ahead, gathered row by row through the page table, V one
 // row early so that the weights of keys a-1 .. a+TK-2 meet it where they lie.
 //
-// What bounds it: decoding reads 2 D f32 values a key and key head, at most 16 rows' FMAs
-// for them; chunks are bound by the FMA pipe and the shared-memory reads that feed it
+// What bounds it: decoding reads 2 D f32 values a key and key head and comes to 70% of the copy
+// rate, held by the latency of a tile's three steps at ten warps an SM; chunks are bound by the FMA pipe and the shared-memory reads that feed it
 // (scores: 6 16-byte reads for 32 FMAs of a thread; P V: 8 for 64).  8 prompts of 40 .. 192 tokens
 // (4 heads of 64) take 25 us, nearly all of it latency: launch, a unit's few tiles, the join.
 #include "ca_paged.cuh"
@@ -38,7 +38,16 @@ struct Config {
   static constexpr int TILE = (TK + 1) * LD;            // floats; row TK is the halo
   static constexpr int FLOATS = 4 * TILE + BR * LD + BR * LS + 4 * BR;
   static constexpr int SMEM = FLOATS * 4 + 3 * (TK + 1) * 8;   // and the prefix sums behind it
-  static_assert(TPR >= 1 && 32 % TPR == 0 && KPT % 4 == 0 && CT % 4 == 0, "");
+  static_assert(TPR >= 1 && 32 % TPR == 0 && CT % 2 == 0, "");
+  static constexpr int VW = CT % 4 == 0 ? 4 : 2;        // output columns of one access
+  static constexpr int SW = KPT < 4 ? KPT : 4;          // scores of one access
+};
+
+template <int N>
+struct alignas(N * 4) Vec {
+  float x[N];
+  static __device__ __forceinline__ Vec load(const float* p) { return *reinterpret_cast<const Vec*>(p); }
+  __device__ __forceinline__ void store(float* p) const { *reinterpret_cast<Vec*>(p) = *this; }
 };
 
 struct Tile {      // what the block knows of a tile (the same in all threads)
@@ -246,12 +255,10 @@ __global__ void __launch_bounds__(C::NT, C::PER_SM)
       float s[C::KPT];
       float top = kMasked;
 #pragma unroll
-      for (int x = 0; x < C::KPT; x += 4) {
-        const float4 v = *reinterpret_cast<const float4*>(sr + x);
-        s[x] = v.x;
-        s[x + 1] = v.y;
-        s[x + 2] = v.z;
-        s[x + 3] = v.w;
+      for (int x = 0; x < C::KPT; x += C::SW) {
+        const Vec<C::SW> v = Vec<C::SW>::load(sr + x);
+#pragma unroll
+        for (int e = 0; e < C::SW; ++e) s[x + e] = v.x[e];
       }
 #pragma unroll
       for (int x = 0; x < C::KPT; ++x) {
@@ -302,8 +309,12 @@ __global__ void __launch_bounds__(C::NT, C::PER_SM)
       carry_s = __shfl_sync(0xffffffffu, sa, C::TPR - 1, C::TPR);
       carry_b = __shfl_sync(0xffffffffu, right, C::TPR - 1, C::TPR);
 #pragma unroll
-      for (int x = 0; x < C::KPT; x += 4)
-        *reinterpret_cast<float4*>(sr + x) = make_float4(p[x], p[x + 1], p[x + 2], p[x + 3]);
+      for (int x = 0; x < C::KPT; x += C::SW) {
+        Vec<C::SW> v;
+#pragma unroll
+        for (int e = 0; e < C::SW; ++e) v.x[e] = p[x + e];
+        v.store(sr + x);
+      }
       if (mpart == 0) row_f[mrow] = f;
     }
     __syncthreads();
@@ -322,18 +333,17 @@ __global__ void __launch_bounds__(C::NT, C::PER_SM)
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
 #pragma unroll
-        for (int c = 0; c < CT; c += 4) {
-          const float4 v = *reinterpret_cast<const float4*>(vs + (k + u) * LD + tc * CT + c);
+        for (int c = 0; c < CT; c += C::VW) {
+          const Vec<C::VW> v = Vec<C::VW>::load(vs + (k + u) * LD + tc * CT + c);
 #pragma unroll
           for (int i = 0; i < RT; ++i) {
             const float w = u == 0 ? p[i].x : u == 1 ? p[i].y : u == 2 ? p[i].z : p[i].w;
-            float2 lo = make_float2(o[i][c], o[i][c + 1]), hi = make_float2(o[i][c + 2], o[i][c + 3]);
-            lo = fma2(splat2(w), make_float2(v.x, v.y), lo);
-            hi = fma2(splat2(w), make_float2(v.z, v.w), hi);
-            o[i][c] = lo.x;
-            o[i][c + 1] = lo.y;
-            o[i][c + 2] = hi.x;
-            o[i][c + 3] = hi.y;
+#pragma unroll
+            for (int e = 0; e < C::VW; e += 2) {
+              const float2 y = fma2(splat2(w), make_float2(v.x[e], v.x[e + 1]), make_float2(o[i][c + e], o[i][c + e + 1]));
+              o[i][c + e] = y.x;
+              o[i][c + e + 1] = y.y;
+            }
           }
         }
       }
@@ -368,19 +378,18 @@ __global__ void __launch_bounds__(C::NT, C::PER_SM)
         float* dst = (float*)a.o +
                      ((size_t)(t.start + tk) * a.H + (size_t)t.h * plan.group + (row - tk * plan.group)) * a.D;
 #pragma unroll
-        for (int c = 0; c < CT; c += 4) {
+        for (int c = 0; c < CT; c += C::VW) {
           const int col = tc * CT + c;
-          float4 y = make_float4(o[i][c], o[i][c + 1], o[i][c + 2], o[i][c + 3]);
-          if (w != 0.f) {
-            const float4 v = *reinterpret_cast<const float4*>(vs + TK * LD + col);
-            y = make_float4(fmaf(w, v.x, y.x), fmaf(w, v.y, y.y), fmaf(w, v.z, y.z), fmaf(w, v.w, y.w));
-          }
+          Vec<C::VW> y = Vec<C::VW>::load(vs + TK * LD + col);
+#pragma unroll
+          for (int e = 0; e < C::VW; ++e) y.x[e] = w != 0.f ? fmaf(w, y.x[e], o[i][c + e]) : o[i][c + e];
           if (!whole) {
-            *reinterpret_cast<float4*>(part_o + (slot_row + r) * DP + col) = y;
+            y.store(part_o + (slot_row + r) * DP + col);
           } else if (col < a.D) {
             // z = 0: the row sees no key
-            *reinterpret_cast<float4*>(dst + col) =
-                zr == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+#pragma unroll
+            for (int e = 0; e < C::VW; ++e) y.x[e] = zr == 0.f ? 0.f : y.x[e] * inv;
+            y.store(dst + col);
           }
         }
       }
@@ -405,10 +414,19 @@ __global__ void __launch_bounds__(C::NT, C::PER_SM)
   cp_wait<0>();
 }
 
-// rows of a unit: 16 for decoding, 64 for chunks
-template <int DP> using Few = Config<DP, 16, 16, 8, DP == 64 ? 5 : 2>;
+// Rows of a unit: 4 or 16 for decoding, 64 for chunks.  In the decoding forms a warp's lanes are the tile's 32
+// keys, then its output columns.  64 sequences of one row over 8192 keys (16 heads of 64): units of 4 rows 955 us
+// (4.5 TB/s; on one warp 1220, on four 1050), of 16 rows 3230; 16 rows over 4096 keys (16 sequences, 32 heads on
+// 2 of 64): 46 us, with threads in 16 x 8 75.
+template <int DP> using One = Config<DP, 4, 2, 32, DP == 64 ? 5 : 3>;
+template <int DP> using Few = Config<DP, 16, 4, 32, DP == 64 ? 4 : 2>;
 template <int DP> using Many = Config<DP, 64, 16, 16, DP == 64 ? 2 : 1>;
 constexpr int kUnitCost = 1;
+
+template <int DP, typename F>
+auto with_form(long long rows, F f) {
+  return rows <= 4 ? f(One<DP>{}) : rows <= 16 ? f(Few<DP>{}) : f(Many<DP>{});
+}
 
 template <typename C>
 cudaError_t launch_main(const Args& a, const Plan& plan, const Pieces& pc) {
@@ -429,18 +447,24 @@ cudaError_t forward_dp(const Args& a, void* workspace) {
   char* ws = (char*)workspace;
   // every sequence in the form that suits the longest: 64-row units leave threads of a short one idle, but
   // in 32 bits the loads and FMAs of a tile are the same whatever its rows
-  const bool few = (long long)a.max_q_len * plan.group <= 16;
-  const Pieces pc = few ? carve<DP>(ws, Few<DP>::BR, Few<DP>::PER_SM) : carve<DP>(ws, Many<DP>::BR, Many<DP>::PER_SM);
-  cudaError_t e = few ? launch_main<Few<DP>>(a, plan, pc) : launch_main<Many<DP>>(a, plan, pc);
-  return e != cudaSuccess ? e : launch_merge<float, DP>(a, plan, pc, Pieces{});
+  const long long rows = (long long)a.max_q_len * plan.group;
+  auto run = [&](auto form) {
+    using C = decltype(form);
+    const Pieces pc = carve<DP>(ws, C::BR, C::PER_SM);
+    const cudaError_t e = launch_main<C>(a, plan, pc);
+    return e != cudaSuccess ? e : launch_merge<float, DP>(a, plan, pc, Pieces{});
+  };
+  return with_form<DP>(rows, run);
 }
 
 }  // namespace
 
 size_t simt_workspace_bytes(long long max_q_len, long long H, long long G, long long D) {
-  const bool few = max_q_len * (H / G) <= 16;
-  if (D <= 64) return few ? pieces_bytes<64>(Few<64>::BR, Few<64>::PER_SM) : pieces_bytes<64>(Many<64>::BR, Many<64>::PER_SM);
-  return few ? pieces_bytes<128>(Few<128>::BR, Few<128>::PER_SM) : pieces_bytes<128>(Many<128>::BR, Many<128>::PER_SM);
+  auto bytes = [](auto form) {
+    using C = decltype(form);
+    return pieces_bytes<C::DP>(C::BR, C::PER_SM);
+  };
+  return D <= 64 ? with_form<64>(max_q_len * (H / G), bytes) : with_form<128>(max_q_len * (H / G), bytes);
 }
 
 int simt_launches(const Args&) { return 2; }
