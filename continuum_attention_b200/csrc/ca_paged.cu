@@ -1,6 +1,6 @@
 // ca_paged.cu -- Continuum Attention of new tokens over a paged cache: the choice of kernels.
 //
-// bf16 and f16 run on the tensor cores (decoding, short chunks and wide heads ca_paged_mma.cu, long
+// bf16 and f16 run on the tensor cores (decoding and short chunks ca_paged_mma.cu, long
 // chunks ca_paged_tc.cu), f32 on the FMA pipes (ca_paged_simt.cu), whose scores are exact to 32 bits as f32
 // inputs ask.
 #include "ca_paged.cuh"

@@ -63,10 +63,10 @@ int simt_launches(const Args& a);
 cudaError_t simt_forward(const Args& a, void* workspace);
 cudaError_t simt_read_status(int* out, bool reset);
 
-// chunks in bf16 and f16 with D <= 64 on tcgen05 (ca_paged_tc.cu): units of tc_br() rows, tc_groups() workers per SM
+// long chunks in bf16 and f16 on tcgen05 (ca_paged_tc.cu): units of tc_br() rows, tc_groups() workers per SM
 struct Pieces;
 int tc_br();
-int tc_groups();
+int tc_groups(int dp);
 // false where the caches' strides do not suit it: nothing was launched
 bool tc_launch(const Args& a, const Plan& plan, int dtype, const Pieces& pc, cudaError_t& e);
 cudaError_t tc_read_status(int* out, bool reset);

@@ -44,7 +44,7 @@
 // 64 sequences over 1 .. 8192 keys (bf16, 16 heads of 64) 50 us for 231 MB, 4.6 TB/s; a single
 // sequence of 2048 keys is all latency, 12 us (launch, page look-ups, one round of copies, the join).
 // Chunks are bound by the scalar work and its dependences (885 issue slots a warp for 1024 scores, 40% of
-// the cycles issue); long ones of narrow heads are ca_paged_tc.cu's.
+// the cycles issue); those of more than 64 rows are ca_paged_tc.cu's.
 #include <algorithm>
 #include <type_traits>
 
@@ -723,11 +723,11 @@ cudaError_t launch_main(const Args& a, Plan plan, const Pieces& pc, bool after_c
                     pc.meta, (int)after_chunks);
 }
 
-// 128-row units on tcgen05 (ca_paged_tc.cu) for heads of up to 64 values, where the longest sequence fills more than
-// half of one; else units of 64 rows on mma.sync.  16 heads, tcgen05 against mma.sync: 16 sequences of 64 rows over
-// 4096 keys 173 and 136 us, of 80 rows 174 and 251; 1 of 128 rows over 16000 keys 77 and 81; 4 prompts of 256 of
-// 512 keys 35 and 31.
-bool use_tc(long long rows, int dp) { return dp == 64 && rows > 64; }
+// 128-row units on tcgen05 (ca_paged_tc.cu) where the longest sequence fills more than half of one; else units of 64
+// rows on mma.sync.  16 heads of 64, tcgen05 against mma.sync: 16 sequences of 64 rows over 4096 keys 173 and 136 us,
+// of 80 rows 174 and 251; 1 of 128 rows over 16000 keys 77 and 81; 4 pieces of 256 rows over 512 keys 35 and 31.
+// Heads of 128: 80 rows 270 and 372, 128 rows 99 and 116, 256 rows 43 and 47.
+bool use_tc(long long rows) { return rows > 64; }
 
 template <typename T, int DP>
 cudaError_t forward_dp(const Args& a, void* workspace) {
@@ -742,18 +742,18 @@ cudaError_t forward_dp(const Args& a, void* workspace) {
                               : launch_main<T, Decode16<DP>>(a, plan, pc, false);
     return e != cudaSuccess ? e : launch_merge<T, DP>(a, plan, pc, Pieces{});
   }
-  // sequences of up to 16 rows in the decoding form, the others as chunks: on tcgen05 where D allows
+  // sequences of up to 16 rows in the decoding form, the others as chunks
   Plan chunks = plan;
   chunks.min_places = 2;
   chunks.unit_cost = kChunkUnitCost;
   chunks.row_lo = 17;
   // (a single sequence is all in one form, whatever its rows)
   if (a.seqs == 1) chunks.row_lo = 0;
-  const bool wide = use_tc(rows, DP);
-  const int br = wide ? tc_br() : Chunk<DP>::BR, groups = wide ? tc_groups() : Chunk<DP>::GROUPS;
+  const bool tall = use_tc(rows);
+  const int br = tall ? tc_br() : Chunk<DP>::BR, groups = tall ? tc_groups(DP) : Chunk<DP>::GROUPS;
   Pieces pc = carve<DP>(ws, br, groups);
   cudaError_t e;
-  if (!wide || !tc_launch(a, chunks, std::is_same_v<T, __nv_bfloat16> ? 1 : 2, pc, e)) {
+  if (!tall || !tc_launch(a, chunks, std::is_same_v<T, __nv_bfloat16> ? 1 : 2, pc, e)) {
     pc = carve<DP>(ws, Chunk<DP>::BR, Chunk<DP>::GROUPS);   // its units are the smaller ones
     e = launch_main<T, Chunk<DP>>(a, chunks, pc, false);
   }
@@ -777,7 +777,7 @@ size_t mma_workspace_bytes(long long max_q_len, long long H, long long G, long l
     const size_t few = pieces_bytes<DP>(D16::BR, D16::GROUPS);
     return rows <= 8 ? pieces_bytes<DP>(D8::BR, D8::GROUPS)
                      : rows <= 16 ? few
-                                  : few + (use_tc(rows, DP) ? pieces_bytes<DP>(tc_br(), tc_groups())
+                                  : few + (use_tc(rows) ? pieces_bytes<DP>(tc_br(), tc_groups(DP))
                                                             : pieces_bytes<DP>(Ck::BR, Ck::GROUPS));
   };
   return D <= 64 ? bytes(Decode8<64>{}, Decode16<64>{}, Chunk<64>{}) : bytes(Decode8<128>{}, Decode16<128>{}, Chunk<128>{});

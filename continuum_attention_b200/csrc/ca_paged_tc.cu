@@ -1,11 +1,12 @@
 // ca_paged_tc.cu -- Continuum Attention of chunks over a paged cache on tcgen05: bf16 and f16,
-// head values up to 64, units of 128 rows.
+// units of 128 rows.
 //
 // Work is divided as in ca_paged_mma.cu (units, places, pieces, merge).  One block runs on an SM,
-// with three workers that share nothing but the tensor pipe: each has four math warps (a thread
-// is a row, its TMEM lane), a warp that issues the products and a warp that loads.
+// with three workers (two where heads have more than 64 values) that share nothing but the tensor
+// pipe: each has four math warps (a thread is a row, its TMEM lane), a warp that issues the products
+// and a warp that loads.
 //
-// A worker's tensor memory: three regions of 32 columns and O in 64.  Tile t of 32 keys has its
+// A worker's tensor memory: three regions of 32 columns and O in 64 or 128.  Tile t of 32 keys has its
 // scores S = Q K^T in region t mod 3; its weights P overwrite them in place, each 16 keys as 8
 // columns of hi pairs and 8 of lo pairs (two 16-bit parts, see ca_paged_mma.cu); then
 // O += P_hi V + P_lo V with P as the A operand from tensor memory.  The products run in issue
@@ -33,7 +34,8 @@
 // for two regions only), one such warp for each of three workers (187 against 179).
 // Measured (16 heads of 64): prompts of 2 x 2048 tokens 112 us (mma.sync form 148), 511 rows over
 // 16001 keys 171 us (235), 23 sequences of 0 .. 300 rows over up to 4000 keys, 4 query heads a key
-// head, 82 us (102).
+// head, 82 us (102).  Heads of 128, with two workers and one unit's queries at a time: the first two 169 (226)
+// and 259 us (352).
 #include <cuda.h>
 
 #include <numeric>
@@ -50,43 +52,52 @@ namespace {
 
 using namespace sm100;
 
-constexpr int TK = 32, BR = 128, NREG = 3, NST = 4, GROUPS = 3, RING = NST + 1;
-constexpr int MATH_WARPS = 4 * GROUPS, THREADS = (MATH_WARPS + 8) * 32;   // and a warpgroup of issuers, one of loaders
-// the moments of 16 pairs want 120 registers (112: 189 us at 511 rows over 16001 keys, 120: 180, 128: 179), which the
-// loaders and issuers give up
-constexpr int REGS_MATH = 128, REGS_OTHER = 48;
-static_assert(GROUPS * REGS_MATH + 2 * REGS_OTHER <= THREADS / 128 * (65536 / THREADS / 8 * 8), "registers of the launch");
-constexpr uint32_t COLS = 160, COL_O = 96;          // a worker's columns: regions at 0, 32, 64
-static_assert(GROUPS * COLS <= 512, "tensor memory");
-constexpr uint32_t Q_BYTES = BR * 128, KV_BYTES = TK * 128;
+constexpr int TK = 32, BR = 128, NREG = 3, NST = 4, RING = NST + 1;
+
+// head values padded to DP, in halves of 64 (128 bytes, a swizzled row)
+template <int DP_>
+struct Config {
+  static constexpr int DP = DP_, HALVES = DP / 64;
+  static constexpr int GROUPS = DP == 64 ? 3 : 2;
+  static constexpr int MATH_WARPS = 4 * GROUPS, THREADS = (MATH_WARPS + 8) * 32;   // and a warpgroup of issuers, one of loaders
+  // the moments of 16 pairs want 120 registers (112: 189 us at 511 rows over 16001 keys, 120: 180, 128: 179), which the
+  // loaders and issuers give up
+  static constexpr int REGS_MATH = DP == 64 ? 128 : 168, REGS_OTHER = DP == 64 ? 48 : 88;
+  static_assert(GROUPS * REGS_MATH + 2 * REGS_OTHER <= THREADS / 128 * (65536 / THREADS / 8 * 8), "registers of the launch");
+  static constexpr uint32_t COL_O = DP == 64 ? 96 : 128, COLS = COL_O + DP;   // a worker's columns: regions at 0, 32, 64
+  static_assert(GROUPS * COLS <= 512, "tensor memory");
+  static constexpr int QBUF = DP == 64 ? 2 : 1;       // units whose queries are held at once
+  static constexpr uint32_t Q_HALF = BR * 128, Q_BYTES = HALVES * Q_HALF;
+  static constexpr uint32_t KV_HALF = TK * 128, KV_BYTES = HALVES * KV_HALF;
+
+  struct alignas(16) Slot {     // what a tile's readers need beside its stage
+    int kt, flags, len, nt;     // tile in its unit, flags, keys of the sequence, tiles of the unit
+    int start, n, h, rt;        // the sequence's rows; key head; row tile
+    uint8_t k_before[2 * DP];   // K of the key before a piece
+    uint8_t v_last[2 * DP];     // V of a piece's last key
+  };
+
+  struct alignas(1024) Group {
+    uint8_t q[QBUF][Q_BYTES];
+    uint8_t k[NST][KV_BYTES];
+    uint8_t v[NST][KV_BYTES];
+  };
+
+  struct alignas(16) Control {
+    uint64_t full[NST];         // a tile's rows and descriptor are there                 (1: the loader)
+    uint64_t free_[NST];        // its products have read them                              (1: commit)
+    uint64_t s_full[NREG];      // its scores are in tensor memory                          (1: commit)
+    uint64_t p_ready[NREG];     // its weights are                                          (4: math warps)
+    uint64_t pv_done[2];        // P V of tile t and all before it: barrier t & 1           (1: commit)
+    uint64_t drained;           // every product, where a wait gave up                      (1: commit)
+    int gave_up;
+    Slot ring[RING];
+  };
+
+  static constexpr size_t SMEM = GROUPS * (sizeof(Group) + sizeof(Control)) + 16;   // and the prefix sums behind it
+};
 
 enum : int { kFirst = 1, kLast = 2, kBad = 4, kEnd = 8, kNone = 16, kQ1 = 32 };   // kQ1: Q is in buffer 1
-
-struct alignas(16) Slot {     // what a tile's readers need beside its stage
-  int kt, flags, len, nt;     // tile in its unit, flags, keys of the sequence, tiles of the unit
-  int start, n, h, rt;        // the sequence's rows; key head; row tile
-  uint8_t k_before[128];      // K of the key before a piece
-  uint8_t v_last[128];        // V of a piece's last key
-};
-
-struct alignas(1024) Group {
-  uint8_t q[2][Q_BYTES];
-  uint8_t k[NST][KV_BYTES];
-  uint8_t v[NST][KV_BYTES];
-};
-
-struct alignas(16) Control {
-  uint64_t full[NST];         // a tile's rows and descriptor are there                 (1: the loader)
-  uint64_t free_[NST];        // its products have read them                              (1: commit)
-  uint64_t s_full[NREG];      // its scores are in tensor memory                          (1: commit)
-  uint64_t p_ready[NREG];     // its weights are                                          (4: math warps)
-  uint64_t pv_done[2];        // P V of tile t and all before it: barrier t & 1           (1: commit)
-  uint64_t drained;           // every product, where a wait gave up                      (1: commit)
-  int gave_up;
-  Slot ring[RING];
-};
-
-constexpr size_t kSmem = GROUPS * (sizeof(Group) + sizeof(Control)) + 16;   // and the prefix sums behind it
 
 template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -117,10 +128,11 @@ struct Maps {
 
 // ------------------------------------------------------------------ the loader
 
-template <typename T>
+template <typename T, typename C>
 __device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const Maps& maps,
                                           const Schedule<BR, TK>& sched, int worker, unsigned per, unsigned x0,
-                                          unsigned x1, Group& gm, Control& ct, Meta* __restrict__ meta) {
+                                          unsigned x1, typename C::Group& gm, typename C::Control& ct,
+                                          Meta* __restrict__ meta) {
   const int lane = threadIdx.x & 31;
   volatile int* ab = &ct.gave_up;
   typename Schedule<BR, TK>::Cursor cur;
@@ -140,17 +152,19 @@ __device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const
   auto row_of = [&](int page, int key, int h) {       // of the maps
     return page * maps.page + (key - plan.page_of(key) * a.page_size) * maps.slot + h * maps.head;
   };
-  // this lane's four rows of the stage: lanes 0 .. 7 of K, 8 .. 15 of V.  Row r is the key at
+  // this lane's four rows of the stage: K and V, each half, eight lanes.  Row r is the key at
   // 16 (r / 16) + (r % 16) / 2 + 8 (r % 2): K of it, V of the key before it
-  const bool is_v = lane >= 8;
-  const uint32_t dst = (is_v ? smem_u32(gm.v) : smem_u32(gm.k)) + (lane & 7) * 512;
+  constexpr int KL = 8 * C::HALVES;
+  const bool is_v = lane >= KL;
+  const int half = C::HALVES == 1 ? 0 : (lane >> 3) & 1;
+  const uint32_t dst = (is_v ? smem_u32(gm.v) : smem_u32(gm.k)) + half * C::KV_HALF + (lane & 7) * 512;
   const int p0 = ((lane & 4) << 2) + ((lane & 3) << 1);    // of its first row: + 0, 8, 1, 9 for the four
   const CUtensorMap* map = is_v ? &maps.v : &maps.k;
   const uint32_t row_bytes = a.D * sizeof(T);
 
   bool first = true, in_first = true;
-  int kt0 = 0, qbuf = 1;
-  int last_tile[2] = {-1, -1};   // the last tiles of the units before this one and before that
+  int kt0 = 0, qbuf = C::QBUF - 1;
+  int last_tile[2] = {-1, -1};   // the last tiles of the unit before this one and of that before it
   int before = -1;               // the row of the key before the tile (-1: none)
   int pg = page_at(cur.kt * TK + lane);
   int pg_before = cur.kt > 0 ? page_at(cur.kt * TK - 1) : -1;
@@ -162,9 +176,9 @@ __device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const
     const int base = cur.kt * TK;
     const bool opens = first || cur.kt == 0;
     int flags = cur.bad ? kBad : 0;
-    Slot& slot = ct.ring[t % RING];
+    typename C::Slot& slot = ct.ring[t % RING];
     const uint32_t bar = smem_u32(&ct.full[st]);
-    uint32_t bytes = 2 * KV_BYTES;
+    uint32_t bytes = 2 * C::KV_BYTES;
     const int key = base + lane;
     bool bad = key < cur.len && (pg < 0 || pg >= a.num_pages);
     const int row = key < cur.len && !bad ? row_of(pg, key, cur.h) : -1;
@@ -173,12 +187,12 @@ __device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const
       kt0 = cur.kt;
       in_first = first;
       first = false;
-      qbuf ^= 1;
-      // Q of the unit before the last one lay in this buffer: its products have to be done (they are known to
-      // be where the stage of its last tile has been filled again since)
-      const int u = last_tile[1];
+      if (C::QBUF == 2) qbuf ^= 1;
+      // Q of an earlier unit lay in this buffer: its products have to be done (they are known to be where the
+      // stage of its last tile has been filled again since)
+      const int u = last_tile[C::QBUF - 1];
       if (u >= 0 && u + NST > t && !mbar_wait_warp(&ct.free_[u % NST], (u / NST) & 1, ab)) break;
-      bytes += Q_BYTES;
+      bytes += C::Q_BYTES;
       before = -1;
       if (base > 0 && base - 1 < cur.len) {
         if (pg_before < 0 || pg_before >= a.num_pages) bad = true;
@@ -236,19 +250,24 @@ __device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const
       r[x] = __shfl_sync(0xffffffffu, row, p & 31);
       if (p < 0) r[x] = before;
     }
-    if (lane < 16) tma_gather4(dst + st * KV_BYTES, map, bar, r[0], r[1], r[2], r[3]);
+    if (lane < 2 * KL) tma_gather4(dst + st * C::KV_BYTES, map, bar, 64 * half, r[0], r[1], r[2], r[3]);
     if (opens) {
       const int rows = n * plan.group;
       if (maps.q_box) {
         // (rows behind the sequence's last are another's or zeros: nothing of theirs is kept)
-        tma_load_3d(gm.q[qbuf], &maps.q, &ct.full[st], 0, h * plan.group, start + rt * maps.q_box);
+#pragma unroll
+        for (int x = 0; x < C::HALVES; ++x)
+          tma_load_3d(gm.q[qbuf] + x * C::Q_HALF, &maps.q, &ct.full[st], 64 * x, h * plan.group,
+                      start + rt * maps.q_box);
       } else {
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int i = rt * BR + 4 * lane + x, tk = i / plan.group;
           r[x] = i < rows ? (start + tk) * maps.q_token + (h * plan.group + i - tk * plan.group) * maps.q_head : -1;
         }
-        tma_gather4(smem_u32(gm.q[qbuf]) + lane * 512, &maps.q, bar, r[0], r[1], r[2], r[3]);
+#pragma unroll
+        for (int x = 0; x < C::HALVES; ++x)
+          tma_gather4(smem_u32(gm.q[qbuf]) + x * C::Q_HALF + lane * 512, &maps.q, bar, 64 * x, r[0], r[1], r[2], r[3]);
       }
       if (lane == 0 && before >= 0)
         bulk_load(smem_u32(slot.k_before), (const T*)a.k_cache + before * maps.unit, row_bytes, bar);
@@ -264,8 +283,8 @@ __device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const
 
 // ------------------------------------------------------------------ the issuer
 
-template <bool kBF16>
-__device__ __forceinline__ void issue_warp(Group& gm, Control& ct, uint32_t tmem) {
+template <bool kBF16, typename C>
+__device__ __forceinline__ void issue_warp(typename C::Group& gm, typename C::Control& ct, uint32_t tmem) {
   volatile int* ab = &ct.gave_up;
   const uint32_t id_s = make_idesc(BR, TK, kBF16, false), id_o = make_idesc(BR, 64, kBF16, true);
   const uint32_t q0 = smem_u32(gm.q), k0 = smem_u32(gm.k), v0 = smem_u32(gm.v);
@@ -279,12 +298,13 @@ __device__ __forceinline__ void issue_warp(Group& gm, Control& ct, uint32_t tmem
       return;
     }
     more = !(flags & kEnd);
-    const uint64_t qd = sdesc_sw128(q0 + (flags & kQ1 ? Q_BYTES : 0), 16, 1024);
-    const uint64_t kd = sdesc_sw128(k0 + st * KV_BYTES, 16, 1024);
+    const uint64_t qd = sdesc_sw128(q0 + (flags & kQ1 ? C::Q_BYTES : 0), 16, 1024);
+    const uint64_t kd = sdesc_sw128(k0 + st * C::KV_BYTES, 16, 1024);
     tc_fence_after();
 #pragma unroll
-    for (int kk = 0; kk < 4; ++kk)
-      mma_ss(tmem + TK * (issued % NREG), qd + 2 * kk, kd + 2 * kk, id_s, kk > 0 ? 1u : 0u);
+    for (int kk = 0; kk < 4 * C::HALVES; ++kk)
+      mma_ss(tmem + TK * (issued % NREG), qd + (kk >> 2) * (C::Q_HALF >> 4) + 2 * (kk & 3),
+             kd + (kk >> 2) * (C::KV_HALF >> 4) + 2 * (kk & 3), id_s, kk > 0 ? 1u : 0u);
     mma_commit(&ct.s_full[issued % NREG]);
     ++issued;
   };
@@ -309,14 +329,17 @@ __device__ __forceinline__ void issue_warp(Group& gm, Control& ct, uint32_t tmem
     if (!good) break;
     const int st = t % NST;
     const bool first = ct.ring[t % RING].flags & kFirst;
-    const uint64_t vd = sdesc_sw128(v0 + st * KV_BYTES, 16384, 1024);
+    const uint64_t vd = sdesc_sw128(v0 + st * C::KV_BYTES, 16384, 1024);
     const uint32_t p = tmem + TK * (t % NREG);
     tc_fence_after();
 #pragma unroll
-    for (int part = 0; part < 2; ++part)
+    for (int x = 0; x < C::HALVES; ++x)
 #pragma unroll
-      for (int kk = 0; kk < TK / 16; ++kk)
-        mma_ts(tmem + COL_O, p + 16 * kk + 8 * part, vd + 128 * kk, id_o, first && part == 0 && kk == 0 ? 0u : 1u);
+      for (int part = 0; part < 2; ++part)
+#pragma unroll
+        for (int kk = 0; kk < TK / 16; ++kk)
+          mma_ts(tmem + C::COL_O + 64 * x, p + 16 * kk + 8 * part, vd + x * (C::KV_HALF >> 4) + 128 * kk, id_o,
+                 first && part == 0 && kk == 0 ? 0u : 1u);
     mma_commit(&ct.pv_done[t & 1]);
     mma_commit(&ct.free_[st]);
     scores(t + 1 + NREG, t + 1);
@@ -331,19 +354,19 @@ __device__ __forceinline__ void issue_warp(Group& gm, Control& ct, uint32_t tmem
 
 // ------------------------------------------------------------------ the math warps
 
-template <typename T>
-__device__ __forceinline__ void math_warp(const Args& a, const Plan& plan, int worker, Group& gm, Control& ct,
-                                          uint32_t tmem, float* __restrict__ part_o, float2* __restrict__ part_mz) {
+template <typename T, typename C>
+__device__ __forceinline__ void math_warp(const Args& a, const Plan& plan, int worker, typename C::Group& gm,
+                                          typename C::Control& ct, uint32_t tmem, float* __restrict__ part_o, float2* __restrict__ part_mz) {
   volatile int* ab = &ct.gave_up;
   const int warp = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31, r = warp * 32 + lane;
-  const uint32_t lanes = (uint32_t)(warp * 32) << 16, t_o = tmem + COL_O + lanes;
+  const uint32_t lanes = (uint32_t)(warp * 32) << 16, t_o = tmem + C::COL_O + lanes;
   float m = -INFINITY, carry_s = kMasked, carry_b = 0.f, scale = 0.f;
   float2 z2 = splat2(0.f);
   int pos = -1, i_min = 0, i_max = -1, kt0 = 0, bad = 0;
   bool in_first = true, first_tile = true;
   for (int t = 0;; ++t) {
     if (!mbar_wait_warp(&ct.full[t % NST], (t / NST) & 1, ab)) return;
-    const Slot& d = ct.ring[t % RING];
+    const typename C::Slot& d = ct.ring[t % RING];
     const int4 head = *reinterpret_cast<const int4*>(&d);
     const int kt = head.x, flags = head.y, base = kt * TK;
     if (flags & kNone) return;
@@ -369,8 +392,8 @@ __device__ __forceinline__ void math_warp(const Args& a, const Plan& plan, int w
         const uint8_t* q = gm.q[flags & kQ1 ? 1 : 0] + r * 128;
         float2 s = splat2(0.f);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          const uint4 x = *reinterpret_cast<const uint4*>(q + ((c ^ (r & 7)) << 4));
+        for (int c = 0; c < C::DP / 8; ++c) {
+          const uint4 x = *reinterpret_cast<const uint4*>(q + (c >> 3) * C::Q_HALF + (((c & 7) ^ (r & 7)) << 4));
           const uint4 y = *reinterpret_cast<const uint4*>(d.k_before + 16 * c);
           s = fma2(unpack2<T>(x.x), unpack2<T>(y.x), s);
           s = fma2(unpack2<T>(x.y), unpack2<T>(y.y), s);
@@ -419,7 +442,7 @@ __device__ __forceinline__ void math_warp(const Args& a, const Plan& plan, int w
           if (!mbar_wait_warp(&ct.pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1, ab)) return;
           tc_fence_after();
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
+          for (int half = 0; half < C::DP / 32; ++half) {
             uint32_t o[32];
             tmem_ld32(t_o + 32 * half, o);
             tmem_ld_wait();
@@ -461,56 +484,62 @@ __device__ __forceinline__ void math_warp(const Args& a, const Plan& plan, int w
       if (t > 0 && !mbar_wait_warp(&ct.pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1, ab)) return;
       if (!mbar_wait_warp(&ct.pv_done[t & 1], (t >> 1) & 1, ab)) return;
       tc_fence_after();
-      uint32_t o[2][32];
-      tmem_ld32(t_o, o[0]);
-      tmem_ld32(t_o + 32, o[1]);
-      tmem_ld_wait();
-      tmem_reg_fence(o[0]);
-      tmem_reg_fence(o[1]);
-      tc_fence_before();
       const int rows = d.n * plan.group, row = d.rt * BR + r;
-      if (row < rows) {
-        const bool whole = kt0 == 0 && kt + 1 == head.w;
-        const int key = base + TK - 1;                      // the key whose weight is still carried
-        const float m2 = m == -INFINITY ? 0.f : m * kLog2e;
-        const float cap = key == pos ? 0.5f * ex2_approx(fmaf(carry_s, kLog2e, -m2)) : 0.f;
-        // beyond the row's own key the weight is 0, and V may hold anything
-        const float w = key <= pos ? carry_b + cap : 0.f;
-        float z = z2.x + z2.y + cap;
-        if (bad) z = __int_as_float(0x7fffffff);
-        const float inv = 1.f / z;
-        const long long prow = ((long long)worker * 2 + (in_first ? 0 : 1)) * BR + r;
-        const int tk = row / plan.group;
-        T* dst = (T*)a.o + ((size_t)(d.start + tk) * a.H + (size_t)d.h * plan.group + (row - tk * plan.group)) * a.D;
+      const bool whole = kt0 == 0 && kt + 1 == head.w;
+      const int key = base + TK - 1;                      // the key whose weight is still carried
+      const float m2 = m == -INFINITY ? 0.f : m * kLog2e;
+      const float cap = key == pos ? 0.5f * ex2_approx(fmaf(carry_s, kLog2e, -m2)) : 0.f;
+      // beyond the row's own key the weight is 0, and V may hold anything
+      const float w = key <= pos ? carry_b + cap : 0.f;
+      float z = z2.x + z2.y + cap;
+      if (bad) z = __int_as_float(0x7fffffff);
+      const float inv = 1.f / z;
+      const long long prow = ((long long)worker * 2 + (in_first ? 0 : 1)) * BR + r;
+      const int tk = row / plan.group;
+      T* dst = (T*)a.o + ((size_t)(d.start + tk) * a.H + (size_t)d.h * plan.group + (row - tk * plan.group)) * a.D;
+      // 64 columns at a time
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          float y[8];
+      for (int half = 0; half < C::HALVES; ++half) {
+        uint32_t o[2][32];
+        tmem_ld32(t_o + 64 * half, o[0]);
+        tmem_ld32(t_o + 64 * half + 32, o[1]);
+        tmem_ld_wait();
+        tmem_reg_fence(o[0]);
+        tmem_reg_fence(o[1]);
+        if (row < rows) {
 #pragma unroll
-          for (int x = 0; x < 8; ++x) y[x] = __uint_as_float(o[(8 * c + x) >> 5][(8 * c + x) & 31]);
-          if (w != 0.f) {
-            const uint4 v = *reinterpret_cast<const uint4*>(d.v_last + 16 * c);
-            const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
+          for (int c8 = 0; c8 < 8; ++c8) {
+            const int c = 8 * half + c8;
+            float y[8];
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-              const float2 vv = unpack2<T>(vw[x]);
-              y[2 * x] = fmaf(w, vv.x, y[2 * x]);
-              y[2 * x + 1] = fmaf(w, vv.y, y[2 * x + 1]);
+            for (int x = 0; x < 8; ++x) y[x] = __uint_as_float(o[(8 * c8 + x) >> 5][(8 * c8 + x) & 31]);
+            if (w != 0.f) {
+              const uint4 v = *reinterpret_cast<const uint4*>(d.v_last + 16 * c);
+              const uint32_t vw[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                const float2 vv = unpack2<T>(vw[x]);
+                y[2 * x] = fmaf(w, vv.x, y[2 * x]);
+                y[2 * x + 1] = fmaf(w, vv.y, y[2 * x + 1]);
+              }
+            }
+            if (!whole) {
+              *reinterpret_cast<float4*>(part_o + prow * C::DP + 8 * c) = make_float4(y[0], y[1], y[2], y[3]);
+              *reinterpret_cast<float4*>(part_o + prow * C::DP + 8 * c + 4) = make_float4(y[4], y[5], y[6], y[7]);
+            } else if (8 * c < a.D) {
+              // z = 0: the row sees no key
+              const bool none = z == 0.f;
+              *reinterpret_cast<uint4*>(dst + 8 * c) =
+                  none ? make_uint4(0u, 0u, 0u, 0u)
+                       : make_uint4(pack2<T>(y[0] * inv, y[1] * inv), pack2<T>(y[2] * inv, y[3] * inv),
+                                    pack2<T>(y[4] * inv, y[5] * inv), pack2<T>(y[6] * inv, y[7] * inv));
             }
           }
-          if (!whole) {
-            *reinterpret_cast<float4*>(part_o + prow * 64 + 8 * c) = make_float4(y[0], y[1], y[2], y[3]);
-            *reinterpret_cast<float4*>(part_o + prow * 64 + 8 * c + 4) = make_float4(y[4], y[5], y[6], y[7]);
-          } else if (8 * c < a.D) {
-            // z = 0: the row sees no key
-            const bool none = z == 0.f;
-            *reinterpret_cast<uint4*>(dst + 8 * c) =
-                none ? make_uint4(0u, 0u, 0u, 0u)
-                     : make_uint4(pack2<T>(y[0] * inv, y[1] * inv), pack2<T>(y[2] * inv, y[3] * inv),
-                                  pack2<T>(y[4] * inv, y[5] * inv), pack2<T>(y[6] * inv, y[7] * inv));
-          }
         }
-        if (!whole) part_mz[prow] = make_float2(m, z);
+        __syncwarp();
       }
+      tc_fence_before();
+      if (!whole && row < rows) part_mz[prow] = make_float2(m, z);
       __syncwarp();
     }
     if (flags & kEnd) return;
@@ -519,17 +548,20 @@ __device__ __forceinline__ void math_warp(const Args& a, const Plan& plan, int w
 
 // ------------------------------------------------------------------ the kernel
 
-template <typename T>
-__global__ void __launch_bounds__(THREADS, 1)
+template <typename T, typename C>
+__global__ void __launch_bounds__(C::THREADS, 1)
     tc_kernel(const __grid_constant__ Args a, const __grid_constant__ Plan plan, const __grid_constant__ Maps maps,
               float* __restrict__ part_o, float2* __restrict__ part_mz, Meta* __restrict__ meta) {
   extern __shared__ __align__(1024) uint8_t smem[];
   pdl_wait();
   pdl_launch_dependents();
+  using Group = typename C::Group;
+  using Control = typename C::Control;
+  constexpr int GROUPS = C::GROUPS, MATH_WARPS = C::MATH_WARPS;
   Group* groups = reinterpret_cast<Group*>(smem);
   Control* controls = reinterpret_cast<Control*>(smem + GROUPS * sizeof(Group));
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(smem + GROUPS * (sizeof(Group) + sizeof(Control)));
-  unsigned* prefix = reinterpret_cast<unsigned*>(smem + kSmem);
+  unsigned* prefix = reinterpret_cast<unsigned*>(smem + C::SMEM);
   const int wid = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int role = wid < MATH_WARPS ? 0 : wid < MATH_WARPS + 4 ? 1 : 2;
   const int group = role == 0 ? wid >> 2 : wid & 3;
@@ -537,9 +569,10 @@ __global__ void __launch_bounds__(THREADS, 1)
   if (role == 2 && group < GROUPS) {
     // values behind D stay 0 (copies write D values a row)
     Control& ct = controls[group];
-    for (int x = lane; x < RING * 8; x += 32) {
-      reinterpret_cast<uint4*>(ct.ring[x >> 3].k_before)[x & 7] = make_uint4(0u, 0u, 0u, 0u);
-      reinterpret_cast<uint4*>(ct.ring[x >> 3].v_last)[x & 7] = make_uint4(0u, 0u, 0u, 0u);
+    constexpr int CH = C::DP / 8;
+    for (int x = lane; x < RING * CH; x += 32) {
+      reinterpret_cast<uint4*>(ct.ring[x / CH].k_before)[x % CH] = make_uint4(0u, 0u, 0u, 0u);
+      reinterpret_cast<uint4*>(ct.ring[x / CH].v_last)[x % CH] = make_uint4(0u, 0u, 0u, 0u);
     }
     fence_proxy_async_smem();
   }
@@ -567,23 +600,23 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
   Schedule<BR, TK> sched(a, plan, prefix);   // a barrier of the block among other things
   tc_fence_after();
-  const uint32_t tmem = *tmem_at + COLS * (group < GROUPS ? group : 0);
+  const uint32_t tmem = *tmem_at + C::COLS * (group < GROUPS ? group : 0);
   const unsigned total = sched.total;
   const int worker = blockIdx.x * GROUPS + group, workers = gridDim.x * GROUPS;
   const unsigned per = plan.places_per_worker(total, workers);
 
   if (role == 0) {
-    regs_up<REGS_MATH>();
-    math_warp<T>(a, plan, worker, groups[group], controls[group], tmem, part_o, part_mz);
+    regs_up<C::REGS_MATH>();
+    math_warp<T, C>(a, plan, worker, groups[group], controls[group], tmem, part_o, part_mz);
   } else {
-    regs_down<REGS_OTHER>();
+    regs_down<C::REGS_OTHER>();
     if (group < GROUPS) {
       if (role == 1) {
-        issue_warp<sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value>(groups[group], controls[group], tmem);
+        issue_warp<std::is_same<T, __nv_bfloat16>::value, C>(groups[group], controls[group], tmem);
       } else {
         const unsigned x0 = (unsigned)min((unsigned long long)worker * per, (unsigned long long)total);
         const unsigned x1 = (unsigned)min((unsigned long long)x0 + per, (unsigned long long)total);
-        load_warp<T>(a, plan, maps, sched, worker, per, x0, x1, groups[group], controls[group], meta);
+        load_warp<T, C>(a, plan, maps, sched, worker, per, x0, x1, groups[group], controls[group], meta);
       }
     }
   }
@@ -598,7 +631,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 }  // namespace
 
 int tc_br() { return BR; }
-int tc_groups() { return GROUPS; }
+int tc_groups(int dp) { return dp == 64 ? Config<64>::GROUPS : Config<128>::GROUPS; }
 
 namespace {
 
@@ -669,6 +702,17 @@ bool make_maps(const Args& a, bool bf16, Maps& m) {
                    {&m.page, &m.slot, &m.head}, &m.unit);
 }
 
+template <typename T, typename C>
+cudaError_t launch(const Args& a, const Plan& plan, const Maps& maps, const Pieces& pc) {
+  static_assert(C::SMEM + (kMaxSeqs + 1) * sizeof(unsigned) <= 232448, "shared memory of a block");
+  const cudaError_t e = cudaFuncSetAttribute(tc_kernel<T, C>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)(C::SMEM + (kMaxSeqs + 1) * sizeof(unsigned)));
+  if (e != cudaSuccess) return e;
+  const size_t smem = C::SMEM + (size_t)(a.seqs + 1) * sizeof(unsigned);
+  return launch_pdl(tc_kernel<T, C>, dim3(num_sms_cached()), dim3(C::THREADS), smem, a.stream, a, plan, maps, pc.o,
+                    pc.mz, pc.meta);
+}
+
 }  // namespace
 
 bool tc_launch(const Args& a, const Plan& plan, int dtype, const Pieces& pc, cudaError_t& e) {
@@ -679,13 +723,8 @@ bool tc_launch(const Args& a, const Plan& plan, int dtype, const Pieces& pc, cud
   if (e != cudaSuccess) return true;
   Maps maps;
   if (!make_maps(a, dtype == 1, maps)) return false;
-  static_assert(kSmem + (kMaxSeqs + 1) * sizeof(unsigned) <= 232448, "shared memory of a block");
-  auto kern = dtype == 1 ? tc_kernel<__nv_bfloat16> : tc_kernel<__half>;
-  e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           (int)(kSmem + (kMaxSeqs + 1) * sizeof(unsigned)));
-  if (e != cudaSuccess) return true;
-  const size_t smem = kSmem + (size_t)(a.seqs + 1) * sizeof(unsigned);
-  e = launch_pdl(kern, dim3(num_sms_cached()), dim3(THREADS), smem, a.stream, a, plan, maps, pc.o, pc.mz, pc.meta);
+  if (a.D <= 64) e = dtype == 1 ? launch<__nv_bfloat16, Config<64>>(a, plan, maps, pc) : launch<__half, Config<64>>(a, plan, maps, pc);
+  else e = dtype == 1 ? launch<__nv_bfloat16, Config<128>>(a, plan, maps, pc) : launch<__half, Config<128>>(a, plan, maps, pc);
   return true;
 }
 

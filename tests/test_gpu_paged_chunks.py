@@ -26,7 +26,8 @@ def run_and_check(dtype, case):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("heads,kv_heads,dim,page", [(2, 2, 64, 16), (8, 2, 64, 64), (6, 2, 56, 7), (5, 1, 8, 1),
-                                                     (3, 3, 64, 128), (64, 1, 16, 32), (128, 1, 64, 16)])
+                                                     (3, 3, 64, 128), (64, 1, 16, 32), (128, 1, 64, 16),
+                                                     (2, 2, 128, 16), (6, 2, 80, 24), (4, 1, 120, 1)])
 def test_shapes(dtype, heads, kv_heads, dim, page):
     case = make_case(dtype, heads, kv_heads, dim, page, [(70, 70), (129, 191), (1, 40), (127, 500)], seed=dim + page)
     run_and_check(dtype, case)
@@ -39,17 +40,18 @@ def test_shapes(dtype, heads, kv_heads, dim, page):
     [(300, 4096)],
     [(200, 200 + L) for L in (0, 1, 31, 32, 33, 95, 96, 97)],
 ])
-def test_lengths(dtype, seqs):
-    run_and_check(dtype, make_case(dtype, 2, 1, 64, 16, seqs, seed=len(seqs)))
+@pytest.mark.parametrize("dim", [64, 128])
+def test_lengths(dtype, dim, seqs):
+    run_and_check(dtype, make_case(dtype, 2, 1, dim, 16, seqs, seed=len(seqs)))
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("seed", range(6))
-def test_random_batches(dtype, seed):
+@pytest.mark.parametrize("seed,dims", [(s, (8, 24, 40, 64)) for s in range(6)] + [(s, (72, 80, 104, 128)) for s in range(6, 12)])
+def test_random_batches(dtype, seed, dims):
     r = random.Random(seed)
     kv_heads = r.choice([1, 2, 3])
     heads = kv_heads * r.choice([1, 2, 3, 4, 7])
-    dim, page = r.choice([8, 24, 40, 64]), r.choice([1, 5, 16, 24, 64])
+    dim, page = r.choice(dims), r.choice([1, 5, 16, 24, 64])
     seqs = []
     for _ in range(r.randint(1, 12)):
         n = r.choice([0, 1, 1, 3, r.randint(1, 40), r.randint(65, 260)])
@@ -59,11 +61,11 @@ def test_random_batches(dtype, seed):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (6, 2)])
-def test_neighbours_and_a_tail_do_not_reach_a_sequence(dtype, heads, kv_heads):
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (6, 2, 64), (4, 2, 96), (6, 2, 128)])
+def test_neighbours_and_a_tail_do_not_reach_a_sequence(dtype, heads, kv_heads, dim):
     """A unit's rows go on behind its sequence's last in the buffer: what stands there stays out of the answers,
     and the rows behind the last sequence keep what they held."""
-    case = make_case(dtype, heads, kv_heads, 64, 16, [(70, 100), (75, 90), (0, 5), (90, 90)], seed=11, tail=40)
+    case = make_case(dtype, heads, kv_heads, dim, 16, [(70, 100), (75, 90), (0, 5), (90, 90)], seed=11, tail=40)
     case["q"][70:145] = float("nan")
     case["q"][235:] = float("inf")
     out = torch.full_like(case["q"], 7.0)
@@ -79,7 +81,7 @@ def test_neighbours_and_a_tail_do_not_reach_a_sequence(dtype, heads, kv_heads):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("dim", [64, 40])
+@pytest.mark.parametrize("dim", [64, 40, 128, 88])
 def test_strided_cache_and_queries(dtype, dim):
     case = make_case(dtype, 4, 2, dim, 16, [(5, 77), (100, 130), (70, 70)], seed=5, cache_layout="psgd")
     want = exact(case)
@@ -159,10 +161,11 @@ def test_offsets_beyond_32_bits(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_bad_lengths_and_pages_are_refused_by_the_kernel(dtype):
+@pytest.mark.parametrize("dim", [64, 128])
+def test_bad_lengths_and_pages_are_refused_by_the_kernel(dtype, dim):
     lib = _native.lib()
     lib.ca_device_status(1)
-    base = make_case(dtype, 4, 2, 64, 16, [(1, 40), (90, 120), (2, 3), (70, 100)], seed=12)
+    base = make_case(dtype, 4, 2, dim, 16, [(1, 40), (90, 120), (2, 3), (70, 100)], seed=12)
     want, mag = exact(base)
     rows = slice(1, 91)
     for what in ("page", "page_neg", "len", "len_neg"):
