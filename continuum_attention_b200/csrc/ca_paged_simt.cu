@@ -440,19 +440,32 @@ cudaError_t launch_main(const Args& a, const Plan& plan, const Pieces& pc) {
                     pc.meta);
 }
 
+// Whether a batch with chunks gives its short sequences (at most One's rows) a launch of their own: where they have to
+// be the most, since there are fewer than 32 rows a sequence.  63 sequences of one row and one of 200 over 8192 keys,
+// 16 heads of 64: 1253 us, in one launch 4981; 8 prompts of 40 .. 192 rows would pay 2 of their 25 us for it.
+bool splits(const Args& a) {
+  const long long group = a.H / a.G;
+  return a.max_q_len * group > 16 && a.seqs > 1 && a.rows * group < 32LL * a.seqs;
+}
+
 template <int DP>
 cudaError_t forward_dp(const Args& a, void* workspace) {
   Plan plan = make_plan(a);
   plan.unit_cost = kUnitCost;
   char* ws = (char*)workspace;
-  // every sequence in the form that suits the longest: 64-row units leave threads of a short one idle, but
-  // in 32 bits the loads and FMAs of a tile are the same whatever its rows
   const long long rows = (long long)a.max_q_len * plan.group;
   auto run = [&](auto form) {
     using C = decltype(form);
-    const Pieces pc = carve<DP>(ws, C::BR, C::PER_SM);
-    const cudaError_t e = launch_main<C>(a, plan, pc);
-    return e != cudaSuccess ? e : launch_merge<float, DP>(a, plan, pc, Pieces{});
+    Pieces pc = carve<DP>(ws, C::BR, C::PER_SM), few{};
+    Plan tall = plan;
+    if (splits(a)) tall.row_lo = One<DP>::BR + 1;
+    cudaError_t e = launch_main<C>(a, tall, pc);
+    if (e == cudaSuccess && splits(a)) {
+      few = carve<DP>(ws + pieces_bytes<DP>(C::BR, C::PER_SM), One<DP>::BR, One<DP>::PER_SM);
+      plan.row_hi = One<DP>::BR;
+      e = launch_main<One<DP>>(a, plan, few);
+    }
+    return e != cudaSuccess ? e : launch_merge<float, DP>(a, plan, pc, few);
   };
   return with_form<DP>(rows, run);
 }
@@ -462,12 +475,14 @@ cudaError_t forward_dp(const Args& a, void* workspace) {
 size_t simt_workspace_bytes(long long max_q_len, long long H, long long G, long long D) {
   auto bytes = [](auto form) {
     using C = decltype(form);
-    return pieces_bytes<C::DP>(C::BR, C::PER_SM);
+    // (a batch with chunks may take two launches)
+    return pieces_bytes<C::DP>(C::BR, C::PER_SM) +
+           (C::BR > 16 ? pieces_bytes<C::DP>(One<C::DP>::BR, One<C::DP>::PER_SM) : 0);
   };
   return D <= 64 ? with_form<64>(max_q_len * (H / G), bytes) : with_form<128>(max_q_len * (H / G), bytes);
 }
 
-int simt_launches(const Args&) { return 2; }
+int simt_launches(const Args& a) { return splits(a) ? 3 : 2; }
 
 cudaError_t simt_forward(const Args& a, void* workspace) {
   return a.D <= 64 ? forward_dp<64>(a, workspace) : forward_dp<128>(a, workspace);
