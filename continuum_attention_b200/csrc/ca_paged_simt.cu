@@ -417,10 +417,11 @@ __global__ void __launch_bounds__(C::NT, C::PER_SM)
 // Rows of a unit: 4 or 16 for decoding, 64 for chunks.  In the decoding forms a warp's lanes are the tile's 32
 // keys, then its output columns.  64 sequences of one row over 8192 keys (16 heads of 64): units of 4 rows 955 us
 // (4.5 TB/s; on one warp 1220, on four 1050), of 16 rows 3230; 16 rows over 4096 keys (16 sequences, 32 heads on
-// 2 of 64): 46 us, with threads in 16 x 8 75.
+// 2 of 64): 46 us, with threads in 16 x 8 75.  Prompts of 2 x 1024 tokens, 16 heads of 128: 371 us in 8 x 32, 395 in
+// 16 x 16, which is better with 64 values (2 x 2048 tokens 639 and 708).
 template <int DP> using One = Config<DP, 4, 2, 32, DP == 64 ? 5 : 3>;
 template <int DP> using Few = Config<DP, 16, 4, 32, DP == 64 ? 4 : 2>;
-template <int DP> using Many = Config<DP, 64, 16, 16, DP == 64 ? 2 : 1>;
+template <int DP> using Many = Config<DP, 64, DP == 64 ? 16 : 8, DP == 64 ? 16 : 32, DP == 64 ? 2 : 1>;
 constexpr int kUnitCost = 1;
 
 template <int DP, typename F>
