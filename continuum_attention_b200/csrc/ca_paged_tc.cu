@@ -30,8 +30,9 @@
 // issue one in 55% of the cycles, with three math warps on each (counters at 511 rows over
 // 16001 keys; tensor pipe 13% busy, transcendental pipe 35%, HBM 5%).  Without the moments that case
 // takes 127 us, without moments and copies 91.  Tried and slower: two workers with tiles of 64 keys (205
-// against 189 us at that case), four workers whose products and copies one warp does (220; registers
-// for two regions only), one such warp for each of three workers (187 against 179).
+// against 189 us at that case), tiles of 48 keys (189 against 170), four workers with 96 registers a thread
+// (216) or with one warp for products and copies (220), one such warp for each of three workers (187
+// against 179).
 // Measured (16 heads of 64): prompts of 2 x 2048 tokens 112 us (mma.sync form 148), 511 rows over
 // 16001 keys 171 us (235), 23 sequences of 0 .. 300 rows over up to 4000 keys, 4 query heads a key
 // head, 82 us (102).  Heads of 128, with two workers and one unit's queries at a time: the first two 169 (226)
