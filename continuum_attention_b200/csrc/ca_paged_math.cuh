@@ -9,6 +9,14 @@ namespace paged {
 
 constexpr float kRescaleNats = 8.f;   // the reference maximum moves when it grows by more
 
+// The reference that exponentials are taken from, in log2 units, for the reference maximum m.  In f16 weights stand
+// 2^4 above it: the largest is then e^8 2^4 = 47700 (a weight is at most its segments' larger exponential), and
+// small ones are whole down to 2^-18 of that of m itself instead of 2^-14.
+template <typename T>
+__device__ __forceinline__ float reference2(float m) {
+  return m == -INFINITY ? 0.f : std::is_same<T, __half>::value ? fmaf(m, kLog2e, -4.f) : m * kLog2e;
+}
+
 // a weight pair as two 16-bit parts: hi + lo keeps 16 bits (bf16) or 21 (f16)
 template <typename T>
 __device__ __forceinline__ void split2(float2 w, uint32_t& hi, uint32_t& lo);
@@ -22,8 +30,8 @@ __device__ __forceinline__ void split2<__nv_bfloat16>(float2 w, uint32_t& hi, ui
 }
 template <>
 __device__ __forceinline__ void split2<__half>(float2 w, uint32_t& hi, uint32_t& lo) {
-  // 10 bits of mantissa by truncation, exact in f16 above its subnormals (2^-14 of the largest weight, where
-  // hi rounds by 2^-25 at most); the remainder is exact
+  // 10 bits of mantissa by truncation, exact in f16 above its subnormals (below 2^-14 hi rounds by 2^-25 at
+  // most); the remainder is exact
   const float2 t = make_float2(__uint_as_float(__float_as_uint(w.x) & 0xffffe000u),
                                __uint_as_float(__float_as_uint(w.y) & 0xffffe000u));
   const __half2 h = __floats2half2_rn(t.x, t.y);
@@ -40,6 +48,13 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) {
 }
 template <>
 __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
+// A segment's M0 and M1 from their closed forms; near d = 0 from M1's series, el ps, and M0 = e - d M1.  (The latter
+// everywhere would cost a select less, and far from 0 all but e 2^-22 of M0's precision.)
+__device__ __forceinline__ void near_zero(float& m0, float& m1, float nd, float el, float ps, float e, float thr) {
+  asm("{\n\t.reg .pred p;\n\t.reg .f32 t;\n\tabs.f32 t, %2;\n\tsetp.lt.f32 p, t, %6;\n\t"
+      "@p mul.f32 %1, %3, %4;\n\t@p fma.rn.f32 %0, %2, %1, %5;\n\t}"
+      : "+f"(m0), "+f"(m1) : "f"(nd), "f"(el), "f"(ps), "f"(e), "f"(thr));
+}
 // Weights of one lane's run of one row, as two 16-bit parts.  sv[j] = scaled scores of keys (kc + j, kc + NJ + j),
 // sL that of key kc - 1, m2 the reference maximum in log2 units.  Parts j weigh keys (kc - 1 + j, kc + NJ - 1 + j);
 // first is the pair of place 0, unsplit, but for the mass that ends at key kc - 1, which is the lane's to
@@ -79,15 +94,13 @@ __device__ __forceinline__ void weigh(const float2 (&sv)[NJ], float m2, float sL
 #pragma unroll
     for (int t = 0; t < 4; ++t) w[t] = mul2(sub2(t ? e[t - 1] : el0, e[t]), rn[t]);                 // M0
 #pragma unroll
-    for (int t = 0; t < 4; ++t) w[t] = mul2(sub2(w[t], e[t]), rn[t]);                               // M1, closed
+    for (int t = 0; t < 4; ++t) m1[t] = mul2(sub2(w[t], e[t]), rn[t]);                              // M1, closed
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const float2 el = t ? e[t - 1] : el0;
-      m1[t] = make_float2(sel_series(w[t].x, nd[t].x, el.x, ps[t].x, kSeriesMaxFwd),
-                          sel_series(w[t].y, nd[t].y, el.y, ps[t].y, kSeriesMaxFwd));
+      near_zero(w[t].x, m1[t].x, nd[t].x, el.x, ps[t].x, e[t].x, kSeriesMaxFwd);
+      near_zero(w[t].y, m1[t].y, nd[t].y, el.y, ps[t].y, e[t].y, kSeriesMaxFwd);
     }
-#pragma unroll
-    for (int t = 0; t < 4; ++t) w[t] = fma2(nd[t], m1[t], e[t]);                                   // M0
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       z2 = add2(z2, w[t]);

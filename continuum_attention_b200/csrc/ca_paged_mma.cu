@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
             }
           }
         }
-        const float m2 = m[u] == -INFINITY ? 0.f : m[u] * kLog2e;
+        const float m2 = reference2<T>(m[u]);
         const int left = (lane & ~3) | ((lane + 3) & 3);
         float got = __shfl_sync(0xffffffffu, s[u][NJ - 1].y, left);
         const float sL = c4 == 0 ? carry_s[u] : got;
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
 #pragma unroll
       for (int u = 0; u < RS; ++u) {
         const int row = row0 + r8 + 8 * u;
-        const float m2 = m[u] == -INFINITY ? 0.f : m[u] * kLog2e;
+        const float m2 = reference2<T>(m[u]);
         float w = __shfl_sync(0xffffffffu, carry_b[u], lane & ~3);
         const float ls = __shfl_sync(0xffffffffu, carry_s[u], lane & ~3);
         const float cap = key == pos[u] ? 0.5f * ex2_approx(fmaf(ls, kLog2e, -m2)) : 0.f;

@@ -455,7 +455,7 @@ __device__ __forceinline__ void math_warp(const Args& a, const Plan& plan, int w
           tmem_st_wait();
         }
       }
-      const float m2 = m == -INFINITY ? 0.f : m * kLog2e;
+      const float m2 = reference2<T>(m);
       const int lowest = flags & kFirst ? base : base - 1;
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
@@ -488,7 +488,7 @@ __device__ __forceinline__ void math_warp(const Args& a, const Plan& plan, int w
       const int rows = d.n * plan.group, row = d.rt * BR + r;
       const bool whole = kt0 == 0 && kt + 1 == head.w;
       const int key = base + TK - 1;                      // the key whose weight is still carried
-      const float m2 = m == -INFINITY ? 0.f : m * kLog2e;
+      const float m2 = reference2<T>(m);
       const float cap = key == pos ? 0.5f * ex2_approx(fmaf(carry_s, kLog2e, -m2)) : 0.f;
       // beyond the row's own key the weight is 0, and V may hold anything
       const float w = key <= pos ? carry_b + cap : 0.f;

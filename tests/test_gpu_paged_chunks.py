@@ -140,10 +140,11 @@ def test_flat_and_steep_scores(dtype, qk_mag):
     # so are the weights
     got = out.double().cpu()
     bound = want.abs() * torch.finfo(DTYPES[dtype]).eps / 2 * 1.001 + 2 * (3e-4 + 4e-5) * mag + 2.0 ** -25
-    # A steep segment of ends e >= e' at distance d: M1 = (M0 - e) / d carries the reciprocal's 2^-23 and two
-    # roundings of 2^-24, 2^-22 together, and M0 = e - d M1 takes d M1 2^-22 < e 2^-22 of it as an absolute
-    # error: of the mass and of the weight M0 - M1 of the segment's other key, whose own size is only
-    # e / d^2.  Summed, over the mass: steepness * 2^-22, times that key's |v| and, for the mass, |y|.
+    # A steep segment of ends e >= e' at distance |d| > 1: M0 = (e - e') / d and M1 = (e - M0) / d carry the
+    # reciprocal's 2^-23 and two roundings of 2^-24, 2^-22 of themselves, which are below e.  The weight
+    # M0 - M1 of the segment's other key is only e / d^2 and takes e 2^-22 of it as an absolute error
+    # (formed as M0 = e - d M1, the mass would as well).  Summed, over the mass: steepness * 2^-22, times
+    # that key's |v| and, for the mass, |y|.
     top_v = max(v.abs().max().item() for v in case["values"])
     steep = torch.cat([steepness(case, s) for s in range(2)])
     bound += steep[..., None] * 2.0 ** -22 * 2 * top_v
