@@ -54,6 +54,7 @@ SIGNATURES = {
     "ca_rotary_qkv_backward": (_int, [_vp, _vp, _vp, _vp, _vp, _i64, _vp] + [_i64] * 7 + [_int, _int, _vp]),
     "ca_rotary_append": (_int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp]
                          + [_i64] * 10 + [_int, _int, _vp]),
+    "ca_selftest_paged_wait_limit": (_int, [_i64]),
     "ca_paged_workspace_size": (_sz, [_i64] * 5 + [_int]),
     "ca_paged_forward": (_int, [_vp, _i64, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _sz]
                          + [_i64] * 9 + [_int, _vp]),

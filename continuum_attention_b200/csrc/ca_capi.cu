@@ -553,6 +553,15 @@ int ca_rotary_append(const void* qkv, int64_t qkv_stride, const float* cos_sin, 
   return ok();
 }
 
+static thread_local unsigned long long g_paged_wait_ns = ca::paged::kWaitNs;
+
+int ca_selftest_paged_wait_limit(int64_t limit_us) {
+  if (limit_us > 10000000)
+    return fail(CA_ERR_INVALID_ARGUMENT, "ca_selftest_paged_wait_limit: limit_us=%lld above 1e7", (long long)limit_us);
+  g_paged_wait_ns = limit_us < 0 ? ca::paged::kWaitNs : (unsigned long long)limit_us * 1000ull;
+  return ok();
+}
+
 size_t ca_paged_workspace_size(int64_t num_seqs, int64_t max_q_len, int64_t heads, int64_t kv_heads, int64_t D,
                                int dtype) {
   if (num_seqs <= 0 || max_q_len <= 0 || heads <= 0 || kv_heads <= 0 || D <= 0) return 0;
@@ -606,7 +615,7 @@ int ca_paged_forward(const void* q, int64_t q_token_stride, int64_t q_head_strid
   ca::paged::Args a{q, q_token_stride, q_head_stride, k_cache, v_cache, page_stride, head_stride, slot_stride,
                     page_table, page_table_stride, kv_lens, q_starts, log_gain, o, (int)num_rows, (int)num_seqs,
                     (int)max_q_len, (int)heads, (int)kv_heads, (int)D, (int)num_pages, (int)page_size,
-                    (int)pages_per_seq, (float)(1.0 / std::sqrt((double)D)), (cudaStream_t)stream};
+                    (int)pages_per_seq, (float)(1.0 / std::sqrt((double)D)), g_paged_wait_ns, (cudaStream_t)stream};
   cudaError_t e = ca::paged::forward(a, dtype, workspace);
   if (e != cudaSuccess) return cuda_fail(e, fn);
   g_last_launches = ca::paged::launches(a, dtype);

@@ -204,9 +204,11 @@ struct Args {
   int rows, seqs, max_q_len, H, G, D;
   int num_pages, page_size, pages_per_seq;
   float inv_sqrt_d;
+  unsigned long long wait_ns;   // after which a wait in the kernels gives up
   cudaStream_t stream;
 };
 constexpr int kMaxSeqs = 2048;   // sequences in one call
+constexpr unsigned long long kWaitNs = 2000000000ull;
 size_t workspace_bytes(long long seqs, long long max_q_len, long long H, long long G, long long D, int dtype);
 cudaError_t forward(const Args& a, int dtype, void* workspace);
 int launches(const Args& a, int dtype);

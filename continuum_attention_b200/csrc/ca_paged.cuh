@@ -30,6 +30,7 @@ struct Plan {
   unsigned min_places;     // places of a worker's range, at least
   int unit_cost;          // places that a unit takes before its first tile
   int unit_rows;          // rows that one copy brings
+  unsigned long long wait_ns;   // after which a wait gives up
 
   __device__ __forceinline__ int page_of(int key) const { return page_shift >= 0 ? key >> page_shift : key / page_size; }
   __device__ __forceinline__ unsigned places_per_worker(unsigned total, int workers) const {
@@ -50,6 +51,7 @@ inline Plan make_plan(const Args& a) {
   p.min_places = 1;
   p.unit_cost = 0;
   p.unit_rows = 1;
+  p.wait_ns = a.wait_ns;
   return p;
 }
 

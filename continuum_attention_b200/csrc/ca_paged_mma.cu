@@ -74,22 +74,31 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
                "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(bar), "r"(parity) : "memory");
   return done != 0;
 }
-// Whole warp; gives up after two seconds (the barrier of copies that never land): records the timeout and
+// Whole warp; gives up after limit_ns (the barrier of copies that never land): records the timeout and
 // raises the group's flag, which ends the others' waits too.
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up,
+                                         unsigned long long limit_ns) {
   bool ok = bar_try(bar, parity);
   if (!ok) {
     unsigned long long t0, t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
     while (!(ok = bar_try(bar, parity)) && !*gave_up) {
       asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-      if (t - t0 > 2000000000ull) {
+      if (t - t0 > limit_ns) {
         atomicCAS(&g_status, 0, 5);
         *gave_up = 1;
       }
     }
   }
   return __all_sync(0xffffffffu, ok);
+}
+// the producer's wait for room: with no limit at all it gives up at once, so that a call can be made to
+__device__ __forceinline__ bool room_wait(uint32_t bar, uint32_t parity, volatile int* gave_up,
+                                          unsigned long long limit_ns) {
+  if (limit_ns > 0) return bar_wait(bar, parity, gave_up, limit_ns);
+  atomicCAS(&g_status, 0, 5);
+  *gave_up = 1;
+  return false;
 }
 template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
@@ -227,6 +236,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       if (after_chunks) pdl_wait();
       return;
     }
+    // nothing to join, until the range's last tile says otherwise: the join reads this of every worker, and one
+    // whose wait gives up writes no more
+    if (lane == 0) meta[worker].pieces = 0;
     // `cur` stands at the next tile to be described; a tile's pages are fetched when it is described, one tile
     // before its copies are issued.  Every instruction here counts: the producer shares a scheduler with
     // the consumers.
@@ -235,7 +247,6 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     if (x0 < x1) cur = sched.locate(x0);
     if (cur.at >= x1) {            // no tile's place lies in this range
       if (lane == 0) {
-        meta[worker].pieces = 0;
         descs[0].flags = kNone;
         bar_expect(full, 0);
       }
@@ -307,21 +318,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   int slot_b = 0, stage_b = 0;
   uint32_t empty_parity = 1;      // of the stage's previous use
   describe();
-  for (int k = 0, end = 0; !end; ++k) {
-    if (k >= NST && !bar_wait(empty + 8 * stage_b, empty_parity, gave_up)) {
-      // copies may still be on their way: leave no sooner than they land, or another limit runs out
-      *gave_up = 0;
-      __syncwarp();
-      for (int i = 0; i < NST; ++i) {
-        bar_wait(full + 8 * stage_b, empty_parity, gave_up);
-        if (++stage_b == NST) {
-          stage_b = 0;
-          empty_parity ^= 1;
-        }
-      }
-      if (after_chunks) pdl_wait();
-      return;
-    }
+  int k = 0;
+  for (int end = 0; !end; ++k) {
+    if (k >= NST && !room_wait(empty + 8 * stage_b, empty_parity, gave_up, plan.wait_ns)) break;
     {
       const uint32_t st = g0 + stage_b * C::STAGE, bar = full + 8 * stage_b;
       const int base = d.kt * TK;
@@ -393,6 +392,9 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     }
     if (!end) describe();
   }
+  // every copy has to land before this block's shared memory is another's, where the consumers gave up too
+  volatile int go = 0;
+  for (int u = max(k - NST, 0); u < k; ++u) bar_wait(full + 8 * (u % NST), (u / NST) & 1, &go, kWaitNs);
   if (after_chunks) pdl_wait();
   return;
   }
@@ -422,7 +424,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
   uint32_t parity = 0;
   bool first_tile = true;
   for (int end = 0; !end;) {
-    if (!bar_wait(full + 8 * stage, parity, gave_up)) break;
+    if (!bar_wait(full + 8 * stage, parity, gave_up, plan.wait_ns)) break;
     const Desc& d = descs[slot];
     const int4 head = *reinterpret_cast<const int4*>(&d);
     const int kt = head.x, flags = head.y, len = head.z;

@@ -90,7 +90,7 @@ struct Config {
     uint64_t s_full[NREG];      // its scores are in tensor memory                          (1: commit)
     uint64_t p_ready[NREG];     // its weights are                                          (4: math warps)
     uint64_t pv_done[2];        // P V of tile t and all before it: barrier t & 1           (1: commit)
-    uint64_t drained;           // every product, where a wait gave up                      (1: commit)
+    uint64_t drained;           // every product                                            (1: commit)
     int gave_up;
     Slot ring[RING];
   };
@@ -111,6 +111,14 @@ __device__ __forceinline__ bool mbar_test_warp(uint64_t* bar, uint32_t parity) {
   asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
                "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
   return __all_sync(0xffffffffu, done != 0);
+}
+// the loader's wait for room: with no limit at all it gives up at once, so that a call can be made to; whole warp
+__device__ __forceinline__ bool room_wait_warp(uint64_t* bar, uint32_t parity, volatile int* gave_up,
+                                               unsigned long long limit_ns) {
+  if (limit_ns > 0) return mbar_wait_warp(bar, parity, gave_up, limit_ns);
+  atomicCAS(&g_device_status, 0, 5);
+  *gave_up = 1;
+  return false;
 }
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
@@ -136,12 +144,14 @@ __device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const
                                           Meta* __restrict__ meta) {
   const int lane = threadIdx.x & 31;
   volatile int* ab = &ct.gave_up;
+  // nothing to join, until the range's last tile says otherwise: the join reads this of every worker, and one
+  // whose wait gives up writes no more
+  if (lane == 0) meta[worker].pieces = 0;
   typename Schedule<BR, TK>::Cursor cur;
   cur.at = x1;
   if (x0 < x1) cur = sched.locate(x0);
   if (cur.at >= x1) {              // no tile's place lies in this range
     if (lane == 0) {
-      meta[worker].pieces = 0;
       ct.ring[0].flags = kNone;
       mbar_arrive(&ct.full[0]);
     }
@@ -173,7 +183,7 @@ __device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const
   int t = 0;
   for (; !end; ++t) {
     const int st = t % NST;
-    if (t >= NST && !mbar_wait_warp(&ct.free_[st], (t / NST - 1) & 1, ab)) break;
+    if (t >= NST && !room_wait_warp(&ct.free_[st], (t / NST - 1) & 1, ab, plan.wait_ns)) break;
     const int base = cur.kt * TK;
     const bool opens = first || cur.kt == 0;
     int flags = cur.bad ? kBad : 0;
@@ -192,7 +202,7 @@ __device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const
       // Q of an earlier unit lay in this buffer: its products have to be done (they are known to be where the
       // stage of its last tile has been filled again since)
       const int u = last_tile[C::QBUF - 1];
-      if (u >= 0 && u + NST > t && !mbar_wait_warp(&ct.free_[u % NST], (u / NST) & 1, ab)) break;
+      if (u >= 0 && u + NST > t && !room_wait_warp(&ct.free_[u % NST], (u / NST) & 1, ab, plan.wait_ns)) break;
       bytes += C::Q_BYTES;
       before = -1;
       if (base > 0 && base - 1 < cur.len) {
@@ -285,7 +295,7 @@ __device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const
 // ------------------------------------------------------------------ the issuer
 
 template <bool kBF16, typename C>
-__device__ __forceinline__ void issue_warp(typename C::Group& gm, typename C::Control& ct, uint32_t tmem) {
+__device__ __forceinline__ void issue_warp(const Plan& plan, typename C::Group& gm, typename C::Control& ct, uint32_t tmem) {
   volatile int* ab = &ct.gave_up;
   const uint32_t id_s = make_idesc(BR, TK, kBF16, false), id_o = make_idesc(BR, 64, kBF16, true);
   const uint32_t q0 = smem_u32(gm.q), k0 = smem_u32(gm.k), v0 = smem_u32(gm.v);
@@ -318,7 +328,7 @@ __device__ __forceinline__ void issue_warp(typename C::Group& gm, typename C::Co
       const uint32_t parity = (issued / NST) & 1;
       if (!mbar_test_warp(bar, parity)) {
         if (issued > awaited) return;
-        good = mbar_wait_warp(bar, parity, ab);
+        good = mbar_wait_warp(bar, parity, ab, plan.wait_ns);
         if (!good) return;
       }
       issue_s();
@@ -326,7 +336,7 @@ __device__ __forceinline__ void issue_warp(typename C::Group& gm, typename C::Co
   };
   scores(NREG, 0);
   for (int t = 0; good && t < issued; ++t) {
-    good = mbar_wait_warp(&ct.p_ready[t % NREG], (t / NREG) & 1, ab);
+    good = mbar_wait_warp(&ct.p_ready[t % NREG], (t / NREG) & 1, ab, plan.wait_ns);
     if (!good) break;
     const int st = t % NST;
     const bool first = ct.ring[t % RING].flags & kFirst;
@@ -345,8 +355,9 @@ __device__ __forceinline__ void issue_warp(typename C::Group& gm, typename C::Co
     mma_commit(&ct.free_[st]);
     scores(t + 1 + NREG, t + 1);
   }
-  if (!good) {
-    // products may still be running: they end before tensor memory is given back
+  if (issued > 0) {
+    // products may still be running where a wait gave up, the math warps' or this one's: they end before tensor
+    // memory is given back
     volatile int go = 0;
     mma_commit(&ct.drained);
     mbar_wait_warp(&ct.drained, 0, &go);
@@ -366,7 +377,7 @@ __device__ __forceinline__ void math_warp(const Args& a, const Plan& plan, int w
   int pos = -1, i_min = 0, i_max = -1, kt0 = 0, bad = 0;
   bool in_first = true, first_tile = true;
   for (int t = 0;; ++t) {
-    if (!mbar_wait_warp(&ct.full[t % NST], (t / NST) & 1, ab)) return;
+    if (!mbar_wait_warp(&ct.full[t % NST], (t / NST) & 1, ab, plan.wait_ns)) return;
     const typename C::Slot& d = ct.ring[t % RING];
     const int4 head = *reinterpret_cast<const int4*>(&d);
     const int kt = head.x, flags = head.y, base = kt * TK;
@@ -405,7 +416,7 @@ __device__ __forceinline__ void math_warp(const Args& a, const Plan& plan, int w
       }
     }
     bad |= flags & kBad;
-    if (!mbar_wait_warp(&ct.s_full[t % NREG], (t / NREG) & 1, ab)) return;
+    if (!mbar_wait_warp(&ct.s_full[t % NREG], (t / NREG) & 1, ab, plan.wait_ns)) return;
     tc_fence_after();
     const uint32_t t_s = tmem + TK * (t % NREG) + lanes;
     if (base - 1 <= i_max && i_max >= 0) {
@@ -440,7 +451,7 @@ __device__ __forceinline__ void math_warp(const Args& a, const Plan& plan, int w
           // O holds P V of the piece's tiles so far: the last of them has to have landed.  Its barrier is
           // neither a phase further on (that needs P of tile t + 1) nor behind (P V of tile t - 3
           // completed before the scores of tile t)
-          if (!mbar_wait_warp(&ct.pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1, ab)) return;
+          if (!mbar_wait_warp(&ct.pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1, ab, plan.wait_ns)) return;
           tc_fence_after();
 #pragma unroll
           for (int half = 0; half < C::DP / 32; ++half) {
@@ -482,8 +493,8 @@ __device__ __forceinline__ void math_warp(const Args& a, const Plan& plan, int w
 
     if (flags & kLast) {
       // (P V of tile t - 1 first: only then can this tile's phase be told from the one before)
-      if (t > 0 && !mbar_wait_warp(&ct.pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1, ab)) return;
-      if (!mbar_wait_warp(&ct.pv_done[t & 1], (t >> 1) & 1, ab)) return;
+      if (t > 0 && !mbar_wait_warp(&ct.pv_done[(t - 1) & 1], ((t - 1) >> 1) & 1, ab, plan.wait_ns)) return;
+      if (!mbar_wait_warp(&ct.pv_done[t & 1], (t >> 1) & 1, ab, plan.wait_ns)) return;
       tc_fence_after();
       const int rows = d.n * plan.group, row = d.rt * BR + r;
       const bool whole = kt0 == 0 && kt + 1 == head.w;
@@ -613,7 +624,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     regs_down<C::REGS_OTHER>();
     if (group < GROUPS) {
       if (role == 1) {
-        issue_warp<std::is_same<T, __nv_bfloat16>::value, C>(groups[group], controls[group], tmem);
+        issue_warp<std::is_same<T, __nv_bfloat16>::value, C>(plan, groups[group], controls[group], tmem);
       } else {
         const unsigned x0 = (unsigned)min((unsigned long long)worker * per, (unsigned long long)total);
         const unsigned x1 = (unsigned)min((unsigned long long)x0 + per, (unsigned long long)total);

@@ -369,6 +369,15 @@ int ca_device_status(int reset);
  */
 int ca_selftest_wait_timeout(int64_t limit_us, void* stream);
 
+/*
+ * Diagnostics (no reference counterpart): the limit of the device-side waits in the
+ * ca_paged_forward calls that this thread makes from here on, in microseconds (at most 1e7;
+ * negative: the ordinary two seconds; 0: in bf16 and f16, where copies are awaited, every worker
+ * that has more tiles than fit its shared memory gives up).  A call whose wait gives up records CA_ERR_DEVICE_TIMEOUT, leaves the rows of o that it did not come to
+ * undefined, writes nothing but o and its workspace, and ends in order.
+ */
+int ca_selftest_paged_wait_limit(int64_t limit_us);
+
 #ifdef __cplusplus
 }
 #endif
