@@ -511,6 +511,8 @@ static int check_cache(const char* fn, int64_t page_stride, int64_t head_stride,
   if (page_size < 1) return fail(CA_ERR_INVALID_ARGUMENT, "%s: page_size must be >= 1", fn);
   if (rows > 0x7fffffffLL || seqs >= 0x7fffffffLL || num_pages > 0x7fffffffLL)
     return fail(CA_ERR_UNSUPPORTED, "%s: rows, sequences and pages are limited to 2^31-1", fn);
+  if (page_size > (1LL << 30))
+    return fail(CA_ERR_UNSUPPORTED, "%s: page_size=%lld exceeds 2^30", fn, (long long)page_size);
   if (pages_per_seq > 0 && page_size > (1LL << 30) / pages_per_seq)
     return fail(CA_ERR_UNSUPPORTED, "%s: pages_per_seq * page_size = %lld * %lld keys exceed 2^30", fn,
                 (long long)pages_per_seq, (long long)page_size);
