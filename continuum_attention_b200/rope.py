@@ -37,8 +37,9 @@ def cos_sin_table(T: int, D: int, theta: float, device) -> torch.Tensor:
         with _tables_lock:
             tab = _tables.get(key)
             if tab is None:
-                ph = rope_phase(T, D, theta, device)
-                tab = torch.stack((ph.cos(), ph.sin()), -1).contiguous()
+                with torch.inference_mode(False), torch.no_grad():    # training may save a table that serving made
+                    ph = rope_phase(T, D, theta, device)
+                    tab = torch.stack((ph.cos(), ph.sin()), -1).contiguous()
                 if settled(tab):
                     _tables[key] = tab
     return tab

@@ -77,8 +77,9 @@ class RotaryTable:
         if max_positions < 1:
             raise ValueError(f"max_positions must be >= 1, got {max_positions}")
         freq, scale = rotary_frequencies(rotary_dim, theta, scaling, factor, original_positions)
-        phase = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * freq.to(device)
-        self.cos_sin = torch.stack((phase.cos() * scale, phase.sin() * scale), -1).float().contiguous()
+        with torch.inference_mode(False), torch.no_grad():    # training may save a table that serving made
+            phase = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] * freq.to(device)
+            self.cos_sin = torch.stack((phase.cos() * scale, phase.sin() * scale), -1).float().contiguous()
 
     @classmethod
     def from_cos_sin(cls, cos_sin: torch.Tensor) -> "RotaryTable":

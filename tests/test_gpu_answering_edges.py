@@ -1,0 +1,27 @@
+"""The decoder answering, in the ways around its plain run: grad modes, threads, prompts' forms."""
+import pytest
+import torch
+
+from continuum_attention_b200 import _native
+from continuum_attention_b200.decoder import ContinuumDecoderConfig, ContinuumDecoderLM
+
+pytestmark = pytest.mark.gpu
+
+
+def model(seed=0, **kw):
+    torch.manual_seed(seed)
+    cfg = ContinuumDecoderConfig(**{**dict(block_size=96, d_model=256, n_heads=4, n_layers=2), **kw})
+    return ContinuumDecoderLM(cfg).cuda()
+
+
+@pytest.mark.parametrize("kw", [dict(rope_theta=4321.0), dict(rope_theta=4321.0, rope_layout="half", rope_dim=32)])
+def test_generate_in_inference_mode_then_training(kw):
+    """The first use of a table is in inference mode, its second (a whole block) saves it for the gradient."""
+    m = model(**kw)
+    with torch.inference_mode():
+        a = m.generate([[1, 2, 3], [4]], 5)
+    ids = torch.arange(96, device="cuda")[None]
+    m(ids, ids)["loss"].backward()
+    assert all(torch.isfinite(p.grad).all() for p in m.parameters())
+    assert torch.equal(m.generate([[1, 2, 3], [4]], 5), a)
+    assert _native.lib().ca_device_status(0) == 0
