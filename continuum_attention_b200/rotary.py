@@ -10,7 +10,7 @@ key heads as query heads, positions 0 .. T-1).  Here:
   ``theta * factor ** (R / (R - 2))``, which keeps the fastest pair and divides the slowest
   by ``factor``; ``"yarn"`` (Peng et al., 2023) keeps pairs that turn more than 32 times
   within ``original_positions``, divides those that turn less than once by ``factor``, ramps
-  between, and scales cosine and sine by ``0.1 ln(factor) + 1``.
+  between (over the pairs' numbers, from whole pair to whole pair) and scales cosine and sine by ``0.1 ln(factor) + 1``.
 * ``rotary_qkv`` splits a projection output into turned q, k and v for training, with its
   gradient (``ca_rotary_qkv_forward`` / ``_backward``).
 * ``rotary_append`` turns new tokens at their cache positions and writes keys and values
@@ -61,7 +61,8 @@ def rotary_frequencies(rotary_dim: int, theta: float = 10000.0, scaling: Optiona
         def pair_of(turns):    # the (real) index of the pair that turns this often in the original length
             return R * math.log(original_positions / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-        low, high = max(math.floor(pair_of(32)), 0), min(math.ceil(pair_of(1)), R // 2 - 1)
+        # the upper end may lie behind the last pair, R / 2 - 1, which then turns more than once and is not divided whole
+        low, high = max(math.floor(pair_of(32)), 0), min(math.ceil(pair_of(1)), R - 1)
         ramp = ((torch.arange(R // 2, dtype=torch.float64) - low) / max(high - low, 1e-3)).clamp(0, 1)
         return freq / factor * ramp + freq * (1 - ramp), 0.1 * math.log(factor) + 1.0
     return freq, 1.0

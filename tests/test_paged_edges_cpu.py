@@ -1,12 +1,13 @@
 """Edges of the paged and rotary operators and of the decoder's answering that need no GPU."""
 import ctypes
+import math
 
 import pytest
 import torch
 
 from continuum_attention_b200 import RotaryTable, _native
 from continuum_attention_b200.rope import cos_sin_table
-from continuum_attention_b200.rotary import rotary_table
+from continuum_attention_b200.rotary import rotary_frequencies, rotary_table
 
 FAKE = ctypes.c_void_p(256)
 
@@ -50,3 +51,22 @@ def test_tables_first_made_in_inference_mode_serve_training(make):
     for table in (first, make()):
         _Saves.apply(x, table).sum().backward()
     assert x.grad.tolist() == [4.0] * 3
+
+
+# the ends of the ramp by hand: 20 and 33, 45 and 70, 4 and 8, 22 and 35, 8 and 21
+@pytest.mark.parametrize("R,original,factor,last", [
+    (64, 65536, 4.0, 1 - 11 / 13 * 3 / 4), (128, 131072, 4.0, 1 - 18 / 25 * 3 / 4), (16, 32768, 4.0, 1 - 3 / 4 * 3 / 4),
+    (64, 131072, 8.0, 1 - 9 / 13 * 7 / 8), (64, 2048, 8.0, 1 / 8)])
+def test_yarn_where_the_slowest_pair_turns_more_than_once(R, original, factor, last):
+    """What is left of each pair's frequency, from the ramp's two ends: the pairs (as real numbers) that turn 32
+    times and once within the original length, to whole pairs outwards, in 0 .. R - 1."""
+    plain, _ = rotary_frequencies(R)
+    freq, _ = rotary_frequencies(R, scaling="yarn", factor=factor, original_positions=original)
+    kept = (freq / plain).tolist()
+    # 10000^(-2 p / R) original / (2 pi) = turns
+    ends = [R / 2 * math.log10(original / (2 * math.pi * turns)) / 4 for turns in (32, 1)]
+    low, high = max(math.floor(ends[0]), 0), min(math.ceil(ends[1]), R - 1)
+    for p, k in enumerate(kept):
+        t = min(max((p - low) / (high - low), 0.0), 1.0)
+        assert k == pytest.approx(1 - t + t / factor, rel=1e-12)
+    assert kept[-1] == pytest.approx(last, rel=1e-9)
