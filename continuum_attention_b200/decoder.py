@@ -153,6 +153,9 @@ class ContinuumSelfAttention(nn.Module):
 
     def forward_paged(self, x, k_cache, v_cache, step: PagedStep, table: RotaryTable):
         """Packed new tokens x [N, C]: their keys and values go to the cache, their queries attend over it."""
+        if self.attention_fn is not continuum_attention:
+            raise ValueError("the cache is answered with continuum_attention: a model with another attention_fn has no "
+                             "paged form")
         layout = self.cfg.rope_layout if self.cfg is not None else "interleaved"
         q = rotary_append(self.qkv(x), k_cache, v_cache, step.page_table, step.kv_lens, step.q_starts, table,
                           heads=self.heads, layout=layout)

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from continuum_attention_b200 import RotaryTable, _native
+from continuum_attention_b200.decoder import ContinuumDecoderConfig, ContinuumDecoderLM
 from continuum_attention_b200.rope import cos_sin_table
 from continuum_attention_b200.rotary import rotary_frequencies, rotary_table
 
@@ -70,3 +71,16 @@ def test_yarn_where_the_slowest_pair_turns_more_than_once(R, original, factor, l
         t = min(max((p - low) / (high - low), 0.0), 1.0)
         assert k == pytest.approx(1 - t + t / factor, rel=1e-12)
     assert kept[-1] == pytest.approx(last, rel=1e-9)
+
+
+def small_decoder(**kw):
+    return ContinuumDecoderLM(ContinuumDecoderConfig(vocab_size=50, block_size=32, d_model=64, n_heads=2, n_layers=2), **kw)
+
+
+def test_a_model_with_another_attention_does_not_answer_with_the_default():
+    m = small_decoder(attention_fn=lambda q, k, v, gain, tile: v)
+    cache = m.make_cache(1)
+    with pytest.raises(ValueError, match="attention_fn"):
+        m.forward_paged(torch.tensor([1, 2]), cache, cache.step([2]))
+    with pytest.raises(ValueError, match="attention_fn"):
+        m.generate([[1, 2]], 2)
