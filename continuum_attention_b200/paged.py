@@ -15,9 +15,35 @@ from dataclasses import dataclass
 from typing import Optional, Sequence
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .attention import _DTYPE_CODE, on_device, raw_stream
+
+
+def refuse_gradients(what, *tensors):
+    """The serving operators drop no gradient without a word."""
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward; call it under torch.no_grad()")
+    refuse_tangents(what, *tensors)
+
+
+def refuse_tangents(what, *tensors):
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what} has no forward-mode gradient")
+
+
+class _NoBackward(torch.autograd.Function):
+    """An output of parameters that ask for a gradient: a backward pass through it says that there is none."""
+
+    @staticmethod
+    def forward(ctx, out, log_gain):
+        return out.view_as(out)
+
+    @staticmethod
+    def backward(ctx, grad):
+        raise RuntimeError("continuum_attention_paged has no backward, for log_gain neither; call it under "
+                           "torch.no_grad()")
 
 
 def check_cache(what, k_cache, v_cache, page_table, kv_lens, q_starts, dtype, device):
@@ -82,10 +108,13 @@ def continuum_attention_paged(q, k_cache, v_cache, page_table, kv_lens, q_starts
     ``q_starts[S]`` are left as they were in ``out`` (undefined without it).  Lengths and pages
     that are out of range give NaN rows and are recorded in the library's device status word.
     ``workspace`` (uint8, ``paged_workspace_bytes``) is allocated per call if not given; calls that
-    may overlap need one each.  Serving only: no gradient.
+    may overlap need one each.  Serving only: q and caches that require a gradient are refused outside
+    ``torch.no_grad()``; with a ``log_gain`` that does, a backward pass through the output raises.
     """
     if q.dim() != 3:
         raise ValueError(f"continuum_attention_paged expects q [N, H, D]; got {tuple(q.shape)}")
+    refuse_gradients("continuum_attention_paged", q, k_cache, v_cache)
+    refuse_tangents("continuum_attention_paged", log_gain)
     N, H, D = q.shape
     if q.dtype not in _DTYPE_CODE:
         raise TypeError(f"CA supports float32, bfloat16 and float16 inputs, not {q.dtype}")
@@ -99,8 +128,6 @@ def continuum_attention_paged(q, k_cache, v_cache, page_table, kv_lens, q_starts
         raise ValueError(f"log_gain must have shape [H]=[{H}], got {tuple(log_gain.shape)}")
     if int(max_q_len) < 1:
         raise ValueError(f"max_q_len must be >= 1, got {max_q_len}")
-    if torch.is_grad_enabled() and (q.requires_grad or k_cache.requires_grad or v_cache.requires_grad):
-        raise RuntimeError("continuum_attention_paged has no backward; call it under torch.no_grad()")
     lg = log_gain.detach()
     if lg.dtype != torch.float32 or lg.device != q.device or not lg.is_contiguous():
         lg = lg.to(device=q.device, dtype=torch.float32).contiguous()
@@ -135,7 +162,7 @@ def continuum_attention_paged(q, k_cache, v_cache, page_table, kv_lens, q_starts
             out.data_ptr(), workspace.data_ptr(), given, N, S, max_q_len, H, G, D, P, page, page_table.shape[1], code,
             raw_stream(q.device))
     _native.check("ca_paged_forward", st)
-    return out
+    return _NoBackward.apply(out, log_gain) if log_gain.requires_grad and torch.is_grad_enabled() else out
 
 
 @dataclass

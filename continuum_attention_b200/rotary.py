@@ -29,7 +29,7 @@ import torch
 
 from . import _native
 from .attention import _DTYPE_CODE, on_device, raw_stream
-from .paged import check_cache
+from .paged import check_cache, refuse_gradients
 from .rope import settled
 
 _LAYOUTS = {"interleaved": _native.CA_ROTARY_INTERLEAVED, "half": _native.CA_ROTARY_HALF}
@@ -236,12 +236,11 @@ def rotary_append(qkv: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     """
     if qkv.dim() != 2:
         raise ValueError(f"rotary_append expects qkv [N, width]; got {tuple(qkv.shape)}")
+    refuse_gradients("rotary_append", qkv, k_cache, v_cache, table.cos_sin)
     P, G, page, D = check_cache("rotary_append", k_cache, v_cache, page_table, kv_lens, q_starts, qkv.dtype,
                                 qkv.device)
     if _head_dim("rotary_append", qkv.shape[1], heads, G, qkv.dtype, qkv.device, table, layout) != D:
         raise ValueError(f"rotary_append: {qkv.shape[1]} values a token are not {heads} + 2 * {G} heads of {D}")
-    if torch.is_grad_enabled() and qkv.requires_grad:
-        raise RuntimeError("rotary_append has no backward; call it under torch.no_grad()")
     N = qkv.shape[0]
     if qkv.stride(1) != 1 or qkv.stride(0) < qkv.shape[1] or (qkv.stride(0) * qkv.element_size()) % 16 \
             or qkv.data_ptr() % 16:

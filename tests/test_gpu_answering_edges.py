@@ -2,8 +2,9 @@
 import pytest
 import torch
 
-from continuum_attention_b200 import _native
+from continuum_attention_b200 import _native, continuum_attention_paged
 from continuum_attention_b200.decoder import ContinuumDecoderConfig, ContinuumDecoderLM
+from paged_testlib import arguments, make_case
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +26,21 @@ def test_generate_in_inference_mode_then_training(kw):
     assert all(torch.isfinite(p.grad).all() for p in m.parameters())
     assert torch.equal(m.generate([[1, 2, 3], [4]], 5), a)
     assert _native.lib().ca_device_status(0) == 0
+
+
+def test_a_gain_that_asks_for_a_gradient():
+    """Its output is the same, and a backward pass through it says that there is none."""
+    c = make_case("bf16", 4, 2, 64, 16, [(1, 20), (2, 5)])
+    args = arguments(c)
+    plain = continuum_attention_paged(*args, max_q_len=2)
+    assert not plain.requires_grad
+    gain = args[6].clone().requires_grad_()
+    out = torch.empty_like(plain)
+    for kw in (dict(), dict(out=out)):
+        y = continuum_attention_paged(*args[:6], gain, max_q_len=2, **kw)
+        assert torch.equal(y.detach(), plain)
+        with pytest.raises(RuntimeError, match="no backward"):
+            (y.float().sum() + gain.sum()).backward()
+    assert torch.equal(out, plain)
+    with torch.no_grad():
+        assert not continuum_attention_paged(*args[:6], gain, max_q_len=2).requires_grad

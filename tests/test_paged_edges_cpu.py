@@ -5,10 +5,11 @@ import math
 import pytest
 import torch
 
-from continuum_attention_b200 import RotaryTable, _native
+from continuum_attention_b200 import RotaryTable, _native, continuum_attention_paged, rotary_append
 from continuum_attention_b200.decoder import ContinuumDecoderConfig, ContinuumDecoderLM
 from continuum_attention_b200.rope import cos_sin_table
 from continuum_attention_b200.rotary import rotary_frequencies, rotary_table
+from paged_testlib import arguments, make_case
 
 FAKE = ctypes.c_void_p(256)
 
@@ -84,3 +85,32 @@ def test_a_model_with_another_attention_does_not_answer_with_the_default():
         m.forward_paged(torch.tensor([1, 2]), cache, cache.step([2]))
     with pytest.raises(ValueError, match="attention_fn"):
         m.generate([[1, 2]], 2)
+
+
+def test_serving_operators_refuse_gradients():
+    c = make_case("bf16", 4, 2, 64, 16, [(1, 20), (2, 5)], device="cpu")
+    args = arguments(c)
+    qkv, table = torch.zeros(3, 8 * 64, dtype=torch.bfloat16), RotaryTable(64, 32, device="cpu")
+    for i in (0, 1, 2):
+        asks = [t.detach().requires_grad_() if j == i else t for j, t in enumerate(args)]
+        with pytest.raises(RuntimeError, match="no backward"):
+            continuum_attention_paged(*asks, max_q_len=2)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):       # as far as the device
+            continuum_attention_paged(*asks, max_q_len=2)
+    for x, cache in [(qkv.detach().requires_grad_(), args[1:6]),
+                     (qkv, [args[1].detach().requires_grad_(), *args[2:6]]),
+                     (qkv, [args[1], args[2].detach().requires_grad_(), *args[3:6]])]:
+        with pytest.raises(RuntimeError, match="no backward"):
+            rotary_append(x, *cache, table, heads=4)
+        with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):
+            rotary_append(x, *cache, table, heads=4)
+    with torch.autograd.forward_ad.dual_level():
+        for i in (0, 1, 2, 6):
+            dual = torch.autograd.forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no forward-mode"):
+                continuum_attention_paged(*args[:i], dual, *args[i + 1:], max_q_len=2)
+        dual = torch.autograd.forward_ad.make_dual(qkv, torch.ones_like(qkv))
+        with pytest.raises(RuntimeError, match="no forward-mode"):
+            rotary_append(dual, *args[1:6], table, heads=4)
+        with pytest.raises(RuntimeError, match="CUDA"):                          # plain inputs inside a level
+            continuum_attention_paged(*args, max_q_len=2)
