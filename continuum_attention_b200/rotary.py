@@ -204,11 +204,14 @@ def rotary_qkv(qkv: torch.Tensor, heads: int, table: RotaryTable, *, kv_heads: O
     """Split [B, T, (heads + 2 kv_heads) D] into turned q [B,heads,T,D], k and plain v [B,kv_heads,T,D].
 
     ``positions`` int32 [T] or [B,T] (default 0 .. T-1).  A position outside the table turns its
-    token's values into NaN and is recorded in the library's device status word.
+    token's values into NaN and is recorded in the library's device status word.  The gradient is
+    qkv's; the table is a constant.
     """
     kv_heads = heads if kv_heads is None else kv_heads
     if qkv.dim() != 3:
         raise ValueError(f"rotary_qkv expects [B, T, width]; got {tuple(qkv.shape)}")
+    if table.cos_sin.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError("rotary_qkv: the table is a constant and gets no gradient; detach its cos_sin")
     B, T, width = qkv.shape
     _head_dim("rotary_qkv", width, heads, kv_heads, qkv.dtype, qkv.device, table, layout)
     if positions is None:

@@ -5,7 +5,7 @@ import math
 import pytest
 import torch
 
-from continuum_attention_b200 import RotaryTable, _native, continuum_attention_paged, rotary_append
+from continuum_attention_b200 import RotaryTable, _native, continuum_attention_paged, rotary_append, rotary_qkv
 from continuum_attention_b200.decoder import ContinuumDecoderConfig, ContinuumDecoderLM
 from continuum_attention_b200.rope import cos_sin_table
 from continuum_attention_b200.rotary import rotary_frequencies, rotary_table
@@ -114,3 +114,12 @@ def test_serving_operators_refuse_gradients():
             rotary_append(dual, *args[1:6], table, heads=4)
         with pytest.raises(RuntimeError, match="CUDA"):                          # plain inputs inside a level
             continuum_attention_paged(*args, max_q_len=2)
+
+
+def test_rotary_qkv_refuses_a_table_that_asks_for_a_gradient():
+    qkv = torch.zeros(1, 3, 8 * 64)
+    table = RotaryTable.from_cos_sin(RotaryTable(64, 32, device="cpu").cos_sin.requires_grad_())
+    with pytest.raises(RuntimeError, match="table is a constant"):
+        rotary_qkv(qkv, 4, table, kv_heads=2)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):       # as far as the device
+        rotary_qkv(qkv, 4, table, kv_heads=2)
