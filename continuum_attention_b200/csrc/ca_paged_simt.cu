@@ -36,7 +36,7 @@ struct Config {
   static constexpr int TPR = NT / BR, KPT = TK / TPR;   // the moments: threads per row, keys per thread
   static constexpr int LD = DP + 4, LS = TK + 4;        // rows of tiles and of scores, on 16 bytes
   static constexpr int TILE = (TK + 1) * LD;            // floats; row TK is the halo
-  static constexpr int FLOATS = 4 * TILE + BR * LD + BR * LS + 4 * BR;
+  static constexpr int FLOATS = 4 * TILE + BR * LD + BR * LS + 2 * BR;
   static constexpr int SMEM = FLOATS * 4 + 3 * (TK + 1) * 8;   // and the prefix sums behind it
   static_assert(TPR >= 1 && 32 % TPR == 0 && CT % 2 == 0, "");
   static constexpr int VW = CT % 4 == 0 ? 4 : 2;        // output columns of one access
@@ -67,8 +67,7 @@ __global__ void __launch_bounds__(C::NT, C::PER_SM)
   float* sq = kv + 4 * C::TILE;                          // Q [BR][LD]
   float* ss = sq + BR * LD;                              // S, then P [BR][LS]
   float* row_f = ss + BR * LS;                           // per row: factor on O, then weight of the last key
-  float* row_m = row_f + BR;
-  float* row_z = row_m + BR;
+  float* row_z = row_f + BR;                             // its mass
   long long* offs = reinterpret_cast<long long*>(smem + C::FLOATS * 4);   // [3][TK + 1]: rows a-1 .. a+TK-1
   unsigned* prefix = reinterpret_cast<unsigned*>(smem + C::SMEM);
   const int tid = threadIdx.x, tr = tid / C::TC, tc = tid % C::TC;
@@ -364,7 +363,6 @@ __global__ void __launch_bounds__(C::NT, C::PER_SM)
       if (mpart == 0) {
         // a key beyond the row's own has no weight, and its V may hold anything
         row_f[mrow] = key <= pos ? carry_b + cap : 0.f;
-        row_m[mrow] = m;
         row_z[mrow] = zz;
         if (!whole && row0 + mrow < rows) part_mz[slot_row + mrow] = make_float2(m, zz);
       }

@@ -18,8 +18,8 @@ FAKE = ctypes.c_void_p(256)
 def test_page_sizes_beyond_32_bits(page):
     """A table without columns, so that no product with the page size is too large."""
     lib = _native.lib()
-    assert lib.ca_paged_forward(FAKE, 256, 64, FAKE, FAKE, 2048, 1024, 64, None, 0, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 40,
-                                4, 2, 2, 4, 2, 64, 16, page, 0, 1, None) == 2
+    assert lib.ca_paged_forward(FAKE, 256, 64, FAKE, FAKE, 2048, 1024, 64, None, 0, FAKE, FAKE, FAKE, FAKE, FAKE,
+                                1 << 40, 4, 2, 2, 4, 2, 64, 16, page, 0, 1, None) == 2
     assert "page_size" in lib.ca_last_error().decode()
     assert lib.ca_rotary_append(FAKE, 512, FAKE, FAKE, FAKE, FAKE, 2048, 1024, 64, None, 0, FAKE, FAKE, 4, 2, 4, 2, 64,
                                 64, 128, 16, page, 0, 0, 1, None) == 2
@@ -75,7 +75,8 @@ def test_yarn_where_the_slowest_pair_turns_more_than_once(R, original, factor, l
 
 
 def small_decoder(**kw):
-    return ContinuumDecoderLM(ContinuumDecoderConfig(vocab_size=50, block_size=32, d_model=64, n_heads=2, n_layers=2), **kw)
+    cfg = ContinuumDecoderConfig(vocab_size=50, block_size=32, d_model=64, n_heads=2, n_layers=2)
+    return ContinuumDecoderLM(cfg, **kw)
 
 
 def test_a_model_with_another_attention_does_not_answer_with_the_default():
