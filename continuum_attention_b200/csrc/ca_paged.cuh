@@ -73,6 +73,13 @@ int tc_groups(int dp);
 bool tc_launch(const Args& a, const Plan& plan, int dtype, const Pieces& pc, cudaError_t& e);
 cudaError_t tc_read_status(int* out, bool reset);
 
+// What merge_kernel does for a worker: nothing (pieces 0), join the pieces of a unit that starts in the worker's range
+// and goes on behind it, or (-1) give NaN to the rows of a launch that was refused, those of the sequences
+// with `start` to `rows` rows.
+struct Meta {
+  int pieces, slot, start, rows, h, rt;
+};
+
 // Prefix sums of the sequences' places in shared memory (all threads of the block take part in the
 // constructor), and cursors into the stream of tiles: sequence, key head, row tile, key tile.
 template <int BR, int TK>
@@ -158,8 +165,9 @@ struct Schedule {
         carry = __shfl_sync(0xffffffffu, v, 31);
       }
       if (lane == 0) {
-        prefix[0] = 0;
-        if (carry >= 0x7fffffffull) {    // more tiles than the stream's index holds: no answer at all
+        const bool refused = carry >= 0x7fffffffull;   // more tiles than the stream's index holds: none is done
+        prefix[0] = refused;
+        if (refused) {
           record_invalid();
           prefix[a.seqs] = 0;
         }
@@ -168,6 +176,9 @@ struct Schedule {
     __syncthreads();
     total = prefix[a.seqs];
   }
+
+  // a worker's record before it has any tile: the join reads it of every worker, also of one whose wait gave up
+  __device__ __forceinline__ Meta none() const { return Meta{-(int)prefix[0], 0, plan.row_lo, plan.row_hi, 0, 0}; }
 
   __device__ __forceinline__ void enter(Cursor& c) const {   // a new sequence
     load(c.s, c.start, c.n, c.len, c.bad);
@@ -262,11 +273,6 @@ __device__ __forceinline__ void store2(T* p, float x, float y) {
 // exponentials are 0.  (Finite, since infinities would meet as NaN.)
 constexpr float kMasked = -1e30f;
 
-// a worker whose unit goes on behind its range: what merge_kernel joins
-struct Meta {
-  int pieces, slot, start, rows, h, rt;
-};
-
 // Joins the pieces of a cut unit: piece 0 is in this worker's slot, the others are the first pieces of the
 // workers that follow.  A block takes up to 4 W rows of a unit, a warp four of them; where rows are fewer than
 // warps, several warps share a row's pieces, each sums its own in order, and then the warps' sums are added
@@ -317,6 +323,21 @@ static __global__ void __launch_bounds__(W * 32) merge_kernel(const __grid_const
   const int row0 = second ? 0 : (int)blockIdx.x % slices * RB;   // of the unit
   const Meta mt = pc.meta[w];
   if (mt.pieces == 0) return;
+  if (mt.pieces < 0) {
+    // more tiles than the stream's index holds: no row of the launch is left as it was
+    const int blocks = second ? two.workers : one.workers * slices;
+    const int block = second ? w : (int)blockIdx.x;
+    for (int s = 0; s < a.seqs; ++s) {
+      const int start = a.q_starts[s], end = a.q_starts[s + 1];
+      if (start < 0 || end > a.rows || start > end) continue;
+      const int rows = (end - start) * group;
+      if (rows < mt.start || rows > mt.rows) continue;
+      const size_t last = (size_t)end * a.H * a.D;
+      for (size_t x = (size_t)start * a.H * a.D + block * blockDim.x + threadIdx.x; x < last; x += blocks * blockDim.x)
+        ((T*)a.o)[x] = from_f32<T>(__int_as_float(0x7fffffff));
+    }
+    return;
+  }
   const int nrows = min(min(BR, mt.rows - mt.rt * BR) - row0, RB);
   if (nrows <= 0) return;
   int share = 1;                                     // warps per row

@@ -236,9 +236,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
       if (after_chunks) pdl_wait();
       return;
     }
-    // nothing to join, until the range's last tile says otherwise: the join reads this of every worker, and one
-    // whose wait gives up writes no more
-    if (lane == 0) meta[worker].pieces = 0;
+    if (lane == 0) meta[worker] = sched.none();
     // `cur` stands at the next tile to be described; a tile's pages are fetched when it is described, one tile
     // before its copies are issued.  Every instruction here counts: the producer shares a scheduler with
     // the consumers.

@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(C::NT, C::PER_SM)
   cur.at = x1;
   if (x0 < x1) cur = sched.locate(x0);
   if (cur.at >= x1) {
-    if (tid == 0) meta[worker].pieces = 0;
+    if (tid == 0) meta[worker] = sched.none();
     return;
   }
 

@@ -144,9 +144,7 @@ __device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const
                                           Meta* __restrict__ meta) {
   const int lane = threadIdx.x & 31;
   volatile int* ab = &ct.gave_up;
-  // nothing to join, until the range's last tile says otherwise: the join reads this of every worker, and one
-  // whose wait gives up writes no more
-  if (lane == 0) meta[worker].pieces = 0;
+  if (lane == 0) meta[worker] = sched.none();
   typename Schedule<BR, TK>::Cursor cur;
   cur.at = x1;
   if (x0 < x1) cur = sched.locate(x0);

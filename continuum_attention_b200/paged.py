@@ -106,7 +106,9 @@ def continuum_attention_paged(q, k_cache, v_cache, page_table, kv_lens, q_starts
 
     A row at a negative position (more rows than keys) sees nothing and gives zeros.  Rows behind
     ``q_starts[S]`` are left as they were in ``out`` (undefined without it).  Lengths and pages
-    that are out of range give NaN rows and are recorded in the library's device status word.
+    that are out of range give NaN rows and are recorded in the library's device status word, and so
+    do calls of more tiles (16 to 128 rows of a key head by 32 or 64 keys) than 2^31, as in a prompt of
+    a million tokens of 16 key heads.
     ``workspace`` (uint8, ``paged_workspace_bytes``) is allocated per call if not given; calls that
     may overlap need one each.  Serving only: q and caches that require a gradient are refused outside
     ``torch.no_grad()``; with a ``log_gain`` that does, a backward pass through the output raises.

@@ -297,8 +297,8 @@ int ca_rotary_qkv_backward(const void* dq, const void* dk, const void* dv, const
  * (q_starts has num_seqs + 1 entries), and kv_lens counts them: row n sits at position
  * kv_lens[s] - (q_starts[s+1] - n).  Rows behind q_starts[num_seqs] are left as they
  * were.  kv_lens, q_starts and page_table are int32 on the device; entries of the page
- * table that no key needs are never used; a row of it covers 2^30 keys at most.  A page outside 0 .. num_pages-1, a length
- * beyond pages_per_seq * page_size, or rows outside the buffers are recorded in
+ * table that no key needs are never used; a page has 2^30 slots and a row of the table covers
+ * 2^30 keys at most.  A page outside 0 .. num_pages-1, a length beyond pages_per_seq * page_size, or rows outside the buffers are recorded in
  * ca_device_status() as CA_ERR_INVALID_ARGUMENT; nothing is read or written there.
  *
  * ca_rotary_append: turns the new tokens' queries and keys at their positions (as
@@ -321,7 +321,8 @@ int ca_rotary_append(const void* qkv, int64_t qkv_stride, const float* cos_sin, 
  * negative position gives zeros.  q rows are q_token_stride and heads q_head_stride elements
  * apart; o is [num_rows][heads][D].  The rows of a sequence whose length is out of range, and
  * those that see a page out of range, come out NaN (see above; other rows of that sequence
- * may).  Keys and values behind a sequence's length, and pages that no sequence holds, may
+ * may), and so do a call's rows where its tiles (16 to 128 rows of a key head by 32 or 64 keys)
+ * are 2^31 or more, as in a prompt of a million tokens of 16 key heads.  Keys and values behind a sequence's length, and pages that no sequence holds, may
  * hold anything; a value that is not finite reaches the rows that see it, and may reach
  * earlier rows of the same call and sequence (0 times it is NaN).  How a row's sum is cut
  * depends on the other sequences of the call, so its last bit may; the same call gives the
