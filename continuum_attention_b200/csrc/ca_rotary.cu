@@ -227,7 +227,9 @@ __global__ void append_kernel(const __grid_constant__ AppendArgs a) {
   __syncthreads();
   for (int s = threadIdx.x; s < a.seqs; s += blockDim.x) {
     const int start = a.q_starts[s], end = a.q_starts[s + 1], len = a.kv_lens[s];
-    if (start > n || n >= end) continue;
+    const bool outside = start < 0 || end > a.tokens || start > end;   // rows that the buffers do not have
+    if (outside && n == 0) record_invalid();
+    if (outside || start > n || n >= end) continue;
     const long long p = (long long)len - end + n;
     long long cache = -1;
     if (p >= 0 && p < a.table_rows) {

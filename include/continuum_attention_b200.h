@@ -305,6 +305,7 @@ int ca_rotary_qkv_backward(const void* dq, const void* dk, const void* dv, const
  * ca_rotary_qkv_forward), writes q [num_rows][heads][D] and writes keys and values into
  * the cache.  A row at a negative position (more rows than keys) writes no key and a q
  * of zeros; a row whose position or page is out of range writes no key and a q of NaN.
+ * A sequence with rows outside the buffers writes nothing.
  * No two rows may share a slot.  One launch, no allocation.
  */
 int ca_rotary_append(const void* qkv, int64_t qkv_stride, const float* cos_sin, void* q, void* k_cache,
