@@ -311,11 +311,17 @@ class ContinuumDecoderLM(nn.Module):
     @torch.no_grad()
     def generate(self, prompts, max_new_tokens: int, *, temperature: float = 0.0, generator=None,
                  page_size: int = 64):
-        """Continue each prompt (1-D ids, of any lengths) by ``max_new_tokens`` tokens; returns their new ids
-        [len(prompts), max_new_tokens].  temperature 0 takes the likeliest token, else tokens are drawn.  The
-        prompts run as one packed step, then every step of one token a sequence replays one CUDA graph."""
+        """Continue each prompt (1-D ids, of any lengths; a [B, T] tensor is B of them) by ``max_new_tokens``
+        tokens; returns their new ids [len(prompts), max_new_tokens].  temperature 0 takes the likeliest token,
+        else tokens are drawn.  The prompts run as one packed step, then every step of one token a sequence
+        replays one CUDA graph."""
+        prompts = [torch.as_tensor(p) for p in prompts]
+        if any(p.dim() != 1 for p in prompts):
+            raise ValueError("generate takes 1-D prompts (or a tensor of one prompt a row)")
         if not prompts or min(len(p) for p in prompts) < 1 or max_new_tokens < 1:
             raise ValueError("generate needs prompts of one token at least and max_new_tokens >= 1")
+        if any(p.is_floating_point() or p.is_complex() for p in prompts):
+            raise ValueError("generate takes prompts of whole numbers")
         if temperature < 0:
             raise ValueError("temperature must be >= 0")
         with torch.cuda.device_of(self.lm_head.weight):      # graphs are captured on the current device
@@ -332,12 +338,14 @@ class ContinuumDecoderLM(nn.Module):
                 return logits.argmax(-1)
             return torch.multinomial((logits.float() / temperature).softmax(-1), 1, generator=generator).squeeze(-1)
 
+        packed = torch.cat([p.to(torch.long) for p in prompts])
+        if packed.min() < 0 or packed.max() >= self.cfg.vocab_size:
+            raise ValueError(f"prompts have ids outside 0 .. {self.cfg.vocab_size - 1}")
         keys = [n + max_new_tokens - 1 for n in lens]
         cache = self.make_cache(len(prompts), pages=sum(-(-n // page_size) for n in keys), page_size=page_size)
         cache.reserve(keys)
         step = cache.step(lens)
-        packed = torch.cat([torch.as_tensor(p, dtype=torch.long).flatten() for p in prompts]).to(device)
-        logits = self.forward_paged(packed, cache, step)
+        logits = self.forward_paged(packed.to(device), cache, step)
         out = torch.empty(len(prompts), max_new_tokens, dtype=torch.long, device=device)
         ids = pick(logits[step.q_starts[1:].long() - 1])
         out[:, 0] = ids

@@ -124,3 +124,19 @@ def test_rotary_qkv_refuses_a_table_that_asks_for_a_gradient():
         rotary_qkv(qkv, 4, table, kv_heads=2)
     with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA"):       # as far as the device
         rotary_qkv(qkv, 4, table, kv_heads=2)
+
+
+def test_prompts_in_every_form():
+    """A tensor of prompts is one prompt a row; a prompt of another shape and ids that the embedding does not have (a
+    read behind it) are refused before anything runs."""
+    m = small_decoder()
+    for bad, match in (([[1, 50]], "0 .. 49"), ([[1], [-1]], "0 .. 49"), (torch.full((2, 3), 50), "0 .. 49"),
+                       ([torch.tensor([[1, 2]])], "1-D"), (torch.tensor([1, 2]), "1-D"), ([[]], "one token"),
+                       (torch.zeros(0, 3, dtype=torch.long), "one token"), ([[1.5]], "whole"),
+                       (torch.zeros(2, 31), "whole")):
+        with pytest.raises(ValueError, match=match):
+            m.generate(bad, 2)
+    for good in (torch.zeros(2, 3, dtype=torch.long), [(1, 2), [3]], [torch.tensor([49]), [0, 1]],
+                 torch.zeros(2, 3, dtype=torch.uint8).numpy()):
+        with pytest.raises(RuntimeError, match="CUDA"):                        # as far as the device
+            m.generate(good, 2)
