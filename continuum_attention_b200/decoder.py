@@ -322,7 +322,7 @@ class ContinuumDecoderLM(nn.Module):
             raise ValueError("generate needs prompts of one token at least and max_new_tokens >= 1")
         if any(p.is_floating_point() or p.is_complex() for p in prompts):
             raise ValueError("generate takes prompts of whole numbers")
-        if temperature < 0:
+        if not temperature >= 0:
             raise ValueError("temperature must be >= 0")
         with torch.cuda.device_of(self.lm_head.weight):      # graphs are captured on the current device
             return self._generate(prompts, max_new_tokens, temperature, generator, page_size)

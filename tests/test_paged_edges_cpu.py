@@ -140,3 +140,8 @@ def test_prompts_in_every_form():
                  torch.zeros(2, 3, dtype=torch.uint8).numpy()):
         with pytest.raises(RuntimeError, match="CUDA"):                        # as far as the device
             m.generate(good, 2)
+
+
+def test_temperature_that_is_no_number():
+    with pytest.raises(ValueError, match="temperature"):
+        small_decoder().generate([[1]], 2, temperature=float("nan"))
