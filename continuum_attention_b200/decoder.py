@@ -289,9 +289,10 @@ class ContinuumDecoderLM(nn.Module):
         dtype = weight.dtype
         if weight.is_cuda and torch.is_autocast_enabled("cuda"):
             dtype = torch.get_autocast_dtype("cuda")
-        return PagedKVCache(cfg.n_layers, pages or max_seqs * -(-cfg.block_size // page_size), page_size, cfg.n_heads,
-                            cfg.d_model // cfg.n_heads, max_seqs=max_seqs, max_len=cfg.block_size, dtype=dtype,
-                            device=weight.device)
+        if pages is None:
+            pages = max_seqs * -(-cfg.block_size // max(page_size, 1))
+        return PagedKVCache(cfg.n_layers, pages, page_size, cfg.n_heads, cfg.d_model // cfg.n_heads, max_seqs=max_seqs,
+                            max_len=cfg.block_size, dtype=dtype, device=weight.device)
 
     @torch.no_grad()
     def forward_paged(self, input_ids, cache: PagedKVCache, step: PagedStep):

@@ -145,3 +145,10 @@ def test_prompts_in_every_form():
 def test_temperature_that_is_no_number():
     with pytest.raises(ValueError, match="temperature"):
         small_decoder().generate([[1]], 2, temperature=float("nan"))
+
+
+def test_a_cache_of_no_pages_is_refused():
+    """It is not the default number of pages."""
+    with pytest.raises(ValueError, match="pages"):
+        small_decoder().make_cache(2, pages=0)
+    assert small_decoder().make_cache(2, page_size=16).free_pages == 4
