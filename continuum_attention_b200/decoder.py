@@ -24,6 +24,7 @@ replay.  The ``rope_*`` options beyond theta select the general rotary positions
 from __future__ import annotations
 
 import math
+import threading
 from dataclasses import dataclass
 from typing import Callable, Optional
 
@@ -40,6 +41,9 @@ from .rmsnorm import supported as native_rms_norm_supported
 from .paged import PagedKVCache, PagedStep, continuum_attention_paged
 from .rope import apply_rope_torch, cos_sin_table, rope_qkv
 from .rotary import RotaryTable, rotary_append, rotary_frequencies, rotary_qkv, rotary_table
+
+# One capture at a time, and no draw meanwhile: the default generator belongs to the graph until it ends.
+_capture_lock = threading.Lock()
 
 
 @dataclass
@@ -337,7 +341,8 @@ class ContinuumDecoderLM(nn.Module):
         def pick(logits):
             if temperature == 0:
                 return logits.argmax(-1)
-            return torch.multinomial((logits.float() / temperature).softmax(-1), 1, generator=generator).squeeze(-1)
+            with _capture_lock:
+                return torch.multinomial((logits.float() / temperature).softmax(-1), 1, generator=generator).squeeze(-1)
 
         packed = torch.cat([p.to(torch.long) for p in prompts])
         if packed.min() < 0 or packed.max() >= self.cfg.vocab_size:
@@ -362,7 +367,8 @@ class ContinuumDecoderLM(nn.Module):
             self.forward_paged(ids, cache, step)         # kernels and workspaces of the libraries, outside the graph
         torch.cuda.current_stream(device).wait_stream(side)
         graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(graph):
+        # (thread_local: other threads may allocate and copy meanwhile)
+        with _capture_lock, torch.cuda.graph(graph, stream=side, capture_error_mode="thread_local"):
             logits = self.forward_paged(ids, cache, step)
         for i in range(1, max_new_tokens):
             graph.replay()                               # (the warm-up wrote the same keys to the same slots)

@@ -1,4 +1,6 @@
 """The decoder answering, in the ways around its plain run: grad modes, threads, prompts' forms."""
+import threading
+
 import pytest
 import torch
 
@@ -44,3 +46,45 @@ def test_a_gain_that_asks_for_a_gradient():
     assert torch.equal(out, plain)
     with torch.no_grad():
         assert not continuum_attention_paged(*args[:6], gain, max_q_len=2).requires_grad
+
+
+@pytest.mark.parametrize("temperature", [0.0, 1.0])
+def test_generate_in_two_threads(temperature):
+    """A capture in one thread bears the other's launches, allocations, copies and draws."""
+    m = model(seed=2)
+    prompts = [[[1, 2, 3], [4] * 20], [[7] * 9]]
+    want = [m.generate(p, 12, page_size=16) for p in prompts]
+    barrier, got, errors = threading.Barrier(2), [[], []], []
+
+    def work(t):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(4):
+                    barrier.wait(60)
+                    got[t].append(m.generate(prompts[t], 12, page_size=16, temperature=temperature))
+                torch.cuda.current_stream().synchronize()
+        except BaseException as e:
+            errors.append(e)
+            barrier.abort()
+
+    threads = [threading.Thread(target=work, args=(t,)) for t in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors
+    for t in range(2):
+        assert len(got[t]) == 4
+        for g in got[t]:
+            assert g.shape == want[t].shape and ((g >= 0) & (g < 256)).all()
+            if temperature == 0:
+                assert torch.equal(g, want[t])
+    assert _native.lib().ca_device_status(0) == 0
+
+
+def test_prompts_as_a_tensor():
+    m = model(seed=5)
+    ids = torch.arange(12).view(3, 4)
+    want = m.generate([p.tolist() for p in ids], 6)
+    for form in (ids, ids.cuda(), ids.to(torch.uint8), ids.numpy(), list(ids.cuda())):
+        assert torch.equal(m.generate(form, 6), want)
