@@ -106,16 +106,26 @@ _tables = {}
 _tables_lock = threading.Lock()
 
 
+def _capturing(device: torch.device) -> bool:
+    if device.type != "cuda":
+        return False
+    with torch.cuda.device(device):
+        return torch.cuda.is_current_stream_capturing()
+
+
 def rotary_table(rotary_dim: int, max_positions: int, theta: float, scaling: Optional[str], factor: float,
                  original_positions: Optional[int], device) -> RotaryTable:
     """The ``RotaryTable`` of these settings, made once per device; not while a CUDA graph is captured."""
+    device = torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
     key = (rotary_dim, max_positions, float(theta), scaling, float(factor), original_positions, str(device))
     table = _tables.get(key)
     if table is None:
         with _tables_lock:
             table = _tables.get(key)
             if table is None:
-                if torch.device(device).type == "cuda" and torch.cuda.is_current_stream_capturing():
+                if _capturing(device):
                     raise RuntimeError("rotary_table: the table of these settings has to be made before a CUDA graph "
                                        "that uses it is captured (one call outside does)")
                 table = RotaryTable(rotary_dim, max_positions, theta=theta, scaling=scaling, factor=factor,

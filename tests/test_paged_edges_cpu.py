@@ -5,7 +5,8 @@ import math
 import pytest
 import torch
 
-from continuum_attention_b200 import RotaryTable, _native, continuum_attention_paged, rotary_append, rotary_qkv
+from continuum_attention_b200 import (RotaryTable, _native, continuum_attention_paged, rotary, rotary_append,
+                                      rotary_qkv)
 from continuum_attention_b200.decoder import ContinuumDecoderConfig, ContinuumDecoderLM
 from continuum_attention_b200.rope import cos_sin_table
 from continuum_attention_b200.rotary import rotary_frequencies, rotary_table
@@ -152,3 +153,22 @@ def test_a_cache_of_no_pages_is_refused():
     with pytest.raises(ValueError, match="pages"):
         small_decoder().make_cache(2, pages=0)
     assert small_decoder().make_cache(2, page_size=16).free_pages == 4
+
+
+def test_tables_of_the_current_device_are_of_that_device(monkeypatch):
+    """"cuda" without a number is another device after a switch: not the table that was made for the first."""
+    made = []
+
+    class Fake:
+        def __init__(self, *a, device, **kw):
+            made.append(torch.device(device))
+            self.cos_sin = torch.zeros(1, 1, 2)
+
+    monkeypatch.setattr(rotary, "RotaryTable", Fake)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(rotary, "_capturing", lambda device: False, raising=False)
+    for current in (0, 1, 0):
+        monkeypatch.setattr(torch.cuda, "current_device", lambda: current)
+        for device in ("cuda", torch.device("cuda"), f"cuda:{current}"):
+            rotary.rotary_table(8, 9, 1234.0, None, 1.0, None, device)
+    assert made == [torch.device("cuda", 0), torch.device("cuda", 1)]
