@@ -598,8 +598,9 @@ int ca_paged_forward(const void* q, int64_t q_token_stride, int64_t q_head_strid
   if (num_seqs > ca::paged::kMaxSeqs)
     return fail(CA_ERR_UNSUPPORTED, "%s: %lld sequences in one call, at most %d are covered", fn, (long long)num_seqs,
                 ca::paged::kMaxSeqs);
-  if (heads > (1LL << 20) || num_rows > 0x7fffffffLL / heads)
-    return fail(CA_ERR_UNSUPPORTED, "%s: num_rows * heads = %lld * %lld exceeds 2^31-1", fn, (long long)num_rows,
+  // (whole tiles of rows are counted in 32 bits)
+  if (heads > (1LL << 20) || num_rows > (0x80000000LL - 1024) / heads)
+    return fail(CA_ERR_UNSUPPORTED, "%s: num_rows * heads = %lld * %lld exceeds 2^31-1024", fn, (long long)num_rows,
                 (long long)heads);
   const int64_t esz = dtype == CA_DTYPE_F32 ? 4 : 2;
   if (q_token_stride < 0 || q_head_stride < 0 || q_token_stride * esz % 16 || q_head_stride * esz % 16)

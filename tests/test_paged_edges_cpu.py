@@ -172,3 +172,12 @@ def test_tables_of_the_current_device_are_of_that_device(monkeypatch):
         for device in ("cuda", torch.device("cuda"), f"cuda:{current}"):
             rotary.rotary_table(8, 9, 1234.0, None, 1.0, None, device)
     assert made == [torch.device("cuda", 0), torch.device("cuda", 1)]
+
+
+def test_as_many_rows_as_32_bits_index():
+    """Rows are counted in whole tiles of 128: a call of nearly 2^31 would pass the index."""
+    lib = _native.lib()
+    for rows, heads in ((2 ** 31 - 2, 1), (2 ** 31 - 512, 1), ((2 ** 31 - 1) // 3, 3)):
+        assert lib.ca_paged_forward(FAKE, 8, 8, FAKE, FAKE, 8, 8, 8, FAKE, 8, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 40, rows, 1,
+                                    1, heads, heads, 8, 16, 16, 8, 1, None) == 2
+        assert "2^31-1024" in lib.ca_last_error().decode()
