@@ -90,7 +90,7 @@ class RotaryTable:
             raise ValueError("cos_sin must be float32 [positions, R/2, 2]; got "
                              f"{cos_sin.dtype} {tuple(cos_sin.shape)}")
         self = cls.__new__(cls)
-        self.cos_sin = cos_sin.contiguous()
+        self.cos_sin = _aligned(cos_sin.contiguous())
         return self
 
     @property

@@ -181,3 +181,12 @@ def test_as_many_rows_as_32_bits_index():
         assert lib.ca_paged_forward(FAKE, 8, 8, FAKE, FAKE, 8, 8, 8, FAKE, 8, FAKE, FAKE, FAKE, FAKE, FAKE, 1 << 40, rows, 1,
                                     1, heads, heads, 8, 16, 16, 8, 1, None) == 2
         assert "2^31-1024" in lib.ca_last_error().decode()
+
+
+def test_a_table_that_starts_anywhere():
+    """The kernels read tables from 16-byte borders on: a slice that starts between two is copied."""
+    full = RotaryTable(6, 40, device="cpu").cos_sin
+    for first in range(4):
+        table = RotaryTable.from_cos_sin(full[first:])
+        assert table.cos_sin.data_ptr() % 16 == 0 and torch.equal(table.cos_sin, full[first:])
+    assert RotaryTable.from_cos_sin(full).cos_sin.data_ptr() == full.data_ptr()
