@@ -88,3 +88,16 @@ def test_prompts_as_a_tensor():
     want = m.generate([p.tolist() for p in ids], 6)
     for form in (ids, ids.cuda(), ids.to(torch.uint8), ids.numpy(), list(ids.cuda())):
         assert torch.equal(m.generate(form, 6), want)
+
+
+@pytest.mark.parametrize("autocast", [False, True])
+def test_a_step_without_tokens(autocast):
+    m = model(seed=6)
+    with torch.autocast("cuda", dtype=torch.bfloat16, enabled=autocast):
+        cache = m.make_cache(2, page_size=16)
+        first = m.forward_paged(torch.tensor([1, 2, 3], device="cuda"), cache, cache.step([3, 0]))
+        kept = cache.k.clone()
+        none = m.forward_paged(torch.zeros(0, dtype=torch.long, device="cuda"), cache, cache.step([0, 0]))
+    assert first.shape == (3, 256) and none.shape == (0, 256)
+    assert torch.equal(cache.k, kept) and cache.lens == [3, 0]
+    assert _native.lib().ca_device_status(0) == 0
