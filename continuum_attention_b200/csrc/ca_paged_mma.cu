@@ -29,8 +29,10 @@
 // then has the pair (j-1, j-1 + NJ) as its left neighbours, every step of the moments is one
 // packed f32x2 instruction for two keys, and neighbours in other lanes are needed once per
 // run.  The weights leave as A fragments with the same dealing of V rows.  Each weight is
-// split into two 16-bit parts (hi + lo, 16 bits or more): one rounding to bf16 would put
-// 1.1e-3 of the output's size on every row.  With 8 rows or fewer hi and lo are the two
+// split into two 16-bit parts (hi + lo: 16 bits in bf16, 21 in f16): one rounding to bf16 would put
+// 1.1e-3 of the output's size on every row.  Against weights in 32 bits, 2 to 5 of a thousand bf16 outputs, and 2 of
+// a hundred f16 ones, are another rounding of a value that lies within 7e-5 of the outputs' size from the border
+// (prompts of 2 x 2048 tokens, 511 rows over 16001 keys); the error against 64 bits is the same to three digits.  With 8 rows or fewer hi and lo are the two
 // halves of one fragment and cost one product.
 //
 // Shared memory.  The eight rows of a fragment lie NJ rows apart, so every NJ rows are
@@ -39,10 +41,11 @@
 // else one copy per row.
 //
 // What bounds it.  Decoding reads every visible key's K and V once and is bound by that: 2 sequences
-// over 90001 .. 131071 keys (f16, 32 heads on 8 of 64, pages of 16) 90 us for 506 MB, 5.6 TB/s; 17
-// sequences of 1 .. 4 rows over up to 20000 keys (bf16, 32 heads on 8 of 128) 98 us for 484 MB, 4.9 TB/s;
-// 64 sequences over 1 .. 8192 keys (bf16, 16 heads of 64) 50 us for 231 MB, 4.6 TB/s; a single
-// sequence of 2048 keys is all latency, 12 us (launch, page look-ups, one round of copies, the join).
+// over 90001 .. 131071 keys (f16, 32 heads on 8 of 64, pages of 16) 97 us for 506 MB, 5.2 TB/s (on the
+// same inputs again, some of them still in L2, 91); 17 sequences of 1 .. 4 rows over up to 20000 keys (bf16, 32
+// heads on 8 of 128) 98 us for 484 MB, 4.9 TB/s; 64 sequences over 1 .. 8192 keys (bf16, 16 heads of 64) 51 us for
+// 231 MB, 4.5 TB/s; a single sequence of 2048 keys is all latency, 13 us (launch, page look-ups, one round of
+// copies, the join).
 // Chunks are bound by the scalar work and its dependences (885 issue slots a warp for 1024 scores, 40% of
 // the cycles issue); those of more than 64 rows are ca_paged_tc.cu's.
 #include <algorithm>
@@ -724,8 +727,8 @@ cudaError_t launch_main(const Args& a, Plan plan, const Pieces& pc, bool after_c
 }
 
 // 128-row units on tcgen05 (ca_paged_tc.cu) where the longest sequence fills more than half of one; else units of 64
-// rows on mma.sync.  16 heads of 64, tcgen05 against mma.sync: 16 sequences of 64 rows over 4096 keys 173 and 136 us,
-// of 80 rows 174 and 251; 1 of 128 rows over 16000 keys 77 and 81; 4 pieces of 256 rows over 512 keys 35 and 31.
+// rows on mma.sync.  16 heads of 64, tcgen05 against mma.sync: 16 sequences of 64 rows over 4096 keys 173 and 139 us,
+// of 80 rows 178 and 251; 1 of 128 rows over 16000 keys 77 and 81; 4 pieces of 256 rows over 512 keys 35 and 31.
 // Heads of 128: 80 rows 270 and 372, 128 rows 99 and 116, 256 rows 43 and 47.
 bool use_tc(long long rows) { return rows > 64; }
 

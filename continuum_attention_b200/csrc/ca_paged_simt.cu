@@ -6,9 +6,13 @@
 // Tiles arrive by cp.async, one ahead, gathered row by row through the page table, V one
 // row early so that the weights of keys a-1 .. a+TK-2 meet it where they lie.
 //
+// Exponentials and reciprocals are the special-function unit's (2^-22 of the value, and e^x another |x| 2^-24 of
+// its argument's rounding), all sums are in 32 bits: outputs of short prompts are 2.7e-7 of their norm from 64 bits,
+// where torch's exp and division in 32 bits leave 3.6e-7; of decoding 3.9e-8 against 3.7e-8.
+//
 // What bounds it: decoding reads 2 D f32 values a key and key head and comes to 70% of the copy
-// rate, held by the latency of a tile's three steps at ten warps an SM; chunks are bound by the FMA pipe and the shared-memory reads that feed it
-// (scores: 6 16-byte reads for 32 FMAs of a thread; P V: 8 for 64).  8 prompts of 40 .. 192 tokens
+// rate, held by the latency of a tile's three steps at ten warps an SM; chunks are bound by the FMA pipe and the
+// shared-memory reads that feed it (scores: 6 16-byte reads for 32 FMAs of a thread; P V: 8 for 64).  8 prompts of 40 .. 192 tokens
 // (4 heads of 64) take 25 us, nearly all of it latency: launch, a unit's few tiles, the join.
 #include "ca_paged.cuh"
 
@@ -413,7 +417,7 @@ __global__ void __launch_bounds__(C::NT, C::PER_SM)
 }
 
 // Rows of a unit: 4 or 16 for decoding, 64 for chunks.  In the decoding forms a warp's lanes are the tile's 32
-// keys, then its output columns.  64 sequences of one row over 8192 keys (16 heads of 64): units of 4 rows 955 us
+// keys, then its output columns.  64 sequences of one row over 8192 keys (16 heads of 64): units of 4 rows 958 us
 // (4.5 TB/s; on one warp 1220, on four 1050), of 16 rows 3230; 16 rows over 4096 keys (16 sequences, 32 heads on
 // 2 of 64): 46 us, with threads in 16 x 8 75.  Prompts of 2 x 1024 tokens, 16 heads of 128: 371 us in 8 x 32, 395 in
 // 16 x 16, which is better with 64 values (2 x 2048 tokens 639 and 708).

@@ -33,10 +33,10 @@
 // against 189 us at that case), tiles of 48 keys (189 against 170), four workers with 96 registers a thread
 // (216) or with one warp for products and copies (220), one such warp for each of three workers (187
 // against 179).
-// Measured (16 heads of 64): prompts of 2 x 2048 tokens 112 us (mma.sync form 148), 511 rows over
-// 16001 keys 171 us (235), 23 sequences of 0 .. 300 rows over up to 4000 keys, 4 query heads a key
-// head, 82 us (102).  Heads of 128, with two workers and one unit's queries at a time: the first two 169 (226)
-// and 259 us (352).
+// Measured (16 heads of 64): prompts of 2 x 2048 tokens 115 us (mma.sync form 148), 511 rows over
+// 16001 keys 173 us (235), 23 sequences of 0 .. 300 rows over up to 4000 keys, 4 query heads a key
+// head, 84 us (102).  Heads of 128, with two workers and one unit's queries at a time: the first two 171 (226)
+// and 262 us (352).
 #include <cuda.h>
 
 #include <numeric>

@@ -12,8 +12,8 @@
 //
 // HBM-bound: each element of [tokens][H + 2G][D] is read once and written once: 8 x 2048 tokens of 48
 // heads of 64 in bf16 take 34.5 us forward and 36.6 backward for 201 MB each (5.8 and 5.5 TB/s), 1731 tokens
-// of 20 heads in f32 3.9 and 4.3 us, 1540 tokens of 48 heads of 128 into a cache 8.7 us for 38 MB, the
-// 64 tokens of a decoding step 2.8 us (latency).  An item
+// of 20 heads in f32 3.9 and 4.3 us, 1540 tokens of 48 heads of 128 into a cache 8.8 us for 38 MB (14 where
+// nothing of it is in L2), the 64 tokens of a decoding step 2.8 us (latency; 4.1).  An item
 // is two vectors of W elements of one head: the two that a turn in halves combines, else
 // two adjacent ones.  A thread keeps its item for several heads, so that it reads the
 // table once, and loads kHeads heads before it stores the first.
