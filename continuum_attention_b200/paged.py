@@ -38,7 +38,8 @@ class _NoBackward(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, out, log_gain):
-        return out.view_as(out)
+        ctx.mark_dirty(out)      # not a view: it may be changed in place
+        return out
 
     @staticmethod
     def backward(ctx, grad):
@@ -164,7 +165,7 @@ def continuum_attention_paged(q, k_cache, v_cache, page_table, kv_lens, q_starts
             out.data_ptr(), workspace.data_ptr(), given, N, S, max_q_len, H, G, D, P, page, page_table.shape[1], code,
             raw_stream(q.device))
     _native.check("ca_paged_forward", st)
-    return _NoBackward.apply(out, log_gain) if log_gain.requires_grad and torch.is_grad_enabled() else out
+    return _NoBackward.apply(out.detach(), log_gain) if log_gain.requires_grad and torch.is_grad_enabled() else out
 
 
 @dataclass

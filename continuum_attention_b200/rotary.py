@@ -10,7 +10,8 @@ key heads as query heads, positions 0 .. T-1).  Here:
   ``theta * factor ** (R / (R - 2))``, which keeps the fastest pair and divides the slowest
   by ``factor``; ``"yarn"`` (Peng et al., 2023) keeps pairs that turn more than 32 times
   within ``original_positions``, divides those that turn less than once by ``factor``, ramps
-  between (over the pairs' numbers, from whole pair to whole pair) and scales cosine and sine by ``0.1 ln(factor) + 1``.
+  between (over the pairs' numbers, from whole pair to whole pair) and scales cosine and sine by
+  ``0.1 ln(factor) + 1``.
 * ``rotary_qkv`` splits a projection output into turned q, k and v for training, with its
   gradient (``ca_rotary_qkv_forward`` / ``_backward``).
 * ``rotary_append`` turns new tokens at their cache positions and writes keys and values

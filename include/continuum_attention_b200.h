@@ -298,8 +298,9 @@ int ca_rotary_qkv_backward(const void* dq, const void* dk, const void* dv, const
  * kv_lens[s] - (q_starts[s+1] - n).  Rows behind q_starts[num_seqs] are left as they
  * were.  kv_lens, q_starts and page_table are int32 on the device; entries of the page
  * table that no key needs are never used; a page has 2^30 slots and a row of the table covers
- * 2^30 keys at most.  A page outside 0 .. num_pages-1, a length beyond pages_per_seq * page_size, or rows outside the buffers are recorded in
- * ca_device_status() as CA_ERR_INVALID_ARGUMENT; nothing is read or written there.
+ * 2^30 keys at most.  A page outside 0 .. num_pages-1, a length beyond pages_per_seq *
+ * page_size, or rows outside the buffers are recorded in ca_device_status() as
+ * CA_ERR_INVALID_ARGUMENT; nothing is read or written there.
  *
  * ca_rotary_append: turns the new tokens' queries and keys at their positions (as
  * ca_rotary_qkv_forward), writes q [num_rows][heads][D] and writes keys and values into
@@ -316,23 +317,22 @@ int ca_rotary_append(const void* qkv, int64_t qkv_stride, const float* cos_sin, 
                      int64_t pages_per_seq, int layout, int dtype, void* stream);
 
 /*
- * Continuum Attention of new tokens over the paged cache, for serving (no gradient): row n
- * of query head h attends to the keys at positions 0 .. its own of key head
- * h / (heads / kv_heads), with the scores, trajectories and caps of ca_forward.  A row at a
- * negative position gives zeros.  q rows are q_token_stride and heads q_head_stride elements
- * apart; o is [num_rows][heads][D].  The rows of a sequence whose length is out of range, and
- * those that see a page out of range, come out NaN (see above; other rows of that sequence
- * may), and so do a call's rows where its tiles (16 to 128 rows of a key head by 32 or 64 keys)
- * are 2^31 or more, as in a prompt of a million tokens of 16 key heads.  Keys and values behind a sequence's length, and pages that no sequence holds, may
- * hold anything; a value that is not finite reaches the rows that see it, and may reach
- * earlier rows of the same call and sequence (0 times it is NaN).  How a row's sum is cut
- * depends on the other sequences of the call, so its last bit may; the same call gives the
- * same bits every time.  max_q_len is the number of new
- * tokens of the longest sequence, by which the kernel is chosen; a wrong one costs time only.
- * heads a multiple of kv_heads; D a multiple of 8, at most 128; at most 2048 sequences; every
- * buffer and stride a multiple of 16 bytes (o and q included).  workspace holds
- * ca_paged_workspace_size() bytes (256-byte aligned; its contents are ignored, and it
- * belongs to this call until the call's GPU work has finished).
+ * Continuum Attention of new tokens over the paged cache, for serving (no gradient): row n of
+ * query head h attends to the keys at positions 0 .. its own of key head h / (heads / kv_heads),
+ * with the scores, trajectories and caps of ca_forward. A row at a negative position gives zeros.
+ * q rows are q_token_stride and heads q_head_stride elements apart; o is [num_rows][heads][D]. The
+ * rows of a sequence whose length is out of range, and those that see a page out of range, come
+ * out NaN (see above; other rows of that sequence may), and so do a call's rows where its tiles
+ * (16 to 128 rows of a key head by 32 or 64 keys) are 2^31 or more, as in a prompt of a million
+ * tokens of 16 key heads. Keys and values behind a sequence's length, and pages that no sequence
+ * holds, may hold anything; a value that is not finite reaches the rows that see it, and may reach
+ * earlier rows of the same call and sequence (0 times it is NaN). How a row's sum is cut depends
+ * on the other sequences of the call, so its last bit may; the same call gives the same bits every
+ * time. max_q_len is the number of new tokens of the longest sequence, by which the kernel is
+ * chosen; a wrong one costs time only. heads a multiple of kv_heads; D a multiple of 8, at most
+ * 128; at most 2048 sequences; every buffer and stride a multiple of 16 bytes (o and q included).
+ * workspace holds ca_paged_workspace_size() bytes (256-byte aligned; its contents are ignored, and
+ * it belongs to this call until the call's GPU work has finished).
  */
 size_t ca_paged_workspace_size(int64_t num_seqs, int64_t max_q_len, int64_t heads, int64_t kv_heads, int64_t D,
                                int dtype);
@@ -375,8 +375,9 @@ int ca_selftest_wait_timeout(int64_t limit_us, void* stream);
  * Diagnostics (no reference counterpart): the limit of the device-side waits in the
  * ca_paged_forward calls that this thread makes from here on, in microseconds (at most 1e7;
  * negative: the ordinary two seconds; 0: in bf16 and f16, where copies are awaited, every worker
- * that has more tiles than fit its shared memory gives up).  A call whose wait gives up records CA_ERR_DEVICE_TIMEOUT, leaves the rows of o that it did not come to
- * undefined, writes nothing but o and its workspace, and ends in order.
+ * that has more tiles than fit its shared memory gives up).  A call whose wait gives up records
+ * CA_ERR_DEVICE_TIMEOUT, leaves the rows of o that it did not come to undefined, writes nothing
+ * but o and its workspace, and ends in order.
  */
 int ca_selftest_paged_wait_limit(int64_t limit_us);
 

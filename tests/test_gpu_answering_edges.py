@@ -41,6 +41,8 @@ def test_a_gain_that_asks_for_a_gradient():
     for kw in (dict(), dict(out=out)):
         y = continuum_attention_paged(*args[:6], gain, max_q_len=2, **kw)
         assert torch.equal(y.detach(), plain)
+        assert y.data_ptr() == kw.get("out", y).data_ptr() and not out.requires_grad
+        y += 0.0
         with pytest.raises(RuntimeError, match="no backward"):
             (y.float().sum() + gain.sum()).backward()
     assert torch.equal(out, plain)
