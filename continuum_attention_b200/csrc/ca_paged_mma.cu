@@ -103,6 +103,14 @@ __device__ __forceinline__ bool room_wait(uint32_t bar, uint32_t parity, volatil
   *gave_up = 1;
   return false;
 }
+// a wait that no other warp's giving up ends (whole warp)
+__device__ __forceinline__ void bar_drain(uint32_t bar, uint32_t parity) {
+  unsigned long long t0, t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t0));
+  do asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  while (!bar_try(bar, parity) && t - t0 < kWaitNs);
+  __syncwarp();
+}
 template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -394,8 +402,7 @@ __global__ void __launch_bounds__(C::THREADS, 1)
     if (!end) describe();
   }
   // every copy has to land before this block's shared memory is another's, where the consumers gave up too
-  volatile int go = 0;
-  for (int u = max(k - NST, 0); u < k; ++u) bar_wait(full + 8 * (u % NST), (u / NST) & 1, &go, kWaitNs);
+  for (int u = max(k - NST, 0); u < k; ++u) bar_drain(full + 8 * (u % NST), (u / NST) & 1);
   if (after_chunks) pdl_wait();
   return;
   }

@@ -112,6 +112,12 @@ __device__ __forceinline__ bool mbar_test_warp(uint64_t* bar, uint32_t parity) {
                "selp.u32 %0, 1, 0, p;\n\t}" : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
   return __all_sync(0xffffffffu, done != 0);
 }
+// a wait that no other warp's giving up ends; whole warp
+__device__ __forceinline__ void mbar_drain_warp(uint64_t* bar, uint32_t parity) {
+  const unsigned long long t0 = globaltimer_ns();
+  while (!mbar_try_wait(bar, parity) && globaltimer_ns() - t0 < kWaitNs) {}
+  __syncwarp();
+}
 // the loader's wait for room: with no limit at all it gives up at once, so that a call can be made to; whole warp
 __device__ __forceinline__ bool room_wait_warp(uint64_t* bar, uint32_t parity, volatile int* gave_up,
                                                unsigned long long limit_ns) {
@@ -286,8 +292,7 @@ __device__ __forceinline__ void load_warp(const Args& a, const Plan& plan, const
     before = behind;
   }
   // every copy has to land before this block's shared memory is another's
-  volatile int go = 0;
-  for (int u = max(t - NST, 0); u < t; ++u) mbar_wait_warp(&ct.full[u % NST], (u / NST) & 1, &go);
+  for (int u = max(t - NST, 0); u < t; ++u) mbar_drain_warp(&ct.full[u % NST], (u / NST) & 1);
 }
 
 // ------------------------------------------------------------------ the issuer
@@ -356,9 +361,8 @@ __device__ __forceinline__ void issue_warp(const Plan& plan, typename C::Group& 
   if (issued > 0) {
     // products may still be running where a wait gave up, the math warps' or this one's: they end before tensor
     // memory is given back
-    volatile int go = 0;
     mma_commit(&ct.drained);
-    mbar_wait_warp(&ct.drained, 0, &go);
+    mbar_drain_warp(&ct.drained, 0);
   }
 }
 
